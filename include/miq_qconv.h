@@ -433,6 +433,89 @@ int miq_bmm_i32(const int32_t* A, const int32_t* B, int32_t* C, int32_t batch, i
 void bmm_matmul_i32(const int32_t* A, const int32_t* B, int32_t* C, int batch, int M, int N, int K,
                     int trans_a, int trans_b);
 
+/* ---- training of token networks: embedding, activations kept in 8 bits ---------------- */
+/* No reference counterpart: the first layer of a network over tokens (its rows are NHWC pixels of
+ * one channel vector each), and what its training step keeps between the forward and the backward
+ * pass.  Rows are dense along channels; `ld_*` is the distance between rows in elements and is
+ * at least the row's length.  No entry point allocates device memory; those that need a workspace
+ * take the caller's (16-byte aligned, not shared by calls in flight together).  Every
+ * call gives the same bits for the same inputs.  Inputs and outputs do not overlap. */
+
+/* Element types.  Sums, scales and activations are computed in fp32; a bf16 output is rounded
+ * once, to nearest even. */
+typedef enum miq_dtype {
+  MIQ_F32 = 0,
+  MIQ_BF16 = 1,
+  MIQ_I32 = 2, /* token ids only */
+  MIQ_I64 = 3  /* token ids only */
+} miq_dtype;
+
+/* y[t, :] = scale * table[ids[t], :] for t < tokens.  A row whose id lies outside [0, vocab) is
+ * zeros (a position without a token).  table: vocab x c of table_type; ids: id_type; y: tokens x c
+ * of y_type.  Negative extents, vocab above 2^28, c above 2^29, tokens above 2^31 - 65 and row
+ * distances shorter than a row are rejected; tokens == 0 or c == 0 enqueues nothing. */
+int miq_embed_fprop(const void* table, const void* ids, void* y, int64_t vocab, int32_t c, int64_t tokens,
+                    int64_t ld_table, int64_t ld_y, float scale, int32_t table_type, int32_t id_type, int32_t y_type,
+                    void* stream);
+
+/* Bytes of device workspace miq_embed_grad needs (no GPU access). */
+int miq_embed_grad_workspace_size(int64_t vocab, int32_t c, int64_t tokens, size_t* bytes);
+
+/* The table's gradient: d[v, :] = scale * (sum of dy[t, :] over the t with ids[t] == v), the tokens
+ * of a row added in an order that depends on the ids alone.  accumulate == 0 overwrites the whole
+ * table (rows without a token are zeros); accumulate != 0 adds to dtable and touches only the rows
+ * that have a token.  Ids outside [0, vocab) contribute nothing.  dy: tokens x c of dy_type;
+ * dtable: vocab x c of dtable_type. */
+int miq_embed_grad(const void* dy, const void* ids, void* dtable, int64_t vocab, int32_t c, int64_t tokens,
+                   int64_t ld_dy, int64_t ld_dtable, float scale, int32_t accumulate, int32_t dy_type, int32_t id_type,
+                   int32_t dtable_type, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The 8-bit form of a tensor of rows x c values: int8 codes, rows x c, and exponent bytes, rows x
+ * ceil(c / 32), both dense.  Each group of 32 channels of a row (the last may be shorter) has one
+ * exponent byte b, and a value stands for code * 2^(b - 127), |code| <= 127 (exact in bf16).  With E
+ * and m the exponent and mantissa fields of the group's largest magnitude in fp32, b = E - 6, one
+ * more where m >= 0x7F0000 (where the code would round to 128), held to [1, 248]; codes round to
+ * nearest even.  The error of a value is at most 1/127 of its group's largest magnitude, or
+ * 2^-127 in a group below 2^-120.  A group that holds an infinity or a NaN has b = 255 and
+ * codes 0, and stands for NaN.
+ * `gated` rows hold a gate of c values and then c values that it multiplies: 2c codes and
+ * 2 * ceil(c / 32) exponent bytes a row, the halves grouped apart. */
+
+typedef enum miq_act {
+  MIQ_ACT_NONE = 0,
+  MIQ_ACT_RELU = 1,
+  MIQ_ACT_SILU = 2, /* v / (1 + exp(-v)) */
+  MIQ_ACT_GELU = 3  /* v * (1 + erf(v / sqrt 2)) / 2 */
+} miq_act;
+
+/* y = act(x), or act(gate) * up for gated rows, and x kept in 8 bits, in one pass.  x: rows x c
+ * (rows x 2c gated) of `type`; y: rows x c of `type`, or NULL to keep x only; codes, scales: as
+ * above.  c up to 2^29, rows up to 2^40 and up to 2^46 values. */
+int miq_act8_fprop(const void* x, void* y, int8_t* codes, uint8_t* scales, int64_t rows, int32_t c, int64_t ld_x,
+                   int64_t ld_y, int32_t act, int32_t gated, int32_t type, void* stream);
+
+/* The activation's backward pass at the kept values x': dx = dy * act'(x'), or, gated, the row
+ * [dy * up' * act'(gate'), dy * act(gate')].  dy: rows x c, dx: rows x c (2c gated), of `type`. */
+int miq_act8_bprop(const void* dy, const int8_t* codes, const uint8_t* scales, void* dx, int64_t rows, int32_t c,
+                   int64_t ld_dy, int64_t ld_dx, int32_t act, int32_t gated, int32_t type, void* stream);
+
+/* The kept values themselves (MIQ_ACT_NONE, not gated), or the activation of them recomputed:
+ * y = act(x') or act(gate') * up'.  y: rows x c of `type`. */
+int miq_act8_expand(const int8_t* codes, const uint8_t* scales, void* y, int64_t rows, int32_t c, int64_t ld_y,
+                    int32_t act, int32_t gated, int32_t type, void* stream);
+
+/* Bytes of device workspace miq_act8_grad needs (no GPU access). */
+int miq_act8_grad_workspace_size(int64_t rows, int32_t c, int32_t k, int32_t dy_type, size_t* bytes);
+
+/* The weight gradient of a linear (1x1) layer from its input kept in 8 bits (not gated):
+ * dw[j, i] = sum over m of dy[m, j] * x'[m, i], j < k, i < c; accumulate != 0 adds it to dw.
+ * On bf16 matrix instructions, which hold x' exactly: bf16 dy directly, fp32 dy split into three
+ * bf16 numbers each, sums in fp32.  dy: rows x k of dy_type; dw: k x c of dw_type (MIQ_F32, or
+ * MIQ_BF16 where dy is).  rows up to 2^31 - 65, c and k up to 2^22; rows == 0 gives zeros. */
+int miq_act8_grad(const void* dy, const int8_t* codes, const uint8_t* scales, void* dw, int64_t rows, int32_t c,
+                  int32_t k, int64_t ld_dy, int64_t ld_dw, int32_t accumulate, int32_t dy_type, int32_t dw_type,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -105,6 +105,7 @@ assert C.sizeof(QParamsU8) == 12 and C.sizeof(QParamsS5) == 8
 
 _P = C.c_void_p
 _I = C.c_int32
+_L = C.c_int64
 _PI = C.POINTER(C.c_int32)
 
 # name -> (restype, argtypes); every function declared in include/miq_qconv.h
@@ -152,7 +153,21 @@ SIGNATURES = {
         C.c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, C.POINTER(BlockConv2DParams), _P, _I, _I, _P]),
     "miq_plan_f32_split": (C.c_int, [_I, _I, _I, _I, _I, _I, _I, _I, C.POINTER(BlockConv2DParams), _PI]),
     "miq_plan_block_f32": (C.c_int, [_I, _I, _I, _I, _I, _I, _I, _I, C.POINTER(BlockConv2DParams), _I, _PI]),
+    "miq_embed_fprop": (C.c_int, [_P, _P, _P, _L, _I, _L, _L, _L, C.c_float, _I, _I, _I, _P]),
+    "miq_embed_grad_workspace_size": (C.c_int, [_L, _I, _L, C.POINTER(C.c_size_t)]),
+    "miq_embed_grad": (
+        C.c_int, [_P, _P, _P, _L, _I, _L, _L, _L, C.c_float, _I, _I, _I, _I, _P, C.c_size_t, _P]),
+    "miq_act8_fprop": (C.c_int, [_P, _P, _P, _P, _L, _I, _L, _L, _I, _I, _I, _P]),
+    "miq_act8_bprop": (C.c_int, [_P, _P, _P, _P, _L, _I, _L, _L, _I, _I, _I, _P]),
+    "miq_act8_expand": (C.c_int, [_P, _P, _P, _L, _I, _L, _I, _I, _I, _P]),
+    "miq_act8_grad_workspace_size": (C.c_int, [_L, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    "miq_act8_grad": (
+        C.c_int, [_P, _P, _P, _P, _L, _I, _I, _L, _L, _I, _I, _I, _P, C.c_size_t, _P]),
 }
+
+# miq_dtype, miq_act: element types and activations of the token-network entry points
+MIQ_F32, MIQ_BF16, MIQ_I32, MIQ_I64 = 0, 1, 2, 3
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 _lib = None
 

@@ -43,6 +43,11 @@ SOURCES = [
     "qconv_qi32.hip",
     "qconv_qi32_band.hip",
     "qconv_qi32_route.hip",
+    "train_capi.cpp",
+    "embed.hip",
+    "embed_grad.hip",
+    "act8.hip",
+    "act8_grad.hip",
     "conv_quant_host.cpp",
     "verify.cpp",
     "bench.cpp",

@@ -1,0 +1,243 @@
+// Activations whose input is kept in 8 bits (miq_act8_fprop, _bprop, _expand).
+//
+// Every kernel is one pass over its tensors.  A lane holds eight consecutive channels, so four
+// neighbouring lanes share one exponent byte; a row's chunks are padded to whole groups, which
+// keeps those four lanes in one row whatever the row's length.
+#include "train_device.h"
+
+namespace miq {
+namespace {
+
+constexpr int kThreads = 256;
+
+enum Act : int { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
+
+// act(v).  NaN stays NaN.
+template <int ACT>
+__device__ __forceinline__ float act_of(float v) {
+  if constexpr (ACT == kRelu) return v < 0.0f ? 0.0f : v;
+  if constexpr (ACT == kSilu) return v / (1.0f + expf(-v));
+  if constexpr (ACT == kGelu) return 0.5f * v * erfcf(v * -0.70710678118654752f);
+  return v;
+}
+
+// act'(v); 0 at relu's corner.
+template <int ACT>
+__device__ __forceinline__ float slope_of(float v) {
+  if constexpr (ACT == kRelu) return v > 0.0f ? 1.0f : (v <= 0.0f ? 0.0f : v);
+  if constexpr (ACT == kSilu) {
+    const float s = 1.0f / (1.0f + expf(-v));
+    return s * (1.0f + v * (1.0f - s));
+  }
+  if constexpr (ACT == kGelu)
+    return 0.5f * erfcf(v * -0.70710678118654752f) + v * expf(-0.5f * v * v) * 0.39894228040143268f;
+  return 1.0f;
+}
+
+struct Rows {
+  int64_t total;     // chunks of eight channels, rows padded to whole groups
+  int64_t ld_x, ld_dy, ld_y;
+  int c, per_row;    // per_row = 4 * groups
+  FastDivM div;      // by per_row
+};
+
+// (row, channel, channels left) of this thread's chunk; false past the end
+__device__ __forceinline__ bool place(const Rows& r, int64_t block, int64_t* row, int* chunk, int* left) {
+  const int64_t base = block * kThreads;
+  const int64_t row0 = base / r.per_row;  // the workgroup's, one division
+  const int at = static_cast<int>(base - row0 * r.per_row) + threadIdx.x;
+  const int over = fdiv(at, r.div);
+  *row = row0 + over;
+  *chunk = at - over * r.per_row;
+  *left = r.c - *chunk * 8;
+  return base + threadIdx.x < r.total;
+}
+
+// The exponent byte of a group, from its largest magnitude (as fp32 bits) in all four lanes.
+__device__ __forceinline__ int exponent_byte(unsigned top) {
+  const int e = static_cast<int>(top >> 23) - 6 + ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0);
+  return top >= 0x7f800000u ? 255 : min(max(e, 1), 248);
+}
+
+// Keeps eight values: codes at `codes`, the group's byte at `scale` (by its first lane).
+__device__ __forceinline__ void keep8(const v8f& v, int left, int8_t* codes, uint8_t* scale) {
+  unsigned top = 0;  // magnitudes order as their bits do, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 1)));
+  top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 2)));
+  const int byte = exponent_byte(top);
+  // 2^(127 - byte), a normal number for every byte below 254; zero codes where the group is not finite
+  const float inverse = byte == 255 ? 0.0f : __uint_as_float(static_cast<unsigned>(254 - byte) << 23);
+  v8c q;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float s = byte == 255 ? 0.0f : v[i] * inverse;  // exact, or below half a code
+    q[i] = static_cast<signed char>(static_cast<int>(__builtin_rintf(fminf(fmaxf(s, -127.0f), 127.0f))));
+  }
+  if (left >= 8) {
+    *reinterpret_cast<v8c_any*>(codes) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) codes[i] = q[i];
+  }
+  if ((threadIdx.x & 3) == 0) *scale = static_cast<uint8_t>(byte);
+}
+
+__device__ __forceinline__ v8f kept8(const int8_t* codes, const uint8_t* scale, int left) {
+  v8c q = {};
+  if (left >= 8) {
+    q = *reinterpret_cast<const v8c_any*>(codes);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) q[i] = codes[i];
+  }
+  // byte 255 is the bits of infinity, which a zero code makes NaN
+  return __builtin_convertvector(q, v8f) * __uint_as_float(static_cast<unsigned>(*scale) << 23);
+}
+
+template <typename T, int ACT, bool GATED>
+__global__ __launch_bounds__(kThreads) void act8_fprop_kernel(Rows r, const T* __restrict__ x, T* __restrict__ y,
+                                                              int8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  constexpr int H = GATED ? 2 : 1;
+  for (int64_t b = blockIdx.x; b * kThreads < r.total; b += gridDim.x) {
+    int64_t row;
+    int chunk, left;
+    if (!place(r, b, &row, &chunk, &left)) continue;  // whole groups of lanes leave together
+    const int groups = r.per_row >> 2;
+    v8f v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int col = h * r.c + chunk * 8;
+      v[h] = load8_of(x + row * r.ld_x + col, left);
+      keep8(v[h], left, codes + row * (H * static_cast<int64_t>(r.c)) + col,
+            scales + (row * H + h) * groups + (chunk >> 2));
+    }
+    if (y != nullptr) {
+      v8f out;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
+      store8_of(y + row * r.ld_y + chunk * 8, out, left);
+    }
+  }
+}
+
+template <typename T, int ACT, bool GATED>
+__global__ __launch_bounds__(kThreads) void act8_bprop_kernel(Rows r, const T* __restrict__ dy,
+                                                              const int8_t* __restrict__ codes,
+                                                              const uint8_t* __restrict__ scales, T* __restrict__ dx) {
+  constexpr int H = GATED ? 2 : 1;
+  for (int64_t b = blockIdx.x; b * kThreads < r.total; b += gridDim.x) {
+    int64_t row;
+    int chunk, left;
+    if (!place(r, b, &row, &chunk, &left) || left <= 0) continue;
+    const int groups = r.per_row >> 2;
+    const v8f d = load8_of(dy + row * r.ld_dy + chunk * 8, left);
+    v8f v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      v[h] = kept8(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + chunk * 8,
+                   scales + (row * H + h) * groups + (chunk >> 2), left);
+    v8f g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = d[i] * (GATED ? v[H - 1][i] : 1.0f) * slope_of<ACT>(v[0][i]);
+    store8_of(dx + row * r.ld_y + chunk * 8, g, left);
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = d[i] * act_of<ACT>(v[0][i]);
+      store8_of(dx + row * r.ld_y + r.c + chunk * 8, g, left);
+    }
+  }
+}
+
+template <typename T, int ACT, bool GATED>
+__global__ __launch_bounds__(kThreads) void act8_expand_kernel(Rows r, const int8_t* __restrict__ codes,
+                                                               const uint8_t* __restrict__ scales, T* __restrict__ y) {
+  constexpr int H = GATED ? 2 : 1;
+  for (int64_t b = blockIdx.x; b * kThreads < r.total; b += gridDim.x) {
+    int64_t row;
+    int chunk, left;
+    if (!place(r, b, &row, &chunk, &left) || left <= 0) continue;
+    const int groups = r.per_row >> 2;
+    v8f v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      v[h] = kept8(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + chunk * 8,
+                   scales + (row * H + h) * groups + (chunk >> 2), left);
+    v8f out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
+    store8_of(y + row * r.ld_y + chunk * 8, out, left);
+  }
+}
+
+Rows rows_of(const Act8Args& a) {
+  Rows r{};
+  const int64_t groups = (static_cast<int64_t>(a.c) + kAct8Group - 1) / kAct8Group;
+  r.per_row = static_cast<int>(4 * groups);
+  r.total = a.rows * r.per_row;
+  r.ld_x = a.ld_x;
+  r.ld_dy = a.ld_dy;
+  r.ld_y = a.ld_y;
+  r.c = a.c;
+  r.div = fastdiv_m(static_cast<uint32_t>(r.per_row));
+  return r;
+}
+
+// Calls go(type, act, gated) with the three as compile-time values.
+template <typename F>
+void dispatch(const Act8Args& a, F&& go) {
+  auto by_gate = [&](auto type, auto act) {
+    a.gated ? go(type, act, std::true_type{}) : go(type, act, std::false_type{});
+  };
+  auto by_act = [&](auto type) {
+    switch (a.act) {
+      case kRelu: by_gate(type, std::integral_constant<int, kRelu>{}); break;
+      case kSilu: by_gate(type, std::integral_constant<int, kSilu>{}); break;
+      case kGelu: by_gate(type, std::integral_constant<int, kGelu>{}); break;
+      default: by_gate(type, std::integral_constant<int, kNone>{}); break;
+    }
+  };
+  a.bf16 ? by_act(__bf16{}) : by_act(float{});
+}
+
+unsigned blocks_of(const Rows& r) {
+  const int64_t blocks = (r.total + kThreads - 1) / kThreads;
+  return static_cast<unsigned>(blocks < (1 << 23) ? blocks : (1 << 23));
+}
+
+}  // namespace
+
+hipError_t launch_act8_fprop(const Act8Args& a, hipStream_t stream) {
+  const Rows r = rows_of(a);
+  dispatch(a, [&](auto type, auto act, auto gated) {
+    using T = decltype(type);
+    act8_fprop_kernel<T, act.value, gated.value><<<blocks_of(r), kThreads, 0, stream>>>(
+        r, static_cast<const T*>(a.x), static_cast<T*>(a.y), a.codes, a.scales);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_act8_bprop(const Act8Args& a, hipStream_t stream) {
+  const Rows r = rows_of(a);
+  dispatch(a, [&](auto type, auto act, auto gated) {
+    using T = decltype(type);
+    act8_bprop_kernel<T, act.value, gated.value><<<blocks_of(r), kThreads, 0, stream>>>(
+        r, static_cast<const T*>(a.dy), a.codes, a.scales, static_cast<T*>(a.y));
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_act8_expand(const Act8Args& a, hipStream_t stream) {
+  const Rows r = rows_of(a);
+  dispatch(a, [&](auto type, auto act, auto gated) {
+    using T = decltype(type);
+    act8_expand_kernel<T, act.value, gated.value><<<blocks_of(r), kThreads, 0, stream>>>(
+        r, a.codes, a.scales, static_cast<T*>(a.y));
+  });
+  return hipGetLastError();
+}
+
+}  // namespace miq

@@ -400,6 +400,14 @@ int i8_entry(miq::Epi epi, const miq_qconv_desc* d, const int8_t* x, const int8_
 
 }  // namespace
 
+int miq::record_error(int status, const char* msg) noexcept {
+  try {
+    return fail(status, msg);
+  } catch (...) {  // no memory for the text: the status alone
+    return status;
+  }
+}
+
 extern "C" {
 
 int miq_version(void) { return MIQ_VERSION; }

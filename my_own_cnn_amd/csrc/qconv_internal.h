@@ -12,6 +12,9 @@ struct miq_conv2d_params;  // include/miq_qconv.h
 
 namespace miq {
 
+// Keeps `msg` as the calling thread's last error and returns `status` (qconv_capi.cpp).
+int record_error(int status, const char* msg) noexcept;
+
 // Validated geometry of one grouped 2-D convolution, NHWC input / KRSC filter.
 struct Geom {
   int N, H, W, C;      // input

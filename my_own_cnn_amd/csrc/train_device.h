@@ -1,0 +1,66 @@
+// Device helpers shared by the token-network kernels: eight consecutive values of a row as fp32,
+// and the 8-bit form of a group of channels.
+#pragma once
+
+#include "qconv_device.h"
+#include "train_internal.h"
+
+namespace miq {
+namespace {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef float v8f __attribute__((ext_vector_type(8)));
+typedef signed char v8c __attribute__((ext_vector_type(8)));
+// Rows start at any multiple of the element's size: global memory takes 16-byte accesses at any
+// address, so odd row lengths run the same loads and stores as aligned ones.
+typedef v8bf v8bf_any __attribute__((aligned(2)));
+typedef v4f v4f_any __attribute__((aligned(4)));
+typedef v8c v8c_any __attribute__((aligned(1)));
+
+__device__ __forceinline__ v8f load8(const float* p) {
+  const v4f a = *reinterpret_cast<const v4f_any*>(p), b = *reinterpret_cast<const v4f_any*>(p + 4);
+  return v8f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+__device__ __forceinline__ v8f load8(const __bf16* p) {
+  return __builtin_convertvector(*reinterpret_cast<const v8bf_any*>(p), v8f);
+}
+__device__ __forceinline__ void store8(float* p, const v8f& v) {
+  const v4f a{v[0], v[1], v[2], v[3]}, b{v[4], v[5], v[6], v[7]};
+  *reinterpret_cast<v4f_any*>(p) = a;
+  store_gap(a);
+  *reinterpret_cast<v4f_any*>(p + 4) = b;
+  store_gap(b);
+}
+__device__ __forceinline__ void store8(__bf16* p, const v8f& v) {
+  const v8bf b = __builtin_convertvector(v, v8bf);  // to nearest even
+  *reinterpret_cast<v8bf_any*>(p) = b;
+  store_gap(__builtin_bit_cast(v4i, b));
+}
+
+// The first n (0 .. 8) of eight values; the rest read zero and are not stored.
+template <typename T>
+__device__ __forceinline__ v8f load8_of(const T* p, int n) {
+  if (n >= 8) return load8(p);
+  v8f v = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) v[i] = static_cast<float>(p[i]);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8_of(T* p, const v8f& v, int n) {
+  if (n >= 8) {
+    store8(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = static_cast<T>(v[i]);
+}
+
+__device__ __forceinline__ int64_t load_id(const void* ids, bool wide, int64_t t) {
+  return wide ? static_cast<const int64_t*>(ids)[t] : static_cast<const int32_t*>(ids)[t];
+}
+
+}  // namespace
+}  // namespace miq
