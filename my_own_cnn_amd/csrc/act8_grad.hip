@@ -2,17 +2,28 @@
 //
 // A kept value, code * 2^e with |code| <= 127, is exact in bf16: bf16 dy multiplies it directly
 // on the bf16 matrix instructions with fp32 sums; fp32 dy is split into three bf16 numbers that
-// add up to it (8 + 8 + 8 significant bits), three products a term.  The terms m are split over
-// workgroups where the output has few tiles, and the partial sums added in order.
+// add up to it (8 + 8 + 8 significant bits), three products a term.
+//
+// A workgroup of four waves computes a TK x TC tile of dw over a range of the rows m, 32 rows a
+// step.  A step's values travel global memory -> registers -> LDS, where both operands lie as bf16
+// rows [m][j] and [m][i]; the codes are turned into bf16 on that way, once per value.  The matrix
+// instructions want eight consecutive m of one column per lane: the transposing LDS read gives a
+// lane four m of its column at once.  The rows of LDS are permuted in units of 16 columns (32
+// bytes) by their m, so that the eight rows of one read lie in different banks.
 #include "train_device.h"
 
 namespace miq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 128;    // output rows and columns per workgroup
-constexpr int kStep = 32;     // terms per step
-constexpr int kPitch = 40;    // bf16 per LDS row: 80 bytes
+constexpr int kStep = 32;  // rows m per step
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef v2i v2i_any __attribute__((aligned(1)));
+typedef v4i v4i_any __attribute__((aligned(1)));
 
 struct Grad {
   const void* dy;
@@ -24,81 +35,245 @@ struct Grad {
   bool accumulate, to_parts;
 };
 
-template <int P>
-__device__ __forceinline__ void split(float v, __bf16 (&p)[P]) {
-  if constexpr (P == 1) {
-    p[0] = static_cast<__bf16>(v);
+// Eight values of dy on their way to LDS.
+template <typename T>
+struct Raw;
+template <>
+struct Raw<__bf16> {
+  v8bf v;
+};
+template <>
+struct Raw<float> {
+  v8f v;
+};
+
+__device__ __forceinline__ void load_raw(Raw<__bf16>& r, const __bf16* p, int n) {
+  if (n >= 8) {
+    r.v = *reinterpret_cast<const v8bf_any*>(p);
   } else {
-    // Truncation leaves at most 16, then 8 significant bits; an infinity or a NaN stays in the
-    // first part alone.
-    const unsigned bits = __float_as_uint(v);
-    const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
-    const unsigned quiet = (bits & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u;
-    const float a = __uint_as_float((bits | quiet) & 0xffff0000u);
-    const float r = finite ? v - a : 0.0f;
-    const float b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-    p[0] = static_cast<__bf16>(a);
-    p[1] = static_cast<__bf16>(b);
-    p[2] = static_cast<__bf16>(r - b);
+    r.v = v8bf{};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) r.v[i] = p[i];
   }
 }
+__device__ __forceinline__ void load_raw(Raw<float>& r, const float* p, int n) { r.v = load8_of(p, n); }
 
-template <typename T, typename TO, int P>
-__global__ __launch_bounds__(kThreads) void act8_grad_kernel(Grad g) {
-  __shared__ __bf16 lds_a[P][kTile][kPitch];
-  __shared__ __bf16 lds_b[kTile][kPitch];
-  const int tile = blockIdx.x % (g.tiles_k * g.tiles_c);
-  const int part = blockIdx.x / (g.tiles_k * g.tiles_c);
-  const int k0 = (tile / g.tiles_c) * kTile;
-  const int c0 = (tile % g.tiles_c) * kTile;
-  const int64_t m0 = static_cast<int64_t>(part) * g.per_split;
-  const int64_t m1 = min(m0 + g.per_split, static_cast<int64_t>(g.rows));
-  const T* dy = static_cast<const T*>(g.dy);
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int wk = (wave >> 1) * 64, wc = (wave & 1) * 64;
-  const int col = threadIdx.x & (kTile - 1);
-  v4f acc[4][4] = {};
-  for (int64_t m = m0; m < m1; m += kStep) {
-    for (int i = threadIdx.x / kTile; i < kStep; i += kThreads / kTile) {
-      const bool there = m + i < m1;
-      const float a = there && k0 + col < g.k ? static_cast<float>(dy[(m + i) * g.ld_dy + k0 + col]) : 0.0f;
-      float b = 0.0f;
-      if (there && c0 + col < g.c) {
-        b = static_cast<float>(g.codes[(m + i) * g.c + c0 + col]) *
-            __uint_as_float(static_cast<unsigned>(g.scales[(m + i) * g.groups + (c0 + col) / kAct8Group]) << 23);
-      }
-      __bf16 p[P];
-      split(a, p);
+// The P bf16 numbers that add up to each of eight values.
+__device__ __forceinline__ void split8(const Raw<__bf16>& r, v8bf (&p)[1]) { p[0] = r.v; }
+__device__ __forceinline__ void split8(const Raw<float>& r, v8bf (&p)[3]) {
+  v8f a, b, c;
 #pragma unroll
-      for (int q = 0; q < P; ++q) lds_a[q][col][i] = p[q];
-      lds_b[col][i] = static_cast<__bf16>(b);
-    }
-    __syncthreads();
-    v8bf fb[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fb[j] = *reinterpret_cast<const v8bf*>(&lds_b[wc + j * 16 + (lane & 15)][(lane >> 4) * 8]);
-#pragma unroll
-    for (int q = P - 1; q >= 0; --q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v8bf fa = *reinterpret_cast<const v8bf*>(&lds_a[q][wk + i * 16 + (lane & 15)][(lane >> 4) * 8]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
-      }
-    __syncthreads();
+  for (int i = 0; i < 8; ++i) {
+    // Truncation leaves at most 16, then 8 significant bits; an infinity or a NaN stays in the
+    // first number alone.
+    const unsigned bits = __float_as_uint(r.v[i]);
+    const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+    const unsigned quiet = (bits & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u;
+    a[i] = __uint_as_float((bits | quiet) & 0xffff0000u);
+    const float rest = finite ? r.v[i] - a[i] : 0.0f;
+    b[i] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+    c[i] = rest - b[i];
   }
+  p[0] = __builtin_convertvector(a, v8bf);
+  p[1] = __builtin_convertvector(b, v8bf);
+  p[2] = __builtin_convertvector(c, v8bf);
+}
+
+// The permutation of a row's 32-byte units: 256 bytes of LDS, all 64 banks, hold the same unit of
+// eight consecutive rows of 256 bytes or more, or of every second one of 128 bytes.
+template <int W>
+__device__ __forceinline__ int turn(int m) {
+  return W >= 128 ? m & 7 : (m >> 1) & 3;
+}
+
+template <typename T, typename TO, int P, int TK, int TC, int STAGES>
+__global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_grad_kernel(Grad g) {
+  constexpr int kPitchA = TK * 2, kPitchB = TC * 2;      // bytes
+  constexpr int kPlane = kStep * kPitchA;
+  constexpr int kStage = P * kPlane + kStep * kPitchB;
+  constexpr int NA = kStep * TK / 8 / kThreads;          // chunks of eight values of dy per thread
+  constexpr int CB = kStep * TC / kThreads < 16 ? 8 : 16;  // codes per chunk
+  constexpr int NB = kStep * TC / CB / kThreads;
+  constexpr int WK = TK / 2, WC = TC / 2;                // a wave's part
+  constexpr int IA = WK / 32, IB = WC / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+
+  const int tiles = g.tiles_k * g.tiles_c;
+  const int at = xcd_tile(blockIdx.x, gridDim.x);
+  const int part = at / tiles;
+  // tiles in bands of four along k: neighbours share their rows of both operands in L2
+  const int tile = at - part * tiles;
+  const int band = tile / (4 * g.tiles_c);
+  const int high = min(4, g.tiles_k - 4 * band);
+  const int in = tile - band * 4 * g.tiles_c;
+  const int k0 = (band * 4 + in % high) * TK;
+  const int c0 = (in / high) * TC;
+  const int m0 = part * g.per_split;  // below rows
+  const int m1 = static_cast<int>(min(static_cast<int64_t>(m0) + g.per_split, static_cast<int64_t>(g.rows)));
+  const int steps = m1 > m0 ? (m1 - m0 + kStep - 1) / kStep : 0;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int wk = (wave >> 1) * WK, wc = (wave & 1) * WC;
+
+  // a thread's chunks: rows a0 + i * (256 * 8 / TK), always the same columns
+  const int a_row = tid / (TK / 8), a_col = (tid % (TK / 8)) * 8;
+  const int b_row = tid / (TC / CB), b_col = (tid % (TC / CB)) * CB;
+  constexpr int kRowsA = kThreads * 8 / TK, kRowsB = kThreads * CB / TC;
+  const int a_left = g.k - k0 - a_col;
+  const int b_left = g.c - c0 - b_col;
+  const T* a_from = static_cast<const T*>(g.dy) + (m0 + a_row) * g.ld_dy + k0 + a_col;
+  const int8_t* b_from = g.codes + (static_cast<int64_t>(m0) + b_row) * g.c + c0 + b_col;
+  const uint8_t* s_from = g.scales + (static_cast<int64_t>(m0) + b_row) * g.groups + (c0 + b_col) / kAct8Group;
+
+  Raw<T> ra[NA];
+  v4i rb[NB];
+  unsigned rs[NB];
+  const bool inner = k0 + TK <= g.k && c0 + TC <= g.c;
+  const T* a_now = a_from;
+  const int8_t* b_now = b_from;
+  const uint8_t* s_now = s_from;
+  auto load = [&](int step) {  // steps in order: the pointers move on
+    const int m = m0 + step * kStep;
+    if (inner && m + kStep <= m1) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) load_raw(ra[i], a_now + i * (kRowsA * g.ld_dy), 8);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int8_t* p = b_now + i * (kRowsB * static_cast<int64_t>(g.c));
+        if constexpr (CB == 16) {
+          rb[i] = *reinterpret_cast<const v4i_any*>(p);
+        } else {
+          const v2i w = *reinterpret_cast<const v2i_any*>(p);
+          rb[i][0] = w[0];
+          rb[i][1] = w[1];
+        }
+        rs[i] = s_now[i * (kRowsB * static_cast<int64_t>(g.groups))];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+        load_raw(ra[i], a_now + i * (kRowsA * g.ld_dy), m + a_row + i * kRowsA < m1 ? a_left : 0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const bool there = m + b_row + i * kRowsB < m1 && b_left > 0;
+        const int8_t* p = b_now + i * (kRowsB * static_cast<int64_t>(g.c));
+        rb[i] = v4i{};
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+          if (there && j < b_left) rb[i][j / 4] |= (p[j] & 0xff) << (8 * (j & 3));
+        rs[i] = there ? s_now[i * (kRowsB * static_cast<int64_t>(g.groups))] : 0;
+      }
+    }
+    a_now += kStep * g.ld_dy;
+    b_now += kStep * static_cast<int64_t>(g.c);
+    s_now += kStep * static_cast<int64_t>(g.groups);
+  };
+  auto write = [&](int stage) {
+    char* const base = lds + stage * kStage;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int row = a_row + i * kRowsA;
+      v8bf p[P];
+      split8(ra[i], p);
+      char* const to = base + row * kPitchA + (((a_col >> 4) ^ turn<TK>(row)) * 32) + (a_col & 8) * 2;
+#pragma unroll
+      for (int q = 0; q < P; ++q) *reinterpret_cast<v8bf*>(to + q * kPlane) = p[q];
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int row = b_row + i * kRowsB;
+      const float scale = __uint_as_float(rs[i] << 23);  // byte 255: infinity, NaN times a zero code
+      char* const to = base + P * kPlane + row * kPitchB + (((b_col >> 4) ^ turn<TC>(row)) * 32) + (b_col & 8) * 2;
+#pragma unroll
+      for (int j = 0; j < CB / 8; ++j) {
+        const v4f lo = codes4(rb[i][2 * j]) * scale, hi = codes4(rb[i][2 * j + 1]) * scale;
+        *reinterpret_cast<v8bf*>(to + j * 16) =
+            __builtin_convertvector(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), v8bf);
+      }
+    }
+  };
+
+  // Fragments: lane l's column is l & 31, its rows of a 16-row half are (l >> 5) * 4 .. + 3 and
+  // those plus 8; one transposing read takes four rows of a 16-column unit per 16 lanes.
+  const int f_row = (lane >> 5) * 4 + ((lane & 15) >> 2);
+  const int f_unit = (lane >> 4) & 1;
+  int a_at[IA], b_at[IB];
+#pragma unroll
+  for (int i = 0; i < IA; ++i)
+    a_at[i] = f_row * kPitchA + (((wk / 16 + 2 * i + f_unit) ^ turn<TK>(f_row)) * 32) + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < IB; ++i)
+    b_at[i] = P * kPlane + f_row * kPitchB + (((wc / 16 + 2 * i + f_unit) ^ turn<TC>(f_row)) * 32) + (lane & 3) * 8;
+  auto fragment = [&](int byte, int pitch) {
+    // rows + 8 have the same permutation
+    const unsigned a = static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds)) + byte;
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<__attribute__((address_space(3))) v4s*>(static_cast<uintptr_t>(a)));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<__attribute__((address_space(3))) v4s*>(static_cast<uintptr_t>(a + 8 * pitch)));
+    return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  v16f acc[IA][IB] = {};
+  v8bf fa[2][P][IA], fb[2][IB];
+  auto read = [&](int stage, int half, int to) {
+    const int base = stage * kStage;
+#pragma unroll
+    for (int i = 0; i < IB; ++i) fb[to][i] = fragment(base + b_at[i] + half * 16 * kPitchB, kPitchB);
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+#pragma unroll
+      for (int i = 0; i < IA; ++i) fa[to][q][i] = fragment(base + q * kPlane + a_at[i] + half * 16 * kPitchA, kPitchA);
+  };
+  auto multiply = [&](int from) {
+#pragma unroll
+    for (int q = P - 1; q >= 0; --q)  // the smallest pieces first
+#pragma unroll
+      for (int i = 0; i < IA; ++i)
+#pragma unroll
+        for (int j = 0; j < IB; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][q][i], fb[from][j], acc[i][j], 0, 0, 0);
+  };
+
+  static_assert(STAGES == 3, "a step reads its own stage and the next one's first half, and writes the third");
+  if (steps > 0) {
+    load(0);
+    write(0);
+    if (steps > 1) {
+      load(1);
+      write(1);
+    }
+    if (steps > 2) load(2);
+    __syncthreads();
+    read(0, 0, 0);
+    int now = 0;
+    for (int t = 0; t < steps; ++t) {
+      const int next = now == 2 ? 0 : now + 1;
+      read(now, 1, 1);
+      multiply(0);
+      if (t + 2 < steps) write(next == 2 ? 0 : next + 1);
+      if (t + 3 < steps) load(t + 3);
+      if (t + 1 < steps) read(next, 0, 0);
+      multiply(1);
+      __syncthreads();
+      now = next;
+    }
+  }
+
   TO* out = static_cast<TO*>(g.out) + (g.to_parts ? static_cast<int64_t>(part) * g.k * g.c : 0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < IA; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < IB; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = k0 + wk + i * 16 + (lane >> 4) * 4 + r;
-        const int at = c0 + wc + j * 16 + (lane & 15);
-        if (row < g.k && at < g.c) {
-          TO* to = out + row * g.ld_out + at;
+      for (int r = 0; r < 16; ++r) {
+        const int row = k0 + wk + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+        const int col = c0 + wc + j * 32 + (lane & 31);
+        if (row < g.k && col < g.c) {
+          TO* to = out + row * g.ld_out + col;
           float v = acc[i][j][r];
           if (g.accumulate) v += static_cast<float>(*to);
           *to = static_cast<TO>(v);
@@ -106,36 +281,85 @@ __global__ __launch_bounds__(kThreads) void act8_grad_kernel(Grad g) {
       }
 }
 
+// Adds the splits' partial sums in order: 64 values per workgroup, the splits shared by its four
+// waves, whose four sums are added in order.
 template <typename TO>
 __global__ __launch_bounds__(kThreads) void act8_grad_join_kernel(Grad g, const float* __restrict__ parts, int splits) {
+  __shared__ float sums[4][64];
   const int64_t n = static_cast<int64_t>(g.k) * g.c;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int each = (splits + 3) / 4;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 64; i0 < n; i0 += static_cast<int64_t>(gridDim.x) * 64) {
+    const int64_t i = i0 + lane;
     float v = 0.0f;
-    for (int s = 0; s < splits; ++s) v += parts[s * n + i];
-    TO* to = static_cast<TO*>(g.out) + (i / g.c) * g.ld_out + i % g.c;
-    if (g.accumulate) v += static_cast<float>(*to);
-    *to = static_cast<TO>(v);
+    if (i < n) {
+      const int end = min((wave + 1) * each, splits);
+#pragma unroll 8
+      for (int s = wave * each; s < end; ++s) v += parts[s * n + i];
+    }
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && i < n) {
+      v = ((v + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
+      TO* to = static_cast<TO*>(g.out) + (i / g.c) * g.ld_out + i % g.c;
+      if (g.accumulate) v += static_cast<float>(*to);
+      *to = static_cast<TO>(v);
+    }
+    __syncthreads();
   }
 }
 
-// Splits of the terms: enough workgroups for two on each of the 256 CUs, 256 terms each or more.
-int splits_of(int32_t rows, int32_t c, int32_t k, int* per) {
-  const int64_t tiles = ((static_cast<int64_t>(c) + kTile - 1) / kTile) * ((static_cast<int64_t>(k) + kTile - 1) / kTile);
-  int64_t n = 512 / tiles;
-  const int64_t most = (static_cast<int64_t>(rows) + 255) / 256;
+struct Shape {
+  int tk, tc, splits, per;
+};
+
+// The tile, and splits of the rows: enough workgroups for every CU, 128 rows each or more.
+Shape shape_of(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
+  auto tiles = [&](int t) { return ((static_cast<int64_t>(c) + t - 1) / t) * ((static_cast<int64_t>(k) + t - 1) / t); };
+  Shape s{};
+  s.tk = dy_bf16 && tiles(256) * (rows / 512) >= 192 ? 256 : 128;
+  if (tiles(128) * (rows / 128) < 192) s.tk = 64;
+  s.tc = s.tk;
+  int64_t n = 256 / tiles(s.tk);
+  const int64_t most = (static_cast<int64_t>(rows) + 127) / 128;
   if (n > most) n = most;
   if (n < 1) n = 1;
   int64_t each = (rows + n - 1) / n;
   each = (each + kStep - 1) / kStep * kStep;
   if (each < kStep) each = kStep;
-  *per = static_cast<int>(each);
+  s.per = static_cast<int>(each);
   n = (rows + each - 1) / each;
-  return static_cast<int>(n < 1 ? 1 : n);
+  s.splits = static_cast<int>(n < 1 ? 1 : n);
+  return s;
+}
+
+template <typename T, typename TO, int P, int TK, int TC>
+hipError_t launch_tile(const Grad& g, unsigned blocks, hipStream_t stream) {
+  constexpr int kBytes = 3 * (P * kStep * TK * 2 + kStep * TC * 2);
+  auto* kernel = &act8_grad_kernel<T, TO, P, TK, TC, 3>;
+  if (kBytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != hipSuccess) return e;
+  }
+  kernel<<<blocks, kThreads, kBytes, stream>>>(g);
+  return hipGetLastError();
 }
 
 template <typename T, typename TO, int P>
-void launch(const Act8GradArgs& a, hipStream_t stream) {
+hipError_t launch_product(const Grad& g, const Shape& s, hipStream_t stream) {
+  const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(g.tiles_k) * g.tiles_c * s.splits);
+  if constexpr (P == 1) {
+    if (s.tk == 256) return launch_tile<T, TO, P, 256, 256>(g, blocks, stream);
+  }
+  if (s.tk == 128) return launch_tile<T, TO, P, 128, 128>(g, blocks, stream);
+  return launch_tile<T, TO, P, 64, 64>(g, blocks, stream);
+}
+
+template <typename T, typename TO, int P>
+hipError_t launch(const Act8GradArgs& a, hipStream_t stream) {
+  const Shape s = shape_of(a.rows, a.c, a.k, a.dy_bf16);
   Grad g{};
   g.dy = a.dy;
   g.codes = a.codes;
@@ -145,46 +369,36 @@ void launch(const Act8GradArgs& a, hipStream_t stream) {
   g.c = a.c;
   g.k = a.k;
   g.groups = (a.c + kAct8Group - 1) / kAct8Group;
-  g.tiles_k = (a.k + kTile - 1) / kTile;
-  g.tiles_c = (a.c + kTile - 1) / kTile;
-  const int splits = splits_of(a.rows, a.c, a.k, &g.per_split);
-  const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(g.tiles_k) * g.tiles_c * splits);
+  g.tiles_k = (a.k + s.tk - 1) / s.tk;
+  g.tiles_c = (a.c + s.tc - 1) / s.tc;
+  g.per_split = s.per;
   g.out = a.dw;
   g.ld_out = a.ld_dw;
   g.accumulate = a.accumulate;
-  if (splits == 1) {
-    act8_grad_kernel<T, TO, P><<<blocks, kThreads, 0, stream>>>(g);
-    return;
-  }
+  if (s.splits == 1) return launch_product<T, TO, P>(g, s, stream);
   Grad h = g;
   h.out = a.ws;
   h.ld_out = a.c;
   h.accumulate = false;
   h.to_parts = true;
-  act8_grad_kernel<T, float, P><<<blocks, kThreads, 0, stream>>>(h);
-  const int64_t n = static_cast<int64_t>(a.k) * a.c;
-  const int64_t join = (n + kThreads - 1) / kThreads;
-  act8_grad_join_kernel<TO><<<static_cast<unsigned>(join < 4096 ? join : 4096), kThreads, 0, stream>>>(
-      g, static_cast<const float*>(a.ws), splits);
+  const hipError_t e = launch_product<T, float, P>(h, s, stream);
+  if (e != hipSuccess) return e;
+  const int64_t join = (static_cast<int64_t>(a.k) * a.c + 63) / 64;
+  act8_grad_join_kernel<TO><<<static_cast<unsigned>(join < 65536 ? join : 65536), kThreads, 0, stream>>>(
+      g, static_cast<const float*>(a.ws), s.splits);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-size_t act8_grad_workspace_bytes(int32_t rows, int32_t c, int32_t k, bool) {
-  int per;
-  const int splits = splits_of(rows, c, k, &per);
-  return splits > 1 ? static_cast<size_t>(splits) * c * k * 4 : 0;
+size_t act8_grad_workspace_bytes(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
+  const Shape s = shape_of(rows, c, k, dy_bf16);
+  return s.splits > 1 ? static_cast<size_t>(s.splits) * c * k * 4 : 0;
 }
 
 hipError_t launch_act8_grad(const Act8GradArgs& a, hipStream_t stream) {
-  if (!a.dy_bf16) {
-    launch<float, float, 3>(a, stream);
-  } else if (a.dw_bf16) {
-    launch<__bf16, __bf16, 1>(a, stream);
-  } else {
-    launch<__bf16, float, 1>(a, stream);
-  }
-  return hipGetLastError();
+  if (!a.dy_bf16) return launch<float, float, 3>(a, stream);
+  return a.dw_bf16 ? launch<__bf16, __bf16, 1>(a, stream) : launch<__bf16, float, 1>(a, stream);
 }
 
 }  // namespace miq

@@ -58,6 +58,13 @@ __device__ __forceinline__ void store8_of(T* p, const v8f& v, int n) {
     if (i < n) p[i] = static_cast<T>(v[i]);
 }
 
+// Four int8 codes of a word as fp32, one conversion with a byte select each.  (A vector conversion
+// of eight chars takes the last one through 64-bit integers.)
+__device__ __forceinline__ v4f codes4(int w) {
+  return v4f{static_cast<float>(static_cast<signed char>(w)), static_cast<float>(static_cast<signed char>(w >> 8)),
+             static_cast<float>(static_cast<signed char>(w >> 16)), static_cast<float>(w >> 24)};
+}
+
 __device__ __forceinline__ int64_t load_id(const void* ids, bool wide, int64_t t) {
   return wide ? static_cast<const int64_t*>(ids)[t] : static_cast<const int32_t*>(ids)[t];
 }

@@ -256,6 +256,7 @@ def test_beyond_32_bit_offsets(device):
 GRADS = [  # rows, c, k
     (1, 1, 1), (1, 33, 5), (2, 32, 64), (31, 128, 128), (32, 127, 129), (33, 130, 70), (64, 257, 200), (257, 64, 300),
     (1000, 96, 513), (513, 1003, 31), (2049, 256, 256), (5000, 65, 40), (300, 512, 384), (20001, 128, 128),
+    (24577, 512, 512), (19999, 300, 1001),
 ]
 
 
