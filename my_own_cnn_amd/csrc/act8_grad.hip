@@ -87,7 +87,7 @@ __device__ __forceinline__ int turn(int m) {
   return W >= 128 ? m & 7 : (m >> 1) & 3;
 }
 
-template <typename T, typename TO, int P, int TK, int TC, int STAGES>
+template <typename T, typename TO, int P, int TK, int TC, int SETS>
 __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_grad_kernel(Grad g) {
   constexpr int kPitchA = TK * 2, kPitchB = TC * 2;      // bytes
   constexpr int kPlane = kStep * kPitchA;
@@ -97,6 +97,7 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
   constexpr int NB = kStep * TC / CB / kThreads;
   constexpr int WK = TK / 2, WC = TC / 2;                // a wave's part
   constexpr int IA = WK / 32, IB = WC / 32;
+  constexpr int VALU = P == 3 ? 8 : 8;
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int tiles = g.tiles_k * g.tiles_c;
@@ -128,56 +129,79 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
   const int8_t* b_from = g.codes + (static_cast<int64_t>(m0) + b_row) * g.c + c0 + b_col;
   const uint8_t* s_from = g.scales + (static_cast<int64_t>(m0) + b_row) * g.groups + (c0 + b_col) / kAct8Group;
 
-  Raw<T> ra[NA];
-  v4i rb[NB];
-  unsigned rs[NB];
-  const bool inner = k0 + TK <= g.k && c0 + TC <= g.c;
-  const T* a_now = a_from;
-  const int8_t* b_now = b_from;
-  const uint8_t* s_now = s_from;
-  auto load = [&](int step) {  // steps in order: the pointers move on
-    const int m = m0 + step * kStep;
-    if (inner && m + kStep <= m1) {
-#pragma unroll
-      for (int i = 0; i < NA; ++i) load_raw(ra[i], a_now + i * (kRowsA * g.ld_dy), 8);
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int8_t* p = b_now + i * (kRowsB * static_cast<int64_t>(g.c));
-        if constexpr (CB == 16) {
-          rb[i] = *reinterpret_cast<const v4i_any*>(p);
-        } else {
-          const v2i w = *reinterpret_cast<const v2i_any*>(p);
-          rb[i][0] = w[0];
-          rb[i][1] = w[1];
-        }
-        rs[i] = s_now[i * (kRowsB * static_cast<int64_t>(g.groups))];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NA; ++i)
-        load_raw(ra[i], a_now + i * (kRowsA * g.ld_dy), m + a_row + i * kRowsA < m1 ? a_left : 0);
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const bool there = m + b_row + i * kRowsB < m1 && b_left > 0;
-        const int8_t* p = b_now + i * (kRowsB * static_cast<int64_t>(g.c));
-        rb[i] = v4i{};
-#pragma unroll
-        for (int j = 0; j < CB; ++j)
-          if (there && j < b_left) rb[i][j / 4] |= (p[j] & 0xff) << (8 * (j & 3));
-        rs[i] = there ? s_now[i * (kRowsB * static_cast<int64_t>(g.groups))] : 0;
-      }
-    }
-    a_now += kStep * g.ld_dy;
-    b_now += kStep * static_cast<int64_t>(g.c);
-    s_now += kStep * static_cast<int64_t>(g.groups);
+  struct Staged {
+    Raw<T> a[NA];
+    v4i b[NB];
+    unsigned scale[NB];
   };
-  auto write = [&](int stage) {
+  // Steps whose 32 rows can be read whole, columns beyond the tensors' widths (other rows' values,
+  // which reach only sums that are not stored) among them: inside the range, and not so near the
+  // tensors' ends that such a column lies beyond them.
+  auto whole = [&](int64_t ld, int64_t width, int64_t first, int64_t span) {
+    const int64_t last = (g.rows - 1) * ld + width - first - span;  // row 0's reads may start here at most
+    return last < 0 ? int64_t{0} : last / ld + 1;
+  };
+  // Spreads a half step's other instructions between its matrix instructions: left alone, the
+  // compiler issues the matrix instructions in one run and the conversions after them.
+  auto mix = [&]() {
+    constexpr int kMul = P * IA * IB;
+    constexpr int kReads = 2 * (P * IA + IB), kWrites = P * NA + NB * CB / 8;
+#pragma unroll
+    for (int i = 0; i < kMul; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                          // matrix
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * ((kReads + kMul - 1) / kMul), 0);  // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);                       // vector ALU
+      __builtin_amdgcn_sched_group_barrier(0x200, (kWrites + kMul - 1) / kMul, 0);  // LDS writes
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                          // loads
+    }
+  };
+  const int64_t safe = min(min(whole(g.ld_dy, g.k, k0, TK), whole(g.c, g.c, c0, TC)),
+                           whole(g.groups, g.groups, c0 / kAct8Group, (TC + kAct8Group - 1) / kAct8Group));
+  const int fast = static_cast<int>(max(min(safe, static_cast<int64_t>(m1)) - m0, int64_t{0})) / kStep;
+  auto load = [&](Staged& r, int step) {
+    const int64_t down = static_cast<int64_t>(step) * kStep;
+    const T* a = a_from + down * g.ld_dy;
+    const int8_t* b = b_from + down * g.c;
+    const uint8_t* s = s_from + down * g.groups;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) load_raw(r.a[i], a + i * (kRowsA * g.ld_dy), 8);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int8_t* p = b + i * (kRowsB * static_cast<int64_t>(g.c));
+      if constexpr (CB == 16) {
+        r.b[i] = *reinterpret_cast<const v4i_any*>(p);
+      } else {
+        const v2i w = *reinterpret_cast<const v2i_any*>(p);
+        r.b[i][0] = w[0];
+        r.b[i][1] = w[1];
+      }
+      r.scale[i] = s[i * (kRowsB * static_cast<int64_t>(g.groups))];
+    }
+  };
+  auto load_edge = [&](Staged& r, int step) {  // value by value at the edges, zeros beyond them
+    const int64_t down = static_cast<int64_t>(step) * kStep;
+    const int m = m0 + step * kStep;
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      load_raw(r.a[i], a_from + (down + i * kRowsA) * g.ld_dy, m + a_row + i * kRowsA < m1 ? a_left : 0);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const bool there = m + b_row + i * kRowsB < m1 && b_left > 0;
+      const int8_t* p = b_from + (down + i * kRowsB) * g.c;
+      r.b[i] = v4i{};
+#pragma unroll
+      for (int j = 0; j < CB; ++j)
+        if (there && j < b_left) r.b[i][j / 4] |= (p[j] & 0xff) << (8 * (j & 3));
+      r.scale[i] = there ? s_from[(down + i * kRowsB) * g.groups] : 0;
+    }
+  };
+  auto write = [&](const Staged& r, int stage) {
     char* const base = lds + stage * kStage;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const int row = a_row + i * kRowsA;
       v8bf p[P];
-      split8(ra[i], p);
+      split8(r.a[i], p);
       char* const to = base + row * kPitchA + (((a_col >> 4) ^ turn<TK>(row)) * 32) + (a_col & 8) * 2;
 #pragma unroll
       for (int q = 0; q < P; ++q) *reinterpret_cast<v8bf*>(to + q * kPlane) = p[q];
@@ -185,11 +209,11 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int row = b_row + i * kRowsB;
-      const float scale = __uint_as_float(rs[i] << 23);  // byte 255: infinity, NaN times a zero code
+      const float scale = __uint_as_float(r.scale[i] << 23);  // byte 255: infinity, NaN times a zero code
       char* const to = base + P * kPlane + row * kPitchB + (((b_col >> 4) ^ turn<TC>(row)) * 32) + (b_col & 8) * 2;
 #pragma unroll
       for (int j = 0; j < CB / 8; ++j) {
-        const v4f lo = codes4(rb[i][2 * j]) * scale, hi = codes4(rb[i][2 * j + 1]) * scale;
+        const v4f lo = codes4(r.b[i][2 * j]) * scale, hi = codes4(r.b[i][2 * j + 1]) * scale;
         *reinterpret_cast<v8bf*>(to + j * 16) =
             __builtin_convertvector(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), v8bf);
       }
@@ -238,29 +262,58 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][q][i], fb[from][j], acc[i][j], 0, 0, 0);
   };
 
-  static_assert(STAGES == 3, "a step reads its own stage and the next one's first half, and writes the third");
-  if (steps > 0) {
-    load(0);
-    write(0);
-    if (steps > 1) {
-      load(1);
-      write(1);
+  // Three stages: a step multiplies its own, reads the next one's first half and writes the third,
+  // whose values were loaded SETS steps before.  Past the last step the loads, writes and reads
+  // repeat that step: their values go unused.
+  if (fast > 0) {
+    Staged first[2], r[SETS];  // step s >= 2 in r[s % SETS]
+    // the sets' loads in order: the waits for one of them do not include the next
+    load(first[0], 0);
+    load(first[1], min(1, fast - 1));
+#pragma unroll
+    for (int i = 2; i < 2 + SETS; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      load(r[i % SETS], min(i, fast - 1));
     }
-    if (steps > 2) load(2);
+    __builtin_amdgcn_sched_barrier(0);
+    write(first[0], 0);
+    write(first[1], 1);
     __syncthreads();
     read(0, 0, 0);
     int now = 0;
-    for (int t = 0; t < steps; ++t) {
+    auto step = [&](Staged& set, int t) {
       const int next = now == 2 ? 0 : now + 1;
       read(now, 1, 1);
+      write(set, next == 2 ? 0 : next + 1);
       multiply(0);
-      if (t + 2 < steps) write(next == 2 ? 0 : next + 1);
-      if (t + 3 < steps) load(t + 3);
-      if (t + 1 < steps) read(next, 0, 0);
+      mix();
+      __builtin_amdgcn_sched_barrier(0);
+      load(set, min(t + 2 + SETS, fast - 1));
+      read(next, 0, 0);
       multiply(1);
+      mix();
       __syncthreads();
       now = next;
+    };
+    int t = 0;
+    for (; t + SETS <= fast; t += SETS) {  // no other way round the loop: its waits count on the loads' order
+#pragma unroll
+      for (int u = 0; u < SETS; ++u) step(r[(u + 2) % SETS], t + u);
     }
+#pragma unroll
+    for (int u = 0; u + 1 < SETS; ++u)
+      if (t + u < fast) step(r[(u + 2) % SETS], t + u);
+  }
+  for (int t = fast; t < steps; ++t) {
+    Staged r;
+    load_edge(r, t);
+    __syncthreads();
+    write(r, 0);
+    __syncthreads();
+    read(0, 0, 0);
+    read(0, 1, 1);
+    multiply(0);
+    multiply(1);
   }
 
   TO* out = static_cast<TO*>(g.out) + (g.to_parts ? static_cast<int64_t>(part) * g.k * g.c : 0);
@@ -337,7 +390,7 @@ Shape shape_of(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
 template <typename T, typename TO, int P, int TK, int TC>
 hipError_t launch_tile(const Grad& g, unsigned blocks, hipStream_t stream) {
   constexpr int kBytes = 3 * (P * kStep * TK * 2 + kStep * TC * 2);
-  auto* kernel = &act8_grad_kernel<T, TO, P, TK, TC, 3>;
+  auto* kernel = &act8_grad_kernel<T, TO, P, TK, TC, 2>;
   if (kBytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
