@@ -507,6 +507,10 @@ int miq_act8_expand(const int8_t* codes, const uint8_t* scales, void* y, int64_t
 /* Bytes of device workspace miq_act8_grad needs (no GPU access). */
 int miq_act8_grad_workspace_size(int64_t rows, int32_t c, int32_t k, int32_t dy_type, size_t* bytes);
 
+/* How miq_act8_grad runs a problem: plan[0] the side of dw's tiles, plan[1] the parts that the rows
+ * are split into; zeros where there is nothing to do.  No GPU access. */
+int miq_plan_act8_grad(int64_t rows, int32_t c, int32_t k, int32_t dy_type, int32_t plan[2]);
+
 /* The weight gradient of a linear (1x1) layer from its input kept in 8 bits (not gated):
  * dw[j, i] = sum over m of dy[m, j] * x'[m, i], j < k, i < c; accumulate != 0 adds it to dw.
  * On bf16 matrix instructions, which hold x' exactly: bf16 dy directly, fp32 dy split into three

@@ -161,6 +161,7 @@ SIGNATURES = {
     "miq_act8_bprop": (C.c_int, [_P, _P, _P, _P, _L, _I, _L, _L, _I, _I, _I, _P]),
     "miq_act8_expand": (C.c_int, [_P, _P, _P, _L, _I, _L, _I, _I, _I, _P]),
     "miq_act8_grad_workspace_size": (C.c_int, [_L, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    "miq_plan_act8_grad": (C.c_int, [_L, _I, _I, _I, _PI]),
     "miq_act8_grad": (
         C.c_int, [_P, _P, _P, _P, _L, _I, _I, _L, _L, _I, _I, _I, _P, C.c_size_t, _P]),
 }

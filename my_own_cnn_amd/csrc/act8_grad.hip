@@ -87,18 +87,18 @@ __device__ __forceinline__ int turn(int m) {
   return W >= 128 ? m & 7 : (m >> 1) & 3;
 }
 
-template <typename T, typename TO, int P, int TK, int TC, int SETS>
-__global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_grad_kernel(Grad g) {
+template <typename T, typename TO, int P, int TK, int TC, int VK, int VC, int STAGES, int SETS>
+__global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8_grad_kernel(Grad g) {
+  constexpr int kThreads = VK * VC * 64;
   constexpr int kPitchA = TK * 2, kPitchB = TC * 2;      // bytes
   constexpr int kPlane = kStep * kPitchA;
   constexpr int kStage = P * kPlane + kStep * kPitchB;
   constexpr int NA = kStep * TK / 8 / kThreads;          // chunks of eight values of dy per thread
   constexpr int CB = kStep * TC / kThreads < 16 ? 8 : 16;  // codes per chunk
   constexpr int NB = kStep * TC / CB / kThreads;
-  constexpr int WK = TK / 2, WC = TC / 2;                // a wave's part
+  constexpr int WK = TK / VK, WC = TC / VC;              // a wave's part
   constexpr int IA = WK / 32, IB = WC / 32;
-  constexpr int VALU = P == 3 ? 8 : 8;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int tiles = g.tiles_k * g.tiles_c;
   const int at = xcd_tile(blockIdx.x, gridDim.x);
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
-  const int wk = (wave >> 1) * WK, wc = (wave & 1) * WC;
+  const int wk = (wave / VC) * WK, wc = (wave % VC) * WC;
 
   // a thread's chunks: rows a0 + i * (256 * 8 / TK), always the same columns
   const int a_row = tid / (TK / 8), a_col = (tid % (TK / 8)) * 8;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
     for (int i = 0; i < kMul; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                          // matrix
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * ((kReads + kMul - 1) / kMul), 0);  // LDS reads
-      __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);                       // vector ALU
+      __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);                          // vector ALU
       __builtin_amdgcn_sched_group_barrier(0x200, (kWrites + kMul - 1) / kMul, 0);  // LDS writes
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                          // loads
     }
@@ -231,26 +231,28 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
 #pragma unroll
   for (int i = 0; i < IB; ++i)
     b_at[i] = P * kPlane + f_row * kPitchB + (((wc / 16 + 2 * i + f_unit) ^ turn<TC>(f_row)) * 32) + (lane & 3) * 8;
-  auto fragment = [&](int byte, int pitch) {
+  typedef __attribute__((address_space(3))) char lds_char;
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  lds_char* const lds3 = (lds_char*)lds;  // an address-space cast
+  auto fragment = [&](lds_char* from, int pitch) {
     // rows + 8 have the same permutation
-    const unsigned a = static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds)) + byte;
-    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        reinterpret_cast<__attribute__((address_space(3))) v4s*>(static_cast<uintptr_t>(a)));
-    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        reinterpret_cast<__attribute__((address_space(3))) v4s*>(static_cast<uintptr_t>(a + 8 * pitch)));
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(from));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(from + 8 * pitch));
     return __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
   v16f acc[IA][IB] = {};
   v8bf fa[2][P][IA], fb[2][IB];
   auto read = [&](int stage, int half, int to) {
-    const int base = stage * kStage;
+    lds_char* const base = lds3 + stage * kStage;
 #pragma unroll
     for (int i = 0; i < IB; ++i) fb[to][i] = fragment(base + b_at[i] + half * 16 * kPitchB, kPitchB);
 #pragma unroll
-    for (int q = 0; q < P; ++q)
+    for (int i = 0; i < IA; ++i) {
+      lds_char* const column = base + a_at[i] + half * 16 * kPitchA;
 #pragma unroll
-      for (int i = 0; i < IA; ++i) fa[to][q][i] = fragment(base + q * kPlane + a_at[i] + half * 16 * kPitchA, kPitchA);
+      for (int q = 0; q < P; ++q) fa[to][q][i] = fragment(column + q * kPlane, kPitchA);
+    }
   };
   auto multiply = [&](int from) {
 #pragma unroll
@@ -262,34 +264,42 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][q][i], fb[from][j], acc[i][j], 0, 0, 0);
   };
 
-  // Three stages: a step multiplies its own, reads the next one's first half and writes the third,
-  // whose values were loaded SETS steps before.  Past the last step the loads, writes and reads
-  // repeat that step: their values go unused.
+  // Three stages: a step multiplies its own, reads the next one's first half and writes the third.
+  // Two, where three do not fit: a step reads and multiplies its own and writes the other.  Either
+  // way the values written were loaded SETS steps before.  Past the last step the loads, writes and
+  // reads repeat that step: their values go unused.
+  constexpr int kAhead = STAGES - 1;  // a step writes the values of step t + kAhead
   if (fast > 0) {
-    Staged first[2], r[SETS];  // step s >= 2 in r[s % SETS]
+    Staged first[kAhead], r[SETS];  // step s >= kAhead in r[s % SETS]
     // the sets' loads in order: the waits for one of them do not include the next
-    load(first[0], 0);
-    load(first[1], min(1, fast - 1));
 #pragma unroll
-    for (int i = 2; i < 2 + SETS; ++i) {
+    for (int i = 0; i < kAhead; ++i) load(first[i], min(i, fast - 1));
+#pragma unroll
+    for (int i = kAhead; i < kAhead + SETS; ++i) {
       __builtin_amdgcn_sched_barrier(0);
       load(r[i % SETS], min(i, fast - 1));
     }
     __builtin_amdgcn_sched_barrier(0);
-    write(first[0], 0);
-    write(first[1], 1);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) write(first[i], i);
     __syncthreads();
-    read(0, 0, 0);
+    if constexpr (STAGES == 3) read(0, 0, 0);
     int now = 0;
     auto step = [&](Staged& set, int t) {
-      const int next = now == 2 ? 0 : now + 1;
-      read(now, 1, 1);
-      write(set, next == 2 ? 0 : next + 1);
+      const int next = now == STAGES - 1 ? 0 : now + 1;
+      if constexpr (STAGES == 3) {
+        read(now, 1, 1);
+        write(set, next == STAGES - 1 ? 0 : next + 1);
+      } else {
+        read(now, 0, 0);
+        read(now, 1, 1);
+        write(set, next);
+      }
       multiply(0);
       mix();
       __builtin_amdgcn_sched_barrier(0);
-      load(set, min(t + 2 + SETS, fast - 1));
-      read(next, 0, 0);
+      load(set, min(t + kAhead + SETS, fast - 1));
+      if constexpr (STAGES == 3) read(next, 0, 0);
       multiply(1);
       mix();
       __syncthreads();
@@ -298,11 +308,11 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
     int t = 0;
     for (; t + SETS <= fast; t += SETS) {  // no other way round the loop: its waits count on the loads' order
 #pragma unroll
-      for (int u = 0; u < SETS; ++u) step(r[(u + 2) % SETS], t + u);
+      for (int u = 0; u < SETS; ++u) step(r[(u + kAhead) % SETS], t + u);
     }
 #pragma unroll
     for (int u = 0; u + 1 < SETS; ++u)
-      if (t + u < fast) step(r[(u + 2) % SETS], t + u);
+      if (t + u < fast) step(r[(u + kAhead) % SETS], t + u);
   }
   for (int t = fast; t < steps; ++t) {
     Staged r;
@@ -334,69 +344,113 @@ __global__ __launch_bounds__(kThreads, TK* TC >= 256 * 256 ? 1 : 2) void act8_gr
       }
 }
 
-// Adds the splits' partial sums in order: 64 values per workgroup, the splits shared by its four
-// waves, whose four sums are added in order.
+// Adds the splits' partial sums in order, four values per lane: `parts_of` lanes of a workgroup
+// share the splits of the same values, and their sums are added in order.
 template <typename TO>
-__global__ __launch_bounds__(kThreads) void act8_grad_join_kernel(Grad g, const float* __restrict__ parts, int splits) {
-  __shared__ float sums[4][64];
+__global__ __launch_bounds__(kThreads) void act8_grad_join_kernel(Grad g, const float* __restrict__ parts, int splits,
+                                                                  int parts_of) {
+  __shared__ v4f sums[kThreads];
   const int64_t n = static_cast<int64_t>(g.k) * g.c;
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int each = (splits + 3) / 4;
-  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 64; i0 < n; i0 += static_cast<int64_t>(gridDim.x) * 64) {
-    const int64_t i = i0 + lane;
-    float v = 0.0f;
-    if (i < n) {
-      const int end = min((wave + 1) * each, splits);
+  const int wide = kThreads / parts_of;  // lanes along the values
+  const int at = threadIdx.x % wide;
+  const int share = threadIdx.x / wide;
+  const int each = (splits + parts_of - 1) / parts_of;
+  const int end = min((share + 1) * each, splits);
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * wide * 4; i0 < n; i0 += static_cast<int64_t>(gridDim.x) * wide * 4) {
+    const int64_t i = i0 + at * 4;
+    const int left = static_cast<int>(min(n - i, int64_t{4}));
+    v4f v = {};
+    if (left == 4) {
 #pragma unroll 8
-      for (int s = wave * each; s < end; ++s) v += parts[s * n + i];
+      for (int s = share * each; s < end; ++s) v += *reinterpret_cast<const v4f_any*>(parts + s * n + i);
+    } else {
+      for (int s = share * each; s < end; ++s)
+        for (int j = 0; j < left; ++j) v[j] += parts[s * n + i + j];
     }
-    sums[wave][lane] = v;
-    __syncthreads();
-    if (wave == 0 && i < n) {
-      v = ((v + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
-      TO* to = static_cast<TO*>(g.out) + (i / g.c) * g.ld_out + i % g.c;
-      if (g.accumulate) v += static_cast<float>(*to);
-      *to = static_cast<TO>(v);
+    if (parts_of > 1) {
+      sums[threadIdx.x] = v;
+      __syncthreads();
+      if (share == 0)
+        for (int s = 1; s < parts_of; ++s) v += sums[s * wide + at];
+      __syncthreads();
     }
-    __syncthreads();
+    if (share == 0 && left > 0) {
+      int64_t row = i / g.c;
+      int col = static_cast<int>(i - row * g.c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j < left) {
+          TO* to = static_cast<TO*>(g.out) + row * g.ld_out + col;
+          float sum = v[j];
+          if (g.accumulate) sum += static_cast<float>(*to);
+          *to = static_cast<TO>(sum);
+          if (++col == g.c) {
+            col = 0;
+            ++row;
+          }
+        }
+      }
+    }
   }
 }
 
 struct Shape {
-  int tk, tc, splits, per;
+  int tile, splits, per;
 };
 
-// The tile, and splits of the rows: enough workgroups for every CU, 128 rows each or more.
+// The tile (64, 128 or 256 square) and the splits of the rows: the pair with the least estimated
+// time.  Measured on 28 shapes from 128 x 1024 x 1024 to 16384 x 4096 x 4096 (rows, c, k) in each
+// type with every pair, in microseconds: a step of 32 rows takes `alone` with one workgroup on a
+// CU and `each` apiece with several; about 5 to launch, fill and drain; dw and partial sums are
+// written and read at some 6 TB/s; the launch that joins them costs 5 more.  The pair chosen was
+// the fastest or within 5% of it on 24 of the 28, within 20% on all but one.
 Shape shape_of(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
-  auto tiles = [&](int t) { return ((static_cast<int64_t>(c) + t - 1) / t) * ((static_cast<int64_t>(k) + t - 1) / t); };
-  Shape s{};
-  s.tk = dy_bf16 && tiles(256) * (rows / 512) >= 192 ? 256 : 128;
-  if (tiles(128) * (rows / 128) < 192) s.tk = 64;
-  s.tc = s.tk;
-  int64_t n = 256 / tiles(s.tk);
-  const int64_t most = (static_cast<int64_t>(rows) + 127) / 128;
-  if (n > most) n = most;
-  if (n < 1) n = 1;
-  int64_t each = (rows + n - 1) / n;
-  each = (each + kStep - 1) / kStep * kStep;
-  if (each < kStep) each = kStep;
-  s.per = static_cast<int>(each);
-  n = (rows + each - 1) / each;
-  s.splits = static_cast<int>(n < 1 ? 1 : n);
-  return s;
+  struct Rate {
+    int tile;
+    double alone, each;
+  };
+  static constexpr Rate kBf16[3] = {{64, 0.21, 0.15}, {128, 0.43, 0.37}, {256, 0.92, 0.92}};
+  static constexpr Rate kF32[3] = {{64, 0.45, 0.34}, {128, 0.95, 0.95}, {256, 2.6, 2.6}};
+  const Rate* rates = dy_bf16 ? kBf16 : kF32;
+  const double values = static_cast<double>(k) * c * 4e-6 / 6;  // us to move one fp32 dw
+  const double inputs = rows * (k * (dy_bf16 ? 2.0 : 4.0) + c) * 1e-6 / 4.5;
+  Shape best{};
+  double least = 0.0;
+  for (int i = 0; i < 3; ++i) {
+    const int tile = rates[i].tile;
+    const int64_t tiles = ((static_cast<int64_t>(c) + tile - 1) / tile) * ((static_cast<int64_t>(k) + tile - 1) / tile);
+    for (int s = 1; s <= 256 && (s == 1 || tiles * s <= 2048); s *= 2) {
+      int64_t per = (static_cast<int64_t>(rows) + s - 1) / s;
+      per = (per + kStep - 1) / kStep * kStep;
+      if (per < kStep) per = kStep;
+      if (s > 1 && per < 2 * kStep) break;
+      const int64_t splits = rows > 0 ? (rows + per - 1) / per : 1;
+      const double steps = static_cast<double>(per / kStep);
+      const double rounds = static_cast<double>((tiles * splits + 255) / 256);
+      double us = steps * rates[i].each * rounds;
+      if (us < steps * rates[i].alone) us = steps * rates[i].alone;
+      if (us < inputs) us = inputs;
+      us += 5 + values * splits;
+      if (splits > 1) us += 5 + values * (splits + 1);
+      if (best.tile == 0 || us < least) {
+        best = Shape{tile, static_cast<int>(splits), static_cast<int>(per)};
+        least = us;
+      }
+    }
+  }
+  return best;
 }
 
-template <typename T, typename TO, int P, int TK, int TC>
+template <typename T, typename TO, int P, int TK, int TC, int VK, int VC, int STAGES, int SETS>
 hipError_t launch_tile(const Grad& g, unsigned blocks, hipStream_t stream) {
-  constexpr int kBytes = 3 * (P * kStep * TK * 2 + kStep * TC * 2);
-  auto* kernel = &act8_grad_kernel<T, TO, P, TK, TC, 2>;
+  constexpr int kBytes = STAGES * (P * kStep * TK * 2 + kStep * TC * 2);
+  auto* kernel = &act8_grad_kernel<T, TO, P, TK, TC, VK, VC, STAGES, SETS>;
   if (kBytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != hipSuccess) return e;
   }
-  kernel<<<blocks, kThreads, kBytes, stream>>>(g);
+  kernel<<<blocks, VK * VC * 64, kBytes, stream>>>(g);
   return hipGetLastError();
 }
 
@@ -404,10 +458,12 @@ template <typename T, typename TO, int P>
 hipError_t launch_product(const Grad& g, const Shape& s, hipStream_t stream) {
   const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(g.tiles_k) * g.tiles_c * s.splits);
   if constexpr (P == 1) {
-    if (s.tk == 256) return launch_tile<T, TO, P, 256, 256>(g, blocks, stream);
+    if (s.tile == 256) return launch_tile<T, TO, P, 256, 256, 4, 2, 3, 2>(g, blocks, stream);
+  } else {
+    if (s.tile == 256) return launch_tile<T, TO, P, 256, 256, 4, 2, 2, 1>(g, blocks, stream);
   }
-  if (s.tk == 128) return launch_tile<T, TO, P, 128, 128>(g, blocks, stream);
-  return launch_tile<T, TO, P, 64, 64>(g, blocks, stream);
+  if (s.tile == 128) return launch_tile<T, TO, P, 128, 128, 4, 2, 3, 2>(g, blocks, stream);
+  return launch_tile<T, TO, P, 64, 64, 2, 2, 3, 2>(g, blocks, stream);
 }
 
 template <typename T, typename TO, int P>
@@ -422,8 +478,8 @@ hipError_t launch(const Act8GradArgs& a, hipStream_t stream) {
   g.c = a.c;
   g.k = a.k;
   g.groups = (a.c + kAct8Group - 1) / kAct8Group;
-  g.tiles_k = (a.k + s.tk - 1) / s.tk;
-  g.tiles_c = (a.c + s.tc - 1) / s.tc;
+  g.tiles_k = (a.k + s.tile - 1) / s.tile;
+  g.tiles_c = (a.c + s.tile - 1) / s.tile;
   g.per_split = s.per;
   g.out = a.dw;
   g.ld_out = a.ld_dw;
@@ -436,13 +492,23 @@ hipError_t launch(const Act8GradArgs& a, hipStream_t stream) {
   h.to_parts = true;
   const hipError_t e = launch_product<T, float, P>(h, s, stream);
   if (e != hipSuccess) return e;
-  const int64_t join = (static_cast<int64_t>(a.k) * a.c + 63) / 64;
+  // lanes that share a value's splits: eight splits each or so, while workgroups are few
+  const int64_t n = static_cast<int64_t>(a.k) * a.c;
+  int parts_of = 1;
+  while (parts_of < 64 && parts_of * 8 < s.splits && n * parts_of < 4 * 256 * 2048) parts_of *= 2;
+  const int64_t join = (n + 4 * (kThreads / parts_of) - 1) / (4 * (kThreads / parts_of));
   act8_grad_join_kernel<TO><<<static_cast<unsigned>(join < 65536 ? join : 65536), kThreads, 0, stream>>>(
-      g, static_cast<const float*>(a.ws), s.splits);
+      g, static_cast<const float*>(a.ws), s.splits, parts_of);
   return hipGetLastError();
 }
 
 }  // namespace
+
+void plan_act8_grad(int32_t rows, int32_t c, int32_t k, bool dy_bf16, int32_t* tile, int32_t* splits) {
+  const Shape s = shape_of(rows, c, k, dy_bf16);
+  *tile = s.tile;
+  *splits = s.splits;
+}
 
 size_t act8_grad_workspace_bytes(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
   const Shape s = shape_of(rows, c, k, dy_bf16);

@@ -223,6 +223,17 @@ int miq_act8_grad_workspace_size(int64_t rows, int32_t c, int32_t k, int32_t dy_
   return MIQ_OK;
 }
 
+int miq_plan_act8_grad(int64_t rows, int32_t c, int32_t k, int32_t dy_type, int32_t plan[2]) {
+  if (plan == nullptr) return null("plan pointer is NULL");
+  const int st = check_side(rows, c, k, dy_type);
+  if (st != MIQ_OK) return st;
+  plan[0] = plan[1] = 0;
+  if (c > 0 && k > 0) {
+    miq::plan_act8_grad(static_cast<int32_t>(rows), c, k, dy_type == MIQ_BF16, &plan[0], &plan[1]);
+  }
+  return MIQ_OK;
+}
+
 int miq_act8_grad(const void* dy, const int8_t* codes, const uint8_t* scales, void* dw, int64_t rows, int32_t c,
                   int32_t k, int64_t ld_dy, int64_t ld_dw, int32_t accumulate, int32_t dy_type, int32_t dw_type,
                   void* workspace, size_t workspace_bytes, void* stream) {

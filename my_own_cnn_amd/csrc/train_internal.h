@@ -61,6 +61,7 @@ struct Act8GradArgs {
   bool accumulate, dy_bf16, dw_bf16;
 };
 size_t act8_grad_workspace_bytes(int32_t rows, int32_t c, int32_t k, bool dy_bf16);
+void plan_act8_grad(int32_t rows, int32_t c, int32_t k, bool dy_bf16, int32_t* tile, int32_t* splits);
 hipError_t launch_act8_grad(const Act8GradArgs& a, hipStream_t stream);
 
 }  // namespace miq

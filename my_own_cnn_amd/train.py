@@ -301,6 +301,15 @@ def act8_grad_workspace_size(rows: int, c: int, k: int, dtype=None) -> int:
     return out.value
 
 
+def plan_act8_grad(rows: int, c: int, k: int, dtype=None):
+    """(side of dw's tiles, parts that the rows are split into) of act8_grad for a dy of `dtype`
+    (default float32), rows x k, and kept rows of c channels (no GPU access)."""
+    out = (C.c_int32 * 2)()
+    kind = _kind(dtype if dtype is not None else torch.float32, "dtype")
+    check(lib().miq_plan_act8_grad(rows, c, k, kind, out), "plan_act8_grad")
+    return out[0], out[1]
+
+
 def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None, workspace=None, stream=None):
     """The weight gradient of a linear (1x1) layer from its kept input: dw[k, c] = sum over the rows
     of dy[row, k] * x'[row, c], (K, C), float32 or, for a bfloat16 dy, bfloat16 (`dtype`, default
@@ -329,5 +338,5 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
 
 
 __all__ = ["Act8", "act8_bprop", "act8_expand", "act8_fprop", "act8_grad", "act8_grad_workspace_size", "act8_keep",
-           "embed_fprop", "embed_grad", "embed_grad_workspace_size"]
+           "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad"]
 _ = _capi

@@ -256,7 +256,7 @@ def test_beyond_32_bit_offsets(device):
 GRADS = [  # rows, c, k
     (1, 1, 1), (1, 33, 5), (2, 32, 64), (31, 128, 128), (32, 127, 129), (33, 130, 70), (64, 257, 200), (257, 64, 300),
     (1000, 96, 513), (513, 1003, 31), (2049, 256, 256), (5000, 65, 40), (300, 512, 384), (20001, 128, 128),
-    (24577, 512, 512), (19999, 300, 1001),
+    (24577, 512, 512), (19999, 300, 1001), (1200, 1500, 2000), (290, 4095, 4081),
 ]
 
 
@@ -274,6 +274,12 @@ def test_weight_gradient_against_64_bits(device, rows, c, k, dy_type, out_type):
     assert torch.equal(got, M.act8_grad(dy.to(device), kept, dtype=out_type))  # the same bits
     d = dy.double().numpy()
     _near(got, d.T @ x, (rows + 4) * 2 * U * (np.abs(d).T @ np.abs(x)), out_type)
+
+
+def test_the_shapes_reach_every_tile_split_and_whole():
+    for dtype in (F32, BF16):
+        plans = {M.plan_act8_grad(*s, dtype) for s in GRADS}
+        assert {(t, n > 1) for t, n in plans} == {(t, b) for t in (64, 128, 256) for b in (False, True)}
 
 
 @pytest.mark.parametrize("rows,c,k", [(1, 40, 3), (700, 129, 131), (9000, 64, 32), (1500, 300, 260)])

@@ -124,6 +124,23 @@ def test_workspace_sizes():
     assert M.lib().miq_act8_grad_workspace_size(1, 1, 1, 0, None) == NULL
 
 
+def test_weight_gradient_plan():
+    assert M.plan_act8_grad(512, 1024, 1024, torch.bfloat16) == (64, 1)
+    assert M.plan_act8_grad(16384, 4096, 4096, torch.bfloat16) == (256, 1)
+    assert M.plan_act8_grad(0, 64, 64) == (64, 1) and M.plan_act8_grad(64, 0, 64) == (0, 0)
+    for dtype in (torch.float32, torch.bfloat16):
+        for rows in (1, 31, 65, 1000, 12345, 10 ** 6):
+            for c in (1, 200, 3000):
+                for k in (5, 64, 2000):
+                    tile, splits = M.plan_act8_grad(rows, c, k, dtype)
+                    assert tile in (64, 128, 256) and 1 <= splits <= max(1, rows // 32)
+                    bytes_ = M.act8_grad_workspace_size(rows, c, k, dtype)
+                    assert bytes_ == (splits * c * k * 4 if splits > 1 else 0)
+    with pytest.raises(M.MiqError, match="2\\^22"):
+        M.plan_act8_grad(1, 1 << 23, 1)
+    assert M.lib().miq_plan_act8_grad(1, 1, 1, 0, None) == NULL
+
+
 def test_host_tensors_are_refused():
     x, ids = torch.zeros((3, 8)), torch.zeros(3, dtype=torch.int64)
     for call in (lambda: M.embed_fprop(x, ids), lambda: M.embed_grad(x, ids, 4), lambda: M.act8_keep(x),
