@@ -67,35 +67,37 @@ __device__ __forceinline__ void keep8(const v8f& v, int left, int8_t* codes, uin
   top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 1)));
   top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 2)));
   const int byte = exponent_byte(top);
-  // 2^(127 - byte), a normal number for every byte below 254; zero codes where the group is not finite
-  const float inverse = byte == 255 ? 0.0f : __uint_as_float(static_cast<unsigned>(254 - byte) << 23);
-  v8c q;
+  // 2^(127 - byte), a normal number for every byte below 254; the products are exact or below half
+  // a code, and adding 1.5 * 2^23 rounds them to nearest even into the low byte
+  const float inverse = __uint_as_float(static_cast<unsigned>(254 - min(byte, 253)) << 23);
+  float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float s = byte == 255 ? 0.0f : v[i] * inverse;  // exact, or below half a code
-    q[i] = static_cast<signed char>(static_cast<int>(__builtin_rintf(fminf(fmaxf(s, -127.0f), 127.0f))));
-  }
+  for (int i = 0; i < 8; ++i) r[i] = __builtin_amdgcn_fmed3f(v[i] * inverse, -127.0f, 127.0f) + 12582912.0f;
+  v2i q{static_cast<int>(pack4_magic(r[0], r[1], r[2], r[3])), static_cast<int>(pack4_magic(r[4], r[5], r[6], r[7]))};
+  if (byte == 255) q = v2i{};  // not a finite group
   if (left >= 8) {
-    *reinterpret_cast<v8c_any*>(codes) = q;
+    *reinterpret_cast<v2i_any*>(codes) = q;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < left) codes[i] = q[i];
+      if (i < left) codes[i] = static_cast<int8_t>(q[i / 4] >> (8 * (i & 3)));
   }
   if ((threadIdx.x & 3) == 0) *scale = static_cast<uint8_t>(byte);
 }
 
 __device__ __forceinline__ v8f kept8(const int8_t* codes, const uint8_t* scale, int left) {
-  v8c q = {};
+  v2i q = {};
   if (left >= 8) {
-    q = *reinterpret_cast<const v8c_any*>(codes);
+    q = *reinterpret_cast<const v2i_any*>(codes);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < left) q[i] = codes[i];
+      if (i < left) q[i / 4] |= (codes[i] & 0xff) << (8 * (i & 3));
   }
   // byte 255 is the bits of infinity, which a zero code makes NaN
-  return __builtin_convertvector(q, v8f) * __uint_as_float(static_cast<unsigned>(*scale) << 23);
+  const float s = __uint_as_float(static_cast<unsigned>(*scale) << 23);
+  const v4f lo = codes4(q[0]) * s, hi = codes4(q[1]) * s;
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 template <typename T, int ACT, bool GATED>

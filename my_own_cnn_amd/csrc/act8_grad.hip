@@ -21,8 +21,6 @@ constexpr int kStep = 32;  // rows m per step
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef int v2i __attribute__((ext_vector_type(2)));
-typedef v2i v2i_any __attribute__((aligned(1)));
 typedef v4i v4i_any __attribute__((aligned(1)));
 
 struct Grad {

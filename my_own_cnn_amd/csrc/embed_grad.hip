@@ -3,12 +3,17 @@
 // The (row, position) pairs of the tokens are sorted, stably, so that a row's tokens stand together
 // in order of position; a position without a token has the key `vocab` and sorts to the end.  Up
 // to kRankTokens tokens each token counts the ones before it directly, in one launch; above that
-// the keys go through stable counting passes of up to 10 bits.  The sorted list is then cut into
-// chunks of a fixed length: a group of lanes walks one chunk and 512 channels, adds the rows of dy
-// of each run of equal keys in fp32 and writes the runs that lie within its chunk.  A run that
-// reaches over a chunk's end leaves one partial sum per chunk in the workspace, and a last launch
-// adds those in order.  The cuts depend on the number of tokens and channels alone: every call
-// gives the same bits.
+// the keys go through stable counting passes of up to 10 bits, two launches each.  The sorted list
+// is then cut into chunks of a fixed length: a group of lanes walks one chunk and 512 channels,
+// adds the rows of dy of each run of equal keys in fp32 and writes the runs that lie within its
+// chunk.  A run that reaches over a chunk's end leaves one partial sum per chunk in the workspace,
+// and a last launch adds those in order.  The cuts depend on the number of tokens and channels
+// alone: every call gives the same bits.
+//
+// Rows without a token, most of the table in a common batch, are zeroed by workgroups of the
+// launch that adds.  A row has a token exactly if where[row] is a place of the sorted list that
+// holds its key: the sort writes where[] for the rows that it sees, and what the others hold is
+// tested, not trusted, so nothing has to be cleared.
 #include "train_device.h"
 
 namespace miq {
@@ -17,16 +22,19 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRankTokens = 8192;   // most tokens that are ranked by counting
 constexpr int kDigitBits = 10;      // most bits of a counting pass
+constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kCached = 4;          // keys per lane that a counting pass reads once
+constexpr int kSortBlocks = 64;     // most workgroups of a counting pass
 constexpr int kCols = 512;          // channels per wave: 64 lanes of 8
 constexpr int kZeroRows = 32;       // table rows per workgroup that zeros rows without a token
-constexpr int kAhead = 8;           // rows of dy in flight per lane
+constexpr int kAhead = 4;           // rows of dy in flight per lane
 
 struct Plan {
   int bits, passes, digit_bits, blocks, per_block;  // counting passes
   int lanes, col_tiles, len, chunks;                // lanes per chunk, chunk length
-  size_t keys0, keys1, order0, order1, hist, part, total;
+  size_t keys0, keys1, order0, order1, hist, where, part, total;
 };
 
 size_t up(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -37,10 +45,10 @@ Plan make_plan(int32_t vocab, int32_t c, int32_t tokens) {
   while ((static_cast<int64_t>(vocab) >> p.bits) != 0) ++p.bits;  // keys 0 .. vocab
   p.passes = (p.bits + kDigitBits - 1) / kDigitBits;
   p.digit_bits = (p.bits + p.passes - 1) / p.passes;
-  // workgroups of the counting passes: 2048 tokens or more each, at most 256
+  // workgroups of the counting passes: 1024 tokens or more each
   const int64_t t = tokens;
-  int64_t per = (t + 255) / 256;
-  per = (per < 2048 ? 2048 : per + kSortThreads - 1) / kSortThreads * kSortThreads;
+  int64_t per = (t + kSortBlocks - 1) / kSortBlocks;
+  per = ((per < 1024 ? 1024 : per) + kSortThreads - 1) / kSortThreads * kSortThreads;
   p.per_block = static_cast<int>(per);
   p.blocks = static_cast<int>((t + per - 1) / per);
   if (t <= kRankTokens) p.passes = 0;
@@ -62,6 +70,7 @@ Plan make_plan(int32_t vocab, int32_t c, int32_t tokens) {
     p.order1 = at; at += list;
     p.hist = at; at += up((static_cast<size_t>(p.blocks) << p.digit_bits) * 4);
   }
+  p.where = at; at += up(static_cast<size_t>(vocab) * 4);
   p.part = at; at += static_cast<size_t>(p.chunks) * 2 * p.col_tiles * (p.lanes * 8) * 4;
   p.total = at;
   return p;
@@ -77,26 +86,37 @@ __device__ __forceinline__ unsigned key_of(const void* ids, bool wide, int64_t t
 // 64 tokens per workgroup, one per lane; the 16 waves share the tokens to compare with.
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const void* __restrict__ ids, bool ids64, int tokens,
                                                           unsigned vocab, unsigned* __restrict__ keys,
-                                                          int* __restrict__ order) {
-  __shared__ unsigned all[kRankTokens];
+                                                          int* __restrict__ order, unsigned* __restrict__ where) {
+  typedef unsigned v4u __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) unsigned all[kRankTokens];
   __shared__ int counts[16][64];
-  for (int i = threadIdx.x; i < tokens; i += 1024) all[i] = key_of(ids, ids64, i, vocab);
+  const int padded = (tokens + 63) & ~63;  // past the tokens: keys that sort before nothing
+  for (int i = threadIdx.x; i < padded; i += 1024) all[i] = i < tokens ? key_of(ids, ids64, i, vocab) : ~0u;
   __syncthreads();
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int t0 = blockIdx.x * 64;
   const int t = t0 + lane;
-  const unsigned mine = t < tokens ? all[t] : 0;
+  const unsigned mine = all[t];
   int n = 0;
-  // waves 0 .. 15 take every 16th group of 64 tokens
-  for (int g = wave * 64; g < tokens; g += 1024) {
-    const int end = min(g + 64, tokens);
-    if (g < t0) {
-      for (int i = g; i < end; ++i) n += all[i] <= mine;
-    } else if (g > t0) {
-      for (int i = g; i < end; ++i) n += all[i] < mine;
+  // waves 0 .. 15 take every 16th group of 64 tokens: equal keys count where they come before
+  for (int g = wave * 64; g < padded; g += 1024) {
+    const unsigned least = g < t0 ? mine : mine - 1;  // all[i] <= least; a key 0 has none before it
+    if (g != t0) {
+      if (g < t0 || mine != 0) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          const v4u k = *reinterpret_cast<const v4u*>(&all[g + i]);
+          n += (k[0] <= least) + (k[1] <= least) + (k[2] <= least) + (k[3] <= least);
+        }
+      }
     } else {
-      for (int i = g; i < end; ++i) n += all[i] < mine || (all[i] == mine && i < t);
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        const v4u k = *reinterpret_cast<const v4u*>(&all[g + i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n += k[j] < mine || (k[j] == mine && i + j < lane);
+      }
     }
   }
   counts[wave][lane] = n;
@@ -107,6 +127,7 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const void* __restrict
     for (int w = 0; w < 16; ++w) place += counts[w][lane];
     keys[place] = mine;
     order[place] = t;
+    if (mine < vocab) where[mine] = static_cast<unsigned>(place);
   }
 }
 
@@ -125,9 +146,9 @@ __device__ __forceinline__ unsigned pass_key(const Pass& p, int t) {
   return p.keys_in != nullptr ? p.keys_in[t] : key_of(p.ids, p.ids64, t, p.vocab);
 }
 
-// hist[digit][block]: the tokens of each workgroup's range by digit
+// hist[workgroup][digit]: the tokens of each workgroup's range by digit
 __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(Pass p, unsigned* __restrict__ hist) {
-  __shared__ unsigned n[1 << kDigitBits];
+  __shared__ unsigned n[kDigits];
   for (int d = threadIdx.x; d < p.digits; d += kSortThreads) n[d] = 0;
   __syncthreads();
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.per_block;
@@ -135,82 +156,106 @@ __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(Pass p, unsign
   for (int64_t t = begin + threadIdx.x; t < end; t += kSortThreads)
     atomicAdd(&n[(pass_key(p, static_cast<int>(t)) >> p.shift) & (p.digits - 1)], 1u);
   __syncthreads();
-  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) hist[static_cast<size_t>(d) * p.blocks + blockIdx.x] = n[d];
-}
-
-// hist -> the place of each (digit, workgroup)'s first token; one workgroup, one digit per thread
-__global__ __launch_bounds__(1 << kDigitBits) void embed_scan_kernel(unsigned* __restrict__ hist, int digits,
-                                                                     int blocks) {
-  __shared__ unsigned sums[1 << kDigitBits];
-  const int d = threadIdx.x;
-  unsigned total = 0;
-  if (d < digits)
-    for (int b = 0; b < blocks; ++b) total += hist[static_cast<size_t>(d) * blocks + b];
-  sums[d] = total;
-  __syncthreads();
-  for (int step = 1; step < (1 << kDigitBits); step *= 2) {
-    const unsigned before = d >= step ? sums[d - step] : 0;
-    __syncthreads();
-    sums[d] += before;
-    __syncthreads();
-  }
-  if (d < digits) {
-    unsigned at = sums[d] - total;
-    for (int b = 0; b < blocks; ++b) {
-      unsigned& h = hist[static_cast<size_t>(d) * blocks + b];
-      const unsigned n = h;
-      h = at;
-      at += n;
-    }
-  }
+  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) hist[blockIdx.x * p.digits + d] = n[d];
 }
 
 // Each wave takes a contiguous part of its workgroup's range, 64 tokens at a time in order: a
 // token's place is its wave's running place of its digit plus the lanes before it with that digit.
+// `where` (or NULL): a place of each key.
 __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(Pass p, const unsigned* __restrict__ hist,
                                                                      unsigned* __restrict__ keys,
-                                                                     int* __restrict__ order) {
-  __shared__ unsigned at[kSortWaves][1 << kDigitBits];
+                                                                     int* __restrict__ order,
+                                                                     unsigned* __restrict__ where) {
+  __shared__ unsigned at[kSortWaves][kDigits];
+  __shared__ unsigned sums[kSortWaves];
   const int wave = threadIdx.x >> 6;
   const int lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < kSortWaves * p.digits; i += kSortThreads) at[i / p.digits][i % p.digits] = 0;
-  __syncthreads();
   const int part = p.per_block / kSortWaves;  // a multiple of 64
-  const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.per_block + wave * part;
+  const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.per_block + wave * static_cast<int64_t>(part);
   const int64_t end = min(begin + part, static_cast<int64_t>(p.tokens));
-  for (int64_t t = begin + lane; t < end; t += 64)
-    atomicAdd(&at[wave][(pass_key(p, static_cast<int>(t)) >> p.shift) & (p.digits - 1)], 1u);
+  // the wave's first keys stay in registers between counting and placing
+  auto pass_pos = [&](int64_t t) { return p.order_in != nullptr ? p.order_in[t] : static_cast<int>(t); };
+  unsigned cache[kCached];
+  int cached_pos[kCached];
+#pragma unroll
+  for (int i = 0; i < kCached; ++i) {
+    const int64_t t = begin + i * 64 + lane;
+    cache[i] = t < end ? pass_key(p, static_cast<int>(t)) : 0;
+    cached_pos[i] = t < end ? pass_pos(t) : 0;
+  }
+  // two digits per thread: the tokens of a digit in all workgroups, and in those before this one
+  static_assert(kDigits == 2 * kSortThreads, "");
+  const int d0 = threadIdx.x * 2;
+  unsigned total[2] = {}, before[2] = {};
+  if (d0 < p.digits) {
+#pragma unroll 16
+    for (int b = 0; b < p.blocks; ++b) {
+      const v2i h = *reinterpret_cast<const v2i*>(hist + b * p.digits + d0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        total[i] += static_cast<unsigned>(h[i]);
+        before[i] += b < static_cast<int>(blockIdx.x) ? static_cast<unsigned>(h[i]) : 0;
+      }
+    }
+  }
+  for (int w = 0; w < kSortWaves; ++w)
+    for (int d = threadIdx.x; d < p.digits; d += kSortThreads) at[w][d] = 0;
   __syncthreads();
-  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) {
-    unsigned place = hist[static_cast<size_t>(d) * p.blocks + blockIdx.x];
-    for (int w = 0; w < kSortWaves; ++w) {
-      const unsigned n = at[w][d];
-      at[w][d] = place;
-      place += n;
+#pragma unroll
+  for (int i = 0; i < kCached; ++i)
+    if (begin + i * 64 + lane < end) atomicAdd(&at[wave][(cache[i] >> p.shift) & (p.digits - 1)], 1u);
+  for (int64_t t = begin + kCached * 64 + lane; t < end; t += 64)
+    atomicAdd(&at[wave][(pass_key(p, static_cast<int>(t)) >> p.shift) & (p.digits - 1)], 1u);
+  // the place of this thread's first digit: the tokens of all digits before it
+  unsigned first = total[0] + total[1];
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) {
+    const unsigned left = __shfl_up(first, step);
+    first += lane >= step ? left : 0;
+  }
+  if (lane == 63) sums[wave] = first;
+  first -= total[0] + total[1];
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) first += sums[w];
+  if (d0 < p.digits) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned place = first + before[i];
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) {
+        const unsigned n = at[w][d0 + i];
+        at[w][d0 + i] = place;
+        place += n;
+      }
+      first += total[i];
     }
   }
   __syncthreads();
-  for (int64_t t0 = begin; t0 < end; t0 += 64) {
-    const int64_t t = t0 + lane;
-    const bool there = t < end;
-    const unsigned key = there ? pass_key(p, static_cast<int>(t)) : 0;
-    const int pos = there ? (p.order_in != nullptr ? p.order_in[t] : static_cast<int>(t)) : 0;
+  auto put = [&](bool there, unsigned key, int pos) {
     const unsigned digit = (key >> p.shift) & (p.digits - 1);
     uint64_t same = __ballot(there);
     for (int bit = 1; bit < p.digits; bit *= 2) {
       const uint64_t set = __ballot((digit & bit) != 0);
       same &= (digit & bit) != 0 ? set : ~set;
     }
-    const int before = __popcll(same & ((uint64_t{1} << lane) - 1));
+    const int earlier = __popcll(same & ((uint64_t{1} << lane) - 1));
     unsigned place = 0;
-    if (there) place = at[wave][digit] + before;
+    if (there) place = at[wave][digit] + earlier;
     __builtin_amdgcn_wave_barrier();
-    if (there && before == 0) at[wave][digit] += __popcll(same);
+    if (there && earlier == 0) at[wave][digit] += __popcll(same);
     __builtin_amdgcn_wave_barrier();
     if (there) {
       keys[place] = key;
       order[place] = pos;
+      if (where != nullptr && key < p.vocab) where[key] = place;
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kCached; ++i)
+    if (begin + i * 64 < end) put(begin + i * 64 + lane < end, cache[i], cached_pos[i]);
+  for (int64_t t0 = begin + kCached * 64; t0 < end; t0 += 64) {
+    const int64_t t = t0 + lane;
+    put(t < end, t < end ? pass_key(p, static_cast<int>(t)) : 0, t < end ? pass_pos(t) : 0);
   }
 }
 
@@ -222,6 +267,7 @@ struct Sum {
   TO* table;
   const unsigned* keys;
   const int* order;
+  const unsigned* where;  // a place of each row's key, for rows that have a token
   float* part;
   int64_t ld_dy, ld_table;
   int tokens, c, lanes, col_tiles, len, chunks, sum_blocks;
@@ -231,20 +277,91 @@ struct Sum {
 
   // partial sums: [chunk][0: the run that reaches in, 1: the run that starts here and reaches on]
   __device__ float* slot(int chunk, int which, int tile, int lane) const {
-    return part + ((static_cast<int64_t>(chunk) * 2 + which) * col_tiles + tile) * (lanes * 8) + lane * 8;
+    return part + ((static_cast<int64_t>(chunk) * 2 + which) * col_tiles + tile) * (lanes * 8) + lane * 4;
   }
-  __device__ void finish(unsigned row, int col, v8f acc) const {
+  // A lane's channels: four from `col` and four `apart` from there.  Where the row ends within a
+  // four, the lane takes the row's last four instead, as its neighbour does in part: both write the
+  // same values.  Adding to the table is no place for that; there such a lane is not `whole` and
+  // goes value by value.  False for a lane beyond the row.
+  __device__ bool place(int tile, int lane, int* col, int* apart, bool* whole) const {
+    const int first = tile * kCols + lane * 4;
+    const int second = first + lanes * 4;
+    *whole = second + 4 <= c || (c >= 4 && !accumulate);
+    *col = first;
+    *apart = lanes * 4;
+    if (second + 4 > c && *whole) {
+      *col = min(first, c - 4);
+      *apart = second < c ? c - 4 - *col : 0;
+    }
+    return first < c;
+  }
+  __device__ void finish(unsigned row, int col, int apart, bool whole, v8f acc) const {
     TO* to = table + row * ld_table + col;
     acc *= scale;
-    if (accumulate) acc += load8_of(to, c - col);
-    store8_of(to, acc, c - col);
+    if (whole) {
+      if (accumulate) acc += load44(to, apart);
+      store44(to, apart, acc);
+    } else {
+      if (accumulate) acc += load44_of(to, apart, c - col);
+      store44_of(to, apart, acc, c - col);
+    }
   }
 };
 
+// Zeros in the rows [first, first + kZeroRows) that no token names.
 template <typename TI, typename TO>
-__device__ __forceinline__ void sum_chunk(const Sum<TI, TO>& s, int chunk, int tile, int lane) {
-  const int col = tile * kCols + lane * 8;
-  if (chunk >= s.chunks || col >= s.c) return;
+__device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
+  __shared__ int empty[kZeroRows];
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kZeroRows), s.vocab - first));
+  if (static_cast<int>(threadIdx.x) < rows) {
+    bool none = true;
+    if (s.tokens > 0) {  // else there is no workspace
+      const unsigned row = static_cast<unsigned>(first) + threadIdx.x;
+      const unsigned at = s.where[row];
+      none = at >= static_cast<unsigned>(s.tokens) || s.keys[at] != row;
+    }
+    empty[threadIdx.x] = none;
+  }
+  __syncthreads();
+  for (int r = 0; r < rows; ++r) {
+    if (!empty[r]) continue;
+    TO* const row = s.table + (first + r) * s.ld_table;
+    if (s.c < 4) {
+      if (static_cast<int>(threadIdx.x) < s.c) row[threadIdx.x] = static_cast<TO>(0.0f);
+    } else {
+#pragma unroll 2
+      for (int col = threadIdx.x * 4; col < s.c; col += kThreads * 4) store4(row + min(col, s.c - 4), v4f{});
+    }
+  }
+}
+
+// A lane's eight values of a row of dy, as loaded.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+  v4f lo, hi;
+};
+template <>
+struct Raw8<__bf16> {
+  v4bf lo, hi;
+};
+__device__ __forceinline__ void load_raw(Raw8<float>& r, const float* p, int apart) {
+  r.lo = *reinterpret_cast<const v4f_any*>(p);
+  r.hi = *reinterpret_cast<const v4f_any*>(p + apart);
+}
+__device__ __forceinline__ void load_raw(Raw8<__bf16>& r, const __bf16* p, int apart) {
+  r.lo = *reinterpret_cast<const v4bf_any*>(p);
+  r.hi = *reinterpret_cast<const v4bf_any*>(p + apart);
+}
+template <typename T>
+__device__ __forceinline__ v8f value(const Raw8<T>& r) {
+  return __builtin_convertvector(__builtin_shufflevector(r.lo, r.hi, 0, 1, 2, 3, 4, 5, 6, 7), v8f);
+}
+
+// WHOLE: the lane's loads of kAhead rows leave together.
+template <bool WHOLE, typename TI, typename TO>
+__device__ __forceinline__ void sum_chunk(const Sum<TI, TO>& s, int chunk, int tile, int lane, int col, int apart) {
   const int begin = chunk * s.len;
   const int end = min(static_cast<int64_t>(begin) + s.len, static_cast<int64_t>(s.tokens));
   unsigned cur = s.keys[begin];
@@ -254,72 +371,73 @@ __device__ __forceinline__ void sum_chunk(const Sum<TI, TO>& s, int chunk, int t
   v8f acc = {};
   auto flush = [&]() {
     if (reaches_in) {
-      store8(s.slot(chunk, 0, tile, lane), acc);
+      store44(s.slot(chunk, 0, tile, lane), s.lanes * 4, acc);
     } else {
-      s.finish(cur, col, acc);
+      s.finish(cur, col, apart, WHOLE, acc);
     }
     reaches_in = false;
     acc = v8f{};
   };
-  for (int i = begin; i < end; i += kAhead) {
-    unsigned key[kAhead];
-    v8f row[kAhead];
+  // The lists are read kAhead entries at a time, past the chunk's end too: they are padded to that.
+  v4i key[kAhead / 4], pos[kAhead / 4];
+  auto list = [&](int i) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      key[j] = i + j < end ? s.keys[i + j] : s.vocab;
-      const int t = i + j < end ? s.order[i + j] : 0;
-      row[j] = key[j] < s.vocab ? load8_of(s.dy + t * s.ld_dy + col, left) : v8f{};
+    for (int j = 0; j < kAhead / 4; ++j) {
+      key[j] = *reinterpret_cast<const v4i*>(s.keys + i + 4 * j);
+      pos[j] = *reinterpret_cast<const v4i*>(s.order + i + 4 * j);
     }
+  };
+  list(begin);
+  for (int i = begin; i < end; i += kAhead) {
+    unsigned k[kAhead];
+    Raw8<TI> row[kAhead];
+    v8f part[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (i + j < end && cur < s.vocab) {
-        if (key[j] != cur) {
+      // a token without a row is read like any other, an entry past the end as the chunk's first
+      k[j] = static_cast<unsigned>(key[j / 4][j & 3]);
+      const int64_t t = i + j < end ? pos[j / 4][j & 3] : s.order[begin];
+      const TI* from = s.dy + t * s.ld_dy + col;
+      if constexpr (WHOLE) {
+        load_raw(row[j], from, apart);
+      } else {
+        part[j] = load44_of(from, apart, left);
+      }
+    }
+    if (i + kAhead < end) list(i + kAhead);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i + j < end) {
+        if (k[j] != cur) {
           flush();
-          cur = key[j];
+          cur = k[j];
         }
-        acc += row[j];
+        if (cur >= s.vocab) return;  // the rest are tokens without a row
+        acc += WHOLE ? value(row[j]) : part[j];
       }
     }
   }
-  if (cur >= s.vocab) return;
   if (end < s.tokens && s.keys[end] == cur) {
-    store8(s.slot(chunk, reaches_in ? 0 : 1, tile, lane), acc);
+    store44(s.slot(chunk, reaches_in ? 0 : 1, tile, lane), s.lanes * 4, acc);
   } else {
     flush();
   }
 }
 
-// Zeros in the rows [first, first + kZeroRows) that no token names.
 template <typename TI, typename TO>
-__device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
-  __shared__ int starts[kZeroRows + 1];
-  const int rows = static_cast<int>(min(static_cast<int64_t>(kZeroRows), s.vocab - first));
-  if (threadIdx.x <= rows) {  // the first place of row first + threadIdx.x
-    const unsigned row = static_cast<unsigned>(first) + threadIdx.x;
-    int lo = 0, hi = s.tokens;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      if (s.keys[mid] < row) lo = mid + 1;
-      else hi = mid;
-    }
-    starts[threadIdx.x] = lo;
-  }
-  __syncthreads();
-  for (int r = 0; r < rows; ++r) {
-    if (starts[r] != starts[r + 1]) continue;
-    for (int col = threadIdx.x * 8; col < s.c; col += kThreads * 8)
-      store8_of(s.table + (first + r) * s.ld_table + col, v8f{}, s.c - col);
-  }
-}
-
-template <typename TI, typename TO>
-__global__ __launch_bounds__(kThreads) void embed_sum_kernel(Sum<TI, TO> s) {
-  if (static_cast<int>(blockIdx.x) < s.sum_blocks) {
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / s.lanes;
-    sum_chunk(s, static_cast<int>(unit / s.col_tiles), static_cast<int>(unit % s.col_tiles), threadIdx.x & (s.lanes - 1));
-  } else {
+__global__ __launch_bounds__(kThreads, sizeof(TI) == 2 ? 6 : 5) void embed_sum_kernel(Sum<TI, TO> s) {
+  if (static_cast<int>(blockIdx.x) >= s.sum_blocks) {
     zero_rows(s, static_cast<int64_t>(blockIdx.x - s.sum_blocks) * kZeroRows);
+    return;
   }
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / s.lanes;
+  const int chunk = static_cast<int>(unit / s.col_tiles), tile = static_cast<int>(unit % s.col_tiles);
+  const int lane = threadIdx.x & (s.lanes - 1);
+  int col, apart;
+  bool whole;
+  if (!s.place(tile, lane, &col, &apart, &whole) || chunk >= s.chunks) return;
+  if (whole) sum_chunk<true>(s, chunk, tile, lane, col, apart);
+  else sum_chunk<false>(s, chunk, tile, lane, col, apart);
 }
 
 // Adds the partial sums of the run that starts in chunk blockIdx.x / col_tiles and reaches over
@@ -342,34 +460,61 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(Sum<TI, TO> s) {
     more += __popcll(same);
     if (same != ~uint64_t{0}) break;
   }
-  const int col = tile * kCols + lane * 8;
-  const bool there = lane < s.lanes && col < s.c;
+  int col, apart;
+  bool whole;
+  const bool there = s.place(tile, lane, &col, &apart, &whole) && lane < s.lanes;
   const int each = (more + 1 + 3) / 4;
   const int from = wave * each;
   const int to = min(from + each, more + 1);
   v8f acc = {};
   if (there) {
-#pragma unroll 4
-    for (int i = from; i < to; ++i) acc += load8(s.slot(chunk + i, i == 0 ? 1 : 0, tile, lane));
+#pragma unroll 8
+    for (int i = from; i < to; ++i) acc += load44(s.slot(chunk + i, i == 0 ? 1 : 0, tile, lane), s.lanes * 4);
   }
   parts[wave][lane] = acc;
   __syncthreads();
   if (wave == 0 && there) {
 #pragma unroll
     for (int w = 1; w < 4; ++w) acc += parts[w][lane];
-    s.finish(key, col, acc);
+    s.finish(key, col, apart, whole, acc);
   }
 }
 
 template <typename TI, typename TO>
-hipError_t launch_sums(const EmbedGradArgs& a, const Plan& p, const unsigned* keys, const int* order,
-                       hipStream_t stream) {
+hipError_t launch(const EmbedGradArgs& a, hipStream_t stream) {
+  const Plan p = make_plan(a.vocab, a.c, a.tokens);
+  char* ws = static_cast<char*>(a.ws);
+  const unsigned vocab = static_cast<unsigned>(a.vocab);
+  unsigned* keys = reinterpret_cast<unsigned*>(ws + p.keys0);
+  int* order = reinterpret_cast<int*>(ws + p.order0);
+  unsigned* where = reinterpret_cast<unsigned*>(ws + p.where);
+  if (a.tokens > 0 && p.passes == 0) {
+    embed_rank_kernel<<<(a.tokens + 63) / 64, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order, where);
+  } else if (a.tokens > 0) {
+    unsigned* keys_to = reinterpret_cast<unsigned*>(ws + p.keys1);
+    int* order_to = reinterpret_cast<int*>(ws + p.order1);
+    unsigned* hist = reinterpret_cast<unsigned*>(ws + p.hist);
+    for (int i = 0; i < p.passes; ++i) {
+      Pass s{i == 0 ? nullptr : keys, i == 0 ? nullptr : order, a.ids, a.ids64, vocab, a.tokens, p.per_block, p.blocks,
+             i * p.digit_bits, 1 << p.digit_bits};
+      embed_hist_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s, hist);
+      embed_scatter_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s, hist, keys_to, order_to,
+                                                                  i == p.passes - 1 ? where : nullptr);
+      unsigned* k = keys;
+      keys = keys_to;
+      keys_to = k;
+      int* o = order;
+      order = order_to;
+      order_to = o;
+    }
+  }
   Sum<TI, TO> s{};
   s.dy = static_cast<const TI*>(a.dy);
   s.table = static_cast<TO*>(a.dtable);
   s.keys = keys;
   s.order = order;
-  s.part = reinterpret_cast<float*>(static_cast<char*>(a.ws) + p.part);
+  s.where = where;
+  s.part = reinterpret_cast<float*>(ws + p.part);
   s.ld_dy = a.ld_dy;
   s.ld_table = a.ld_dtable;
   s.tokens = a.tokens;
@@ -378,7 +523,7 @@ hipError_t launch_sums(const EmbedGradArgs& a, const Plan& p, const unsigned* ke
   s.col_tiles = p.col_tiles;
   s.len = p.len;
   s.chunks = p.chunks;
-  s.vocab = static_cast<unsigned>(a.vocab);
+  s.vocab = vocab;
   s.scale = a.scale;
   s.accumulate = a.accumulate;
   const int64_t units = static_cast<int64_t>(p.chunks) * p.col_tiles;
@@ -398,37 +543,8 @@ size_t embed_grad_workspace_bytes(int32_t vocab, int32_t c, int32_t tokens) {
 }
 
 hipError_t launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {
-  const Plan p = make_plan(a.vocab, a.c, a.tokens);
-  char* ws = static_cast<char*>(a.ws);
-  unsigned* keys = reinterpret_cast<unsigned*>(ws + p.keys0);
-  int* order = reinterpret_cast<int*>(ws + p.order0);
-  const unsigned vocab = static_cast<unsigned>(a.vocab);
-  if (a.tokens > 0 && p.passes == 0) {
-    embed_rank_kernel<<<(a.tokens + 63) / 64, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order);
-  } else if (a.tokens > 0) {
-    unsigned* keys_to = reinterpret_cast<unsigned*>(ws + p.keys1);
-    int* order_to = reinterpret_cast<int*>(ws + p.order1);
-    unsigned* hist = reinterpret_cast<unsigned*>(ws + p.hist);
-    for (int i = 0; i < p.passes; ++i) {
-      Pass s{i == 0 ? nullptr : keys, i == 0 ? nullptr : order, a.ids, a.ids64, vocab, a.tokens, p.per_block, p.blocks,
-             i * p.digit_bits, 1 << p.digit_bits};
-      embed_hist_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s, hist);
-      embed_scan_kernel<<<1, 1 << kDigitBits, 0, stream>>>(hist, s.digits, p.blocks);
-      embed_scatter_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s, hist, keys_to, order_to);
-      unsigned* k = keys;
-      keys = keys_to;
-      keys_to = k;
-      int* o = order;
-      order = order_to;
-      order_to = o;
-    }
-  }
-  if (a.dy_bf16) {
-    return a.dtable_bf16 ? launch_sums<__bf16, __bf16>(a, p, keys, order, stream)
-                         : launch_sums<__bf16, float>(a, p, keys, order, stream);
-  }
-  return a.dtable_bf16 ? launch_sums<float, __bf16>(a, p, keys, order, stream)
-                       : launch_sums<float, float>(a, p, keys, order, stream);
+  if (a.dy_bf16) return a.dtable_bf16 ? launch<__bf16, __bf16>(a, stream) : launch<__bf16, float>(a, stream);
+  return a.dtable_bf16 ? launch<float, __bf16>(a, stream) : launch<float, float>(a, stream);
 }
 
 }  // namespace miq

@@ -10,12 +10,12 @@ namespace {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v8f __attribute__((ext_vector_type(8)));
-typedef signed char v8c __attribute__((ext_vector_type(8)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 // Rows start at any multiple of the element's size: global memory takes 16-byte accesses at any
 // address, so odd row lengths run the same loads and stores as aligned ones.
 typedef v8bf v8bf_any __attribute__((aligned(2)));
 typedef v4f v4f_any __attribute__((aligned(4)));
-typedef v8c v8c_any __attribute__((aligned(1)));
+typedef v2i v2i_any __attribute__((aligned(1)));
 
 __device__ __forceinline__ v8f load8(const float* p) {
   const v4f a = *reinterpret_cast<const v4f_any*>(p), b = *reinterpret_cast<const v4f_any*>(p + 4);
@@ -56,6 +56,51 @@ __device__ __forceinline__ void store8_of(T* p, const v8f& v, int n) {
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < n) p[i] = static_cast<T>(v[i]);
+}
+
+// Eight values as two runs of four, `apart` elements from each other: neighbouring lanes' runs are
+// neighbours in memory, so that every store of a wave covers whole lines.
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+typedef v4bf v4bf_any __attribute__((aligned(2)));
+
+__device__ __forceinline__ v4f load4(const float* p) { return *reinterpret_cast<const v4f_any*>(p); }
+__device__ __forceinline__ v4f load4(const __bf16* p) {
+  return __builtin_convertvector(*reinterpret_cast<const v4bf_any*>(p), v4f);
+}
+__device__ __forceinline__ void store4(float* p, const v4f& v) {
+  *reinterpret_cast<v4f_any*>(p) = v;
+  store_gap(v);
+}
+__device__ __forceinline__ void store4(__bf16* p, const v4f& v) {
+  *reinterpret_cast<v4bf_any*>(p) = __builtin_convertvector(v, v4bf);  // to nearest even
+}
+template <typename T>
+__device__ __forceinline__ v8f load44(const T* p, int apart) {
+  return __builtin_shufflevector(load4(p), load4(p + apart), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <typename T>
+__device__ __forceinline__ void store44(T* p, int apart, const v8f& v) {
+  store4(p, __builtin_shufflevector(v, v, 0, 1, 2, 3));
+  store4(p + apart, __builtin_shufflevector(v, v, 4, 5, 6, 7));
+}
+// Of a row that ends n elements after p.
+template <typename T>
+__device__ __forceinline__ v8f load44_of(const T* p, int apart, int n) {
+  v8f v = {};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (h * apart + i < n) v[4 * h + i] = static_cast<float>(p[h * apart + i]);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store44_of(T* p, int apart, const v8f& v, int n) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (h * apart + i < n) p[h * apart + i] = static_cast<T>(v[4 * h + i]);
 }
 
 // Four int8 codes of a word as fp32, one conversion with a byte select each.  (A vector conversion

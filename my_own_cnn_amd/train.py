@@ -53,18 +53,19 @@ def _act(act: str) -> int:
 
 
 def _on_device(t, what: str) -> None:
-    if not t.is_cuda:
+    at = t.get_device()
+    if at < 0:
         raise ValueError(f"{what} must live in device memory")
-    if t.get_device() != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+    if at != (_current_device() if _current_device is not None else torch.cuda.current_device()):
         raise ValueError(f"{what} must live on the current device")
 
 
 def _rows(t, what: str):
     """(rows, channels, row distance) of a tensor (..., C)."""
     _on_device(t, what)
-    if t.dim() == 0:
-        raise ValueError(f"{what} must have a channel dimension")
     shape = t.shape
+    if not shape:
+        raise ValueError(f"{what} must have a channel dimension")
     c = shape[-1]
     if t.is_contiguous():
         return (t.numel() // c if c else 0), c, c
@@ -102,12 +103,15 @@ def _alloc(shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _output(out, shape, dtype, device, stream):
+def _output(out, shape, dtype, like, stream):
+    """(tensor, row distance) of a call's result: `out`, or a new one on the device of `like`."""
     if out is None:
-        return _alloc(shape, dtype, device, stream)
+        if stream is None:
+            return like.new_empty(shape, dtype=dtype), shape[-1]
+        return _alloc(shape, dtype, like.device, stream), shape[-1]
     if out.shape != shape or out.dtype != dtype:
         raise ValueError(f"out must be {dtype} of shape {tuple(shape)}")
-    return out
+    return out, _rows(out, "out")[2]
 
 
 _sizes = {}  # workspace bytes by problem
@@ -145,14 +149,17 @@ def embed_fprop(table, ids, *, scale: float = 1.0, dtype=None, out=None, stream=
         raise ValueError("table must be (vocab, channels)")
     if ids.dtype not in _IDS:
         raise ValueError(f"ids must be int32 or int64, got {ids.dtype}")
-    vocab, c, ld = _rows(table, "table")
+    _, c, ld = _rows(table, "table")
     vocab = table.shape[0]
     ids_at = _dense(ids, ids.dtype, "ids")
-    y = _output(out, ids.shape + (c,), dtype if dtype is not None else (out.dtype if out is not None else table.dtype),
-                table.device, stream)
-    _, _, ld_y = _rows(y, "out")
-    check(lib().miq_embed_fprop(table.data_ptr(), ids_at, y.data_ptr(), vocab, c, ids.numel(), ld, ld_y, scale, kind,
-                                _IDS[ids.dtype], _kind(y.dtype, "out"), _stream(stream)), "embed_fprop")
+    if dtype is None:
+        dtype = out.dtype if out is not None else table.dtype
+    y_kind = _kind(dtype, "dtype")
+    y, ld_y = _output(out, ids.shape + (c,), dtype, table, stream)
+    status = lib().miq_embed_fprop(table.data_ptr(), ids_at, y.data_ptr(), vocab, c, ids.numel(), ld, ld_y, scale, kind,
+                                   _IDS[ids.dtype], y_kind, _stream(stream))
+    if status:
+        check(status, "embed_fprop")
     return y
 
 
@@ -181,12 +188,14 @@ def embed_grad(dy, ids, vocab: int, *, scale: float = 1.0, dtype=None, accumulat
     ids_at = _dense(ids, ids.dtype, "ids")
     if dtype is None:
         dtype = out.dtype if out is not None else torch.float32
-    d = _output(out, (vocab, c), dtype, dy.device, stream)
-    _, _, ld_d = _rows(d, "out")
-    at, size, held = _workspace(workspace, "miq_embed_grad_workspace_size", (vocab, c, ids.numel()), dy.device, stream)
-    check(lib().miq_embed_grad(dy.data_ptr(), ids_at, d.data_ptr(), vocab, c, ids.numel(), ld, ld_d, scale,
-                               1 if accumulate else 0, kind, _IDS[ids.dtype], _kind(d.dtype, "out"), at, size,
-                               _stream(stream)), "embed_grad")
+    d_kind = _kind(dtype, "dtype")
+    tokens = ids.numel()
+    d, ld_d = _output(out, (vocab, c), dtype, dy, stream)
+    at, size, held = _workspace(workspace, "miq_embed_grad_workspace_size", (vocab, c, tokens), dy.device, stream)
+    status = lib().miq_embed_grad(dy.data_ptr(), ids_at, d.data_ptr(), vocab, c, tokens, ld, ld_d, scale,
+                                  1 if accumulate else 0, kind, _IDS[ids.dtype], d_kind, at, size, _stream(stream))
+    if status:
+        check(status, "embed_grad")
     return d
 
 
@@ -203,8 +212,12 @@ def _halves(width: int, gated: bool) -> int:
 def _new_kept(x, c: int, act: str, gated: bool, kept: Optional[Act8], stream) -> Act8:
     groups = (c + GROUP - 1) // GROUP * (2 if gated else 1)
     if kept is None:
-        return Act8(_alloc(x.shape, torch.int8, x.device, stream),
-                    _alloc(x.shape[:-1] + (groups,), torch.uint8, x.device, stream), act, gated)
+        shape = x.shape
+        if stream is None:
+            return Act8(x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1] + (groups,), dtype=torch.uint8), act,
+                        gated)
+        return Act8(_alloc(shape, torch.int8, x.device, stream),
+                    _alloc(shape[:-1] + (groups,), torch.uint8, x.device, stream), act, gated)
     _dense(kept.codes, torch.int8, "codes")
     _dense(kept.scales, torch.uint8, "scales")
     if kept.codes.shape != x.shape or kept.scales.shape != x.shape[:-1] + (groups,):
@@ -214,17 +227,19 @@ def _new_kept(x, c: int, act: str, gated: bool, kept: Optional[Act8], stream) ->
 
 def _kept(kept: Act8):
     """(rows, channels) of a kept tensor."""
-    codes, scales = kept.codes, kept.scales
+    codes, scales, _, gated = kept
     _dense(codes, torch.int8, "codes")
     _dense(scales, torch.uint8, "scales")
-    if codes.dim() == 0:
+    shape = codes.shape
+    if not shape:
         raise ValueError("codes must have a channel dimension")
-    width = codes.shape[-1]
-    c = _halves(width, kept.gated)
-    groups = (c + GROUP - 1) // GROUP * (2 if kept.gated else 1)
-    if scales.shape != codes.shape[:-1] + (groups,):
-        raise ValueError(f"scales must be {tuple(codes.shape[:-1]) + (groups,)}, got {tuple(scales.shape)}")
-    return (codes.numel() // width if width else 0), c
+    width = shape[-1]
+    c = _halves(width, gated)
+    groups = (c + GROUP - 1) // GROUP * (2 if gated else 1)
+    lead = shape[:-1]
+    if scales.shape != lead + (groups,):
+        raise ValueError(f"scales must be {tuple(lead) + (groups,)}, got {tuple(scales.shape)}")
+    return lead.numel(), c
 
 
 def act8_fprop(x, act: str = "silu", *, gated: bool = False, out=None, kept: Optional[Act8] = None, stream=None):
@@ -235,11 +250,12 @@ def act8_fprop(x, act: str = "silu", *, gated: bool = False, out=None, kept: Opt
     kind, which = _kind(x.dtype, "x"), _act(act)
     rows, width, ld = _rows(x, "x")
     c = _halves(width, gated)
-    y = _output(out, x.shape[:-1] + (c,), x.dtype, x.device, stream)
-    _, _, ld_y = _rows(y, "out")
+    y, ld_y = _output(out, x.shape[:-1] + (c,), x.dtype, x, stream)
     held = _new_kept(x, c, act, gated, kept, stream)
-    check(lib().miq_act8_fprop(x.data_ptr(), y.data_ptr(), held.codes.data_ptr(), held.scales.data_ptr(), rows, c, ld,
-                               ld_y, which, 1 if gated else 0, kind, _stream(stream)), "act8_fprop")
+    status = lib().miq_act8_fprop(x.data_ptr(), y.data_ptr(), held[0].data_ptr(), held[1].data_ptr(), rows, c, ld, ld_y,
+                                  which, 1 if gated else 0, kind, _stream(stream))
+    if status:
+        check(status, "act8_fprop")
     return y, held
 
 
@@ -249,8 +265,10 @@ def act8_keep(x, *, kept: Optional[Act8] = None, stream=None) -> Act8:
     kind = _kind(x.dtype, "x")
     rows, c, ld = _rows(x, "x")
     held = _new_kept(x, c, "none", False, kept, stream)
-    check(lib().miq_act8_fprop(x.data_ptr(), None, held.codes.data_ptr(), held.scales.data_ptr(), rows, c, ld, c, 0, 0,
-                               kind, _stream(stream)), "act8_keep")
+    status = lib().miq_act8_fprop(x.data_ptr(), None, held[0].data_ptr(), held[1].data_ptr(), rows, c, ld, c, 0, 0, kind,
+                                  _stream(stream))
+    if status:
+        check(status, "act8_keep")
     return held
 
 
@@ -262,18 +280,21 @@ def act8_expand(kept: Act8, *, apply: bool = False, dtype=None, out=None, stream
     if dtype is None:
         dtype = out.dtype if out is not None else torch.float32
     kind = _kind(dtype, "dtype")
+    shape = codes.shape
     gated = kept.gated and apply
-    if kept.gated and not apply:  # the halves of a gated row are rows of their own
-        if out is not None and not out.is_contiguous():
-            raise ValueError("out must be contiguous for gated rows")
+    if gated:
+        shape = shape[:-1] + (c,)
+    elif kept.gated:  # the halves of a gated row are rows of their own
         rows *= 2
-    y = _output(out, codes.shape[:-1] + (c,) if gated or not kept.gated else codes.shape, dtype, codes.device, stream)
-    _, _, ld_y = _rows(y, "out")
+    y, ld_y = _output(out, shape, dtype, codes, stream)
     if kept.gated and not apply:
+        if not y.is_contiguous():
+            raise ValueError("out must be contiguous for the values of gated rows")
         ld_y = c
-    check(lib().miq_act8_expand(codes.data_ptr(), kept.scales.data_ptr(), y.data_ptr(), rows, c, ld_y,
-                                _act(kept.act) if apply else 0, 1 if gated else 0, kind, _stream(stream)),
-          "act8_expand")
+    status = lib().miq_act8_expand(codes.data_ptr(), kept.scales.data_ptr(), y.data_ptr(), rows, c, ld_y,
+                                   _act(kept.act) if apply else 0, 1 if gated else 0, kind, _stream(stream))
+    if status:
+        check(status, "act8_expand")
     return y
 
 
@@ -282,13 +303,15 @@ def act8_bprop(dy, kept: Act8, *, out=None, stream=None):
     [dy * up' * act'(gate'), dy * act(gate')]; dy (..., C), float32 or bfloat16."""
     kind = _kind(dy.dtype, "dy")
     rows, c = _kept(kept)
-    if dy.shape != kept.codes.shape[:-1] + (c,):
-        raise ValueError(f"dy must be {tuple(kept.codes.shape[:-1]) + (c,)}, got {tuple(dy.shape)}")
+    codes, scales, act, gated = kept
+    if dy.shape != codes.shape[:-1] + (c,):
+        raise ValueError(f"dy must be {tuple(codes.shape[:-1]) + (c,)}, got {tuple(dy.shape)}")
     _, _, ld = _rows(dy, "dy")
-    dx = _output(out, kept.codes.shape, dy.dtype, dy.device, stream)
-    _, _, ld_dx = _rows(dx, "out")
-    check(lib().miq_act8_bprop(dy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), dx.data_ptr(), rows, c, ld,
-                               ld_dx, _act(kept.act), 1 if kept.gated else 0, kind, _stream(stream)), "act8_bprop")
+    dx, ld_dx = _output(out, codes.shape, dy.dtype, dy, stream)
+    status = lib().miq_act8_bprop(dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), rows, c, ld, ld_dx,
+                                  _act(act), 1 if gated else 0, kind, _stream(stream))
+    if status:
+        check(status, "act8_bprop")
     return dx
 
 
@@ -325,15 +348,15 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
         raise ValueError(f"dy and the kept rows differ: {tuple(dy.shape[:-1])} and {tuple(kept.codes.shape[:-1])}")
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
-    rows = dy.shape[:-1].numel()
     if dtype is None:
         dtype = out.dtype if out is not None else torch.float32
-    dw = _output(out, (k, c), dtype, dy.device, stream)
-    _, _, ld_dw = _rows(dw, "out")
+    dw_kind = _kind(dtype, "dtype")
+    dw, ld_dw = _output(out, (k, c), dtype, dy, stream)
     at, size, held = _workspace(workspace, "miq_act8_grad_workspace_size", (rows, c, k, kind), dy.device, stream)
-    check(lib().miq_act8_grad(dy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), dw.data_ptr(), rows, c, k,
-                              ld, ld_dw, 1 if accumulate else 0, kind, _kind(dw.dtype, "out"), at, size,
-                              _stream(stream)), "act8_grad")
+    status = lib().miq_act8_grad(dy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), dw.data_ptr(), rows, c, k,
+                                 ld, ld_dw, 1 if accumulate else 0, kind, dw_kind, at, size, _stream(stream))
+    if status:
+        check(status, "act8_grad")
     return dw
 
 
