@@ -1,8 +1,8 @@
 // Activations whose input is kept in 8 bits (miq_act8_fprop, _bprop, _expand).
 //
-// Every kernel is one pass over its tensors.  A lane holds eight consecutive channels, so four
-// neighbouring lanes share one exponent byte; a row's chunks are padded to whole groups, which
-// keeps those four lanes in one row whatever the row's length.
+// Every kernel is one pass over its tensors.  A lane holds 16 bytes of consecutive channels (8 of
+// bf16, 4 of fp32), so 4 or 8 neighbouring lanes share one exponent byte; a row's chunks are padded
+// to whole groups, which keeps those lanes in one row whatever the row's length.
 #include "train_device.h"
 
 namespace miq {
@@ -35,21 +35,63 @@ __device__ __forceinline__ float slope_of(float v) {
 }
 
 struct Rows {
-  int64_t total;     // chunks of eight channels, rows padded to whole groups
+  int64_t total;     // chunks of a lane's channels, rows padded to whole groups
   int64_t ld_x, ld_dy, ld_y;
-  int c, per_row;    // per_row = 4 * groups
-  FastDivM div;      // by per_row
+  int c, groups, per_row;  // chunks per row: groups * (32 / a lane's channels)
+  FastDivM div;            // by per_row
 };
 
-// (row, channel, channels left) of this thread's chunk; false past the end
-__device__ __forceinline__ bool place(const Rows& r, int64_t block, int64_t* row, int* chunk, int* left) {
+// A lane's channels: 16 bytes of the tensor's type.
+template <typename T>
+constexpr int kWide = 16 / static_cast<int>(sizeof(T));
+
+template <int W>
+struct Vec;
+template <>
+struct Vec<8> {
+  typedef v8f type;
+};
+template <>
+struct Vec<4> {
+  typedef v4f type;
+};
+
+__device__ __forceinline__ v8f load_all(const __bf16* p) { return load8(p); }
+__device__ __forceinline__ v4f load_all(const float* p) { return load4(p); }
+__device__ __forceinline__ void store_all(__bf16* p, const v8f& v) { store8(p, v); }
+__device__ __forceinline__ void store_all(float* p, const v4f& v) { store4(p, v); }
+
+// The first `left` of a lane's channels; the rest read zero and are not stored.
+template <typename T>
+__device__ __forceinline__ typename Vec<kWide<T>>::type load_some(const T* p, int left) {
+  if (left >= kWide<T>) return load_all(p);
+  typename Vec<kWide<T>>::type v = {};
+#pragma unroll
+  for (int i = 0; i < kWide<T>; ++i)
+    if (i < left) v[i] = static_cast<float>(p[i]);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, const typename Vec<kWide<T>>::type& v, int left) {
+  if (left >= kWide<T>) {
+    store_all(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kWide<T>; ++i)
+    if (i < left) p[i] = static_cast<T>(v[i]);
+}
+
+// (row, channel, channels left) of this thread's chunk of W; false past the end
+template <int W>
+__device__ __forceinline__ bool place(const Rows& r, int64_t block, int64_t* row, int* col, int* left) {
   const int64_t base = block * kThreads;
   const int64_t row0 = base / r.per_row;  // the workgroup's, one division
   const int at = static_cast<int>(base - row0 * r.per_row) + threadIdx.x;
   const int over = fdiv(at, r.div);
   *row = row0 + over;
-  *chunk = at - over * r.per_row;
-  *left = r.c - *chunk * 8;
+  *col = (at - over * r.per_row) * W;
+  *left = r.c - *col;
   return base + threadIdx.x < r.total;
 }
 
@@ -59,69 +101,87 @@ __device__ __forceinline__ int exponent_byte(unsigned top) {
   return top >= 0x7f800000u ? 255 : min(max(e, 1), 248);
 }
 
-// Keeps eight values: codes at `codes`, the group's byte at `scale` (by its first lane).
-__device__ __forceinline__ void keep8(const v8f& v, int left, int8_t* codes, uint8_t* scale) {
+// Keeps a lane's W values: codes at `codes`, the group's byte at `scale` (by its first lane).
+template <int W>
+__device__ __forceinline__ void keep(const typename Vec<W>::type& v, int left, int8_t* codes, uint8_t* scale) {
   unsigned top = 0;  // magnitudes order as their bits do, NaN above infinity
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 1)));
-  top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 2)));
+  for (int i = 0; i < W; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int step = 1; step < kAct8Group / W; step *= 2)
+    top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), step)));
   const int byte = exponent_byte(top);
   // 2^(127 - byte), a normal number for every byte below 254; the products are exact or below half
   // a code, and adding 1.5 * 2^23 rounds them to nearest even into the low byte
   const float inverse = __uint_as_float(static_cast<unsigned>(254 - min(byte, 253)) << 23);
-  float r[8];
+  float r[W];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = __builtin_amdgcn_fmed3f(v[i] * inverse, -127.0f, 127.0f) + 12582912.0f;
-  v2i q{static_cast<int>(pack4_magic(r[0], r[1], r[2], r[3])), static_cast<int>(pack4_magic(r[4], r[5], r[6], r[7]))};
-  if (byte == 255) q = v2i{};  // not a finite group
-  if (left >= 8) {
-    *reinterpret_cast<v2i_any*>(codes) = q;
+  for (int i = 0; i < W; ++i) r[i] = __builtin_amdgcn_fmed3f(v[i] * inverse, -127.0f, 127.0f) + 12582912.0f;
+  int q[W / 4];
+#pragma unroll
+  for (int i = 0; i < W; i += 4)
+    q[i / 4] = byte == 255 ? 0 : static_cast<int>(pack4_magic(r[i], r[i + 1], r[i + 2], r[i + 3]));  // 255: not finite
+  if (left >= W) {
+    if constexpr (W == 8) *reinterpret_cast<v2i_any*>(codes) = v2i{q[0], q[1]};
+    else *reinterpret_cast<int_any*>(codes) = q[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < W; ++i)
       if (i < left) codes[i] = static_cast<int8_t>(q[i / 4] >> (8 * (i & 3)));
   }
-  if ((threadIdx.x & 3) == 0) *scale = static_cast<uint8_t>(byte);
+  if ((threadIdx.x & (kAct8Group / W - 1)) == 0) *scale = static_cast<uint8_t>(byte);
 }
 
-__device__ __forceinline__ v8f kept8(const int8_t* codes, const uint8_t* scale, int left) {
-  v2i q = {};
-  if (left >= 8) {
-    q = *reinterpret_cast<const v2i_any*>(codes);
+template <int W>
+__device__ __forceinline__ typename Vec<W>::type kept(const int8_t* codes, const uint8_t* scale, int left) {
+  int q[W / 4] = {};
+  if (left >= W) {
+    if constexpr (W == 8) {
+      const v2i w = *reinterpret_cast<const v2i_any*>(codes);
+      q[0] = w[0];
+      q[1] = w[1];
+    } else {
+      q[0] = *reinterpret_cast<const int_any*>(codes);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < W; ++i)
       if (i < left) q[i / 4] |= (codes[i] & 0xff) << (8 * (i & 3));
   }
   // byte 255 is the bits of infinity, which a zero code makes NaN
   const float s = __uint_as_float(static_cast<unsigned>(*scale) << 23);
-  const v4f lo = codes4(q[0]) * s, hi = codes4(q[1]) * s;
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  typename Vec<W>::type v;
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    const v4f four = codes4(q[i / 4]) * s;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[i + j] = four[j];
+  }
+  return v;
 }
 
 template <typename T, int ACT, bool GATED>
 __global__ __launch_bounds__(kThreads) void act8_fprop_kernel(Rows r, const T* __restrict__ x, T* __restrict__ y,
                                                               int8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  constexpr int H = GATED ? 2 : 1;
+  constexpr int H = GATED ? 2 : 1, W = kWide<T>;
+  typedef typename Vec<W>::type V;
   for (int64_t b = blockIdx.x; b * kThreads < r.total; b += gridDim.x) {
     int64_t row;
-    int chunk, left;
-    if (!place(r, b, &row, &chunk, &left)) continue;  // whole groups of lanes leave together
-    const int groups = r.per_row >> 2;
-    v8f v[H];
+    int at, left;
+    if (!place<W>(r, b, &row, &at, &left)) continue;  // whole groups of lanes leave together
+    V v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      const int col = h * r.c + chunk * 8;
-      v[h] = load8_of(x + row * r.ld_x + col, left);
-      keep8(v[h], left, codes + row * (H * static_cast<int64_t>(r.c)) + col,
-            scales + (row * H + h) * groups + (chunk >> 2));
+      const int col = h * r.c + at;
+      v[h] = load_some(x + row * r.ld_x + col, left);
+      keep<W>(v[h], left, codes + row * (H * static_cast<int64_t>(r.c)) + col,
+              scales + (row * H + h) * r.groups + at / kAct8Group);
     }
     if (y != nullptr) {
-      v8f out;
+      V out;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
-      store8_of(y + row * r.ld_y + chunk * 8, out, left);
+      for (int i = 0; i < W; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
+      store_some(y + row * r.ld_y + at, out, left);
     }
   }
 }
@@ -130,26 +190,26 @@ template <typename T, int ACT, bool GATED>
 __global__ __launch_bounds__(kThreads) void act8_bprop_kernel(Rows r, const T* __restrict__ dy,
                                                               const int8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, T* __restrict__ dx) {
-  constexpr int H = GATED ? 2 : 1;
+  constexpr int H = GATED ? 2 : 1, W = kWide<T>;
+  typedef typename Vec<W>::type V;
   for (int64_t b = blockIdx.x; b * kThreads < r.total; b += gridDim.x) {
     int64_t row;
-    int chunk, left;
-    if (!place(r, b, &row, &chunk, &left) || left <= 0) continue;
-    const int groups = r.per_row >> 2;
-    const v8f d = load8_of(dy + row * r.ld_dy + chunk * 8, left);
-    v8f v[H];
+    int at, left;
+    if (!place<W>(r, b, &row, &at, &left) || left <= 0) continue;
+    const V d = load_some(dy + row * r.ld_dy + at, left);
+    V v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h)
-      v[h] = kept8(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + chunk * 8,
-                   scales + (row * H + h) * groups + (chunk >> 2), left);
-    v8f g;
+      v[h] = kept<W>(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + at,
+                     scales + (row * H + h) * r.groups + at / kAct8Group, left);
+    V g;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = d[i] * (GATED ? v[H - 1][i] : 1.0f) * slope_of<ACT>(v[0][i]);
-    store8_of(dx + row * r.ld_y + chunk * 8, g, left);
+    for (int i = 0; i < W; ++i) g[i] = d[i] * (GATED ? v[H - 1][i] : 1.0f) * slope_of<ACT>(v[0][i]);
+    store_some(dx + row * r.ld_y + at, g, left);
     if constexpr (GATED) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = d[i] * act_of<ACT>(v[0][i]);
-      store8_of(dx + row * r.ld_y + r.c + chunk * 8, g, left);
+      for (int i = 0; i < W; ++i) g[i] = d[i] * act_of<ACT>(v[0][i]);
+      store_some(dx + row * r.ld_y + r.c + at, g, left);
     }
   }
 }
@@ -157,28 +217,29 @@ __global__ __launch_bounds__(kThreads) void act8_bprop_kernel(Rows r, const T* _
 template <typename T, int ACT, bool GATED>
 __global__ __launch_bounds__(kThreads) void act8_expand_kernel(Rows r, const int8_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales, T* __restrict__ y) {
-  constexpr int H = GATED ? 2 : 1;
+  constexpr int H = GATED ? 2 : 1, W = kWide<T>;
+  typedef typename Vec<W>::type V;
   for (int64_t b = blockIdx.x; b * kThreads < r.total; b += gridDim.x) {
     int64_t row;
-    int chunk, left;
-    if (!place(r, b, &row, &chunk, &left) || left <= 0) continue;
-    const int groups = r.per_row >> 2;
-    v8f v[H];
+    int at, left;
+    if (!place<W>(r, b, &row, &at, &left) || left <= 0) continue;
+    V v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h)
-      v[h] = kept8(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + chunk * 8,
-                   scales + (row * H + h) * groups + (chunk >> 2), left);
-    v8f out;
+      v[h] = kept<W>(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + at,
+                     scales + (row * H + h) * r.groups + at / kAct8Group, left);
+    V out;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
-    store8_of(y + row * r.ld_y + chunk * 8, out, left);
+    for (int i = 0; i < W; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
+    store_some(y + row * r.ld_y + at, out, left);
   }
 }
 
 Rows rows_of(const Act8Args& a) {
   Rows r{};
   const int64_t groups = (static_cast<int64_t>(a.c) + kAct8Group - 1) / kAct8Group;
-  r.per_row = static_cast<int>(4 * groups);
+  r.groups = static_cast<int>(groups);
+  r.per_row = static_cast<int>(groups * (a.bf16 ? 4 : 8));
   r.total = a.rows * r.per_row;
   r.ld_x = a.ld_x;
   r.ld_dy = a.ld_dy;

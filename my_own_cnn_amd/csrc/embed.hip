@@ -1,4 +1,10 @@
 // y[t, :] = scale * table[ids[t], :] (miq_embed_fprop).
+//
+// Bound by memory: the rows read and the rows written, each once.  A lane writes runs of 16 bytes,
+// neighbouring lanes neighbouring runs, so that every store of a wave covers whole lines: eight
+// channels of bf16, or four of fp32 twice (fp32 rows to bf16, 65536 rows of 2048: 95 us, and 111
+// with stores of 8 bytes).  Where a row ends within a run, the lane takes the row's last run
+// instead: it writes what its neighbour writes in part, the same values.
 #include "train_device.h"
 
 namespace miq {
@@ -6,22 +12,44 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// One row per 2^row_log threads, eight channels per thread and step.
+template <int W, typename TI, typename TO>
+__device__ __forceinline__ void move(const TI* from, TO* to, float scale, bool there) {
+  if constexpr (W == 8) {
+    v8f v = {};
+    if (there) v = load8(from) * scale;
+    store8(to, v);
+  } else {
+    v4f v = {};
+    if (there) v = load4(from) * scale;
+    store4(to, v);
+  }
+}
+
+// One row per 2^row_log threads.
 template <typename TI, typename TO>
 __global__ __launch_bounds__(kThreads) void embed_fprop_kernel(const TI* __restrict__ table, const void* __restrict__ ids,
                                                                TO* __restrict__ y, int vocab, int c, int64_t tokens,
                                                                int64_t ld_table, int64_t ld_y, float scale, bool ids64,
                                                                int row_log) {
+  constexpr int W = 16 / static_cast<int>(sizeof(TO)), kRuns = 8 / W;
   const int rows = kThreads >> row_log;
   const int lane = threadIdx.x & ((1 << row_log) - 1);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * rows + (threadIdx.x >> row_log); t < tokens;
        t += static_cast<int64_t>(gridDim.x) * rows) {
     const int64_t id = load_id(ids, ids64, t);
     const bool there = id >= 0 && id < vocab;
-    for (int col = lane * 8; col < c; col += 8 << row_log) {
-      v8f v = {};
-      if (there) v = load8_of(table + id * ld_table + col, c - col) * scale;
-      store8_of(y + t * ld_y + col, v, c - col);
+    const TI* from = table + (there ? id : 0) * ld_table;
+    TO* to = y + t * ld_y;
+    if (c < W) {
+      if (lane < c) to[lane] = there ? static_cast<TO>(static_cast<float>(from[lane]) * scale) : static_cast<TO>(0.0f);
+      continue;
+    }
+    for (int base = lane * W; base < c; base += (kRuns * W) << row_log) {
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        const int col = base + ((r * W) << row_log);
+        if (col < c) move<W>(from + min(col, c - W), to + min(col, c - W), scale, there);
+      }
     }
   }
 }

@@ -279,19 +279,27 @@ struct Sum {
   __device__ float* slot(int chunk, int which, int tile, int lane) const {
     return part + ((static_cast<int64_t>(chunk) * 2 + which) * col_tiles + tile) * (lanes * 8) + lane * 4;
   }
-  // A lane's channels: four from `col` and four `apart` from there.  Where the row ends within a
-  // four, the lane takes the row's last four instead, as its neighbour does in part: both write the
-  // same values.  Adding to the table is no place for that; there such a lane is not `whole` and
-  // goes value by value.  False for a lane beyond the row.
+  // A lane's channels, so that neighbouring lanes store neighbouring runs of 16 bytes: of an fp32
+  // table four from `col` and four `apart` from there, of a bf16 table eight from `col` (apart = 4).
+  // Where the row ends within a run, the lane takes the row's last run instead, as its neighbour
+  // does in part: both write the same values.  Adding to the table is no place for that; there such
+  // a lane is not `whole` and goes value by value.  False for a lane beyond the row.
+  static constexpr bool kPairs = sizeof(TO) == 4;
   __device__ bool place(int tile, int lane, int* col, int* apart, bool* whole) const {
-    const int first = tile * kCols + lane * 4;
-    const int second = first + lanes * 4;
-    *whole = second + 4 <= c || (c >= 4 && !accumulate);
+    const int first = tile * kCols + lane * (kPairs ? 4 : 8);
     *col = first;
-    *apart = lanes * 4;
-    if (second + 4 > c && *whole) {
-      *col = min(first, c - 4);
-      *apart = second < c ? c - 4 - *col : 0;
+    if constexpr (kPairs) {
+      const int second = first + lanes * 4;
+      *whole = second + 4 <= c || (c >= 4 && !accumulate);
+      *apart = lanes * 4;
+      if (second + 4 > c && *whole) {
+        *col = min(first, c - 4);
+        *apart = second < c ? c - 4 - *col : 0;
+      }
+    } else {
+      *whole = first + 8 <= c || (c >= 8 && !accumulate);
+      *apart = 4;
+      if (*whole) *col = min(first, c - 8);
     }
     return first < c;
   }
@@ -299,8 +307,13 @@ struct Sum {
     TO* to = table + row * ld_table + col;
     acc *= scale;
     if (whole) {
-      if (accumulate) acc += load44(to, apart);
-      store44(to, apart, acc);
+      if constexpr (kPairs) {
+        if (accumulate) acc += load44(to, apart);
+        store44(to, apart, acc);
+      } else {
+        if (accumulate) acc += load8(to);
+        store8(to, acc);
+      }
     } else {
       if (accumulate) acc += load44_of(to, apart, c - col);
       store44_of(to, apart, acc, c - col);
@@ -326,11 +339,15 @@ __device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
   for (int r = 0; r < rows; ++r) {
     if (!empty[r]) continue;
     TO* const row = s.table + (first + r) * s.ld_table;
-    if (s.c < 4) {
+    constexpr int W = 16 / static_cast<int>(sizeof(TO));
+    if (s.c < W) {
       if (static_cast<int>(threadIdx.x) < s.c) row[threadIdx.x] = static_cast<TO>(0.0f);
     } else {
 #pragma unroll 2
-      for (int col = threadIdx.x * 4; col < s.c; col += kThreads * 4) store4(row + min(col, s.c - 4), v4f{});
+      for (int col = threadIdx.x * W; col < s.c; col += kThreads * W) {
+        if constexpr (W == 4) store4(row + min(col, s.c - 4), v4f{});
+        else store8(row + min(col, s.c - 8), v8f{});
+      }
     }
   }
 }
@@ -346,13 +363,21 @@ template <>
 struct Raw8<__bf16> {
   v4bf lo, hi;
 };
+template <bool PAIRS>
 __device__ __forceinline__ void load_raw(Raw8<float>& r, const float* p, int apart) {
   r.lo = *reinterpret_cast<const v4f_any*>(p);
-  r.hi = *reinterpret_cast<const v4f_any*>(p + apart);
+  r.hi = *reinterpret_cast<const v4f_any*>(p + (PAIRS ? apart : 4));
 }
+template <bool PAIRS>
 __device__ __forceinline__ void load_raw(Raw8<__bf16>& r, const __bf16* p, int apart) {
-  r.lo = *reinterpret_cast<const v4bf_any*>(p);
-  r.hi = *reinterpret_cast<const v4bf_any*>(p + apart);
+  if constexpr (PAIRS) {
+    r.lo = *reinterpret_cast<const v4bf_any*>(p);
+    r.hi = *reinterpret_cast<const v4bf_any*>(p + apart);
+  } else {
+    const v8bf v = *reinterpret_cast<const v8bf_any*>(p);
+    r.lo = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+    r.hi = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+  }
 }
 template <typename T>
 __device__ __forceinline__ v8f value(const Raw8<T>& r) {
@@ -399,7 +424,7 @@ __device__ __forceinline__ void sum_chunk(const Sum<TI, TO>& s, int chunk, int t
       const int64_t t = i + j < end ? pos[j / 4][j & 3] : s.order[begin];
       const TI* from = s.dy + t * s.ld_dy + col;
       if constexpr (WHOLE) {
-        load_raw(row[j], from, apart);
+        load_raw<Sum<TI, TO>::kPairs>(row[j], from, apart);
       } else {
         part[j] = load44_of(from, apart, left);
       }

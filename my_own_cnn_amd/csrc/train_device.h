@@ -16,6 +16,7 @@ typedef int v2i __attribute__((ext_vector_type(2)));
 typedef v8bf v8bf_any __attribute__((aligned(2)));
 typedef v4f v4f_any __attribute__((aligned(4)));
 typedef v2i v2i_any __attribute__((aligned(1)));
+typedef int int_any __attribute__((aligned(1)));
 
 __device__ __forceinline__ v8f load8(const float* p) {
   const v4f a = *reinterpret_cast<const v4f_any*>(p), b = *reinterpret_cast<const v4f_any*>(p + 4);
@@ -78,8 +79,7 @@ template <typename T>
 __device__ __forceinline__ v8f load44(const T* p, int apart) {
   return __builtin_shufflevector(load4(p), load4(p + apart), 0, 1, 2, 3, 4, 5, 6, 7);
 }
-template <typename T>
-__device__ __forceinline__ void store44(T* p, int apart, const v8f& v) {
+__device__ __forceinline__ void store44(float* p, int apart, const v8f& v) {
   store4(p, __builtin_shufflevector(v, v, 0, 1, 2, 3));
   store4(p + apart, __builtin_shufflevector(v, v, 4, 5, 6, 7));
 }
