@@ -58,8 +58,6 @@ struct Vec<4> {
 
 __device__ __forceinline__ v8f load_all(const __bf16* p) { return load8(p); }
 __device__ __forceinline__ v4f load_all(const float* p) { return load4(p); }
-__device__ __forceinline__ void store_all(__bf16* p, const v8f& v) { store8(p, v); }
-__device__ __forceinline__ void store_all(float* p, const v4f& v) { store4(p, v); }
 
 // The first `left` of a lane's channels; the rest read zero and are not stored.
 template <typename T>
@@ -71,10 +69,10 @@ __device__ __forceinline__ typename Vec<kWide<T>>::type load_some(const T* p, in
     if (i < left) v[i] = static_cast<float>(p[i]);
   return v;
 }
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void store_some(T* p, const typename Vec<kWide<T>>::type& v, int left) {
   if (left >= kWide<T>) {
-    store_all(p, v);
+    store_run<STREAM>(p, v);
     return;
   }
 #pragma unroll
@@ -160,7 +158,7 @@ __device__ __forceinline__ typename Vec<W>::type kept(const int8_t* codes, const
   return v;
 }
 
-template <typename T, int ACT, bool GATED>
+template <typename T, int ACT, bool GATED, bool STREAM>
 __global__ __launch_bounds__(kThreads) void act8_fprop_kernel(Rows r, const T* __restrict__ x, T* __restrict__ y,
                                                               int8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int H = GATED ? 2 : 1, W = kWide<T>;
@@ -181,12 +179,12 @@ __global__ __launch_bounds__(kThreads) void act8_fprop_kernel(Rows r, const T* _
       V out;
 #pragma unroll
       for (int i = 0; i < W; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
-      store_some(y + row * r.ld_y + at, out, left);
+      store_some<STREAM>(y + row * r.ld_y + at, out, left);
     }
   }
 }
 
-template <typename T, int ACT, bool GATED>
+template <typename T, int ACT, bool GATED, bool STREAM>
 __global__ __launch_bounds__(kThreads) void act8_bprop_kernel(Rows r, const T* __restrict__ dy,
                                                               const int8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, T* __restrict__ dx) {
@@ -205,16 +203,16 @@ __global__ __launch_bounds__(kThreads) void act8_bprop_kernel(Rows r, const T* _
     V g;
 #pragma unroll
     for (int i = 0; i < W; ++i) g[i] = d[i] * (GATED ? v[H - 1][i] : 1.0f) * slope_of<ACT>(v[0][i]);
-    store_some(dx + row * r.ld_y + at, g, left);
+    store_some<STREAM>(dx + row * r.ld_y + at, g, left);
     if constexpr (GATED) {
 #pragma unroll
       for (int i = 0; i < W; ++i) g[i] = d[i] * act_of<ACT>(v[0][i]);
-      store_some(dx + row * r.ld_y + r.c + at, g, left);
+      store_some<STREAM>(dx + row * r.ld_y + r.c + at, g, left);
     }
   }
 }
 
-template <typename T, int ACT, bool GATED>
+template <typename T, int ACT, bool GATED, bool STREAM>
 __global__ __launch_bounds__(kThreads) void act8_expand_kernel(Rows r, const int8_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales, T* __restrict__ y) {
   constexpr int H = GATED ? 2 : 1, W = kWide<T>;
@@ -231,7 +229,7 @@ __global__ __launch_bounds__(kThreads) void act8_expand_kernel(Rows r, const int
     V out;
 #pragma unroll
     for (int i = 0; i < W; ++i) out[i] = act_of<ACT>(v[0][i]) * (GATED ? v[H - 1][i] : 1.0f);
-    store_some(y + row * r.ld_y + at, out, left);
+    store_some<STREAM>(y + row * r.ld_y + at, out, left);
   }
 }
 
@@ -249,11 +247,16 @@ Rows rows_of(const Act8Args& a) {
   return r;
 }
 
-// Calls go(type, act, gated) with the three as compile-time values.
+// Calls go(type, act, gated, stream) with the four as compile-time values; `wide`: the length of an
+// output row in units of c.
 template <typename F>
-void dispatch(const Act8Args& a, F&& go) {
+void dispatch(const Act8Args& a, int wide, F&& go) {
+  const bool stream = stream_stores(a.y, a.rows, static_cast<int64_t>(a.c) * wide, a.ld_y, a.bf16 ? 2 : 4);
+  auto by_stream = [&](auto type, auto act, auto gated) {
+    stream ? go(type, act, gated, std::true_type{}) : go(type, act, gated, std::false_type{});
+  };
   auto by_gate = [&](auto type, auto act) {
-    a.gated ? go(type, act, std::true_type{}) : go(type, act, std::false_type{});
+    a.gated ? by_stream(type, act, std::true_type{}) : by_stream(type, act, std::false_type{});
   };
   auto by_act = [&](auto type) {
     switch (a.act) {
@@ -275,9 +278,9 @@ unsigned blocks_of(const Rows& r) {
 
 hipError_t launch_act8_fprop(const Act8Args& a, hipStream_t stream) {
   const Rows r = rows_of(a);
-  dispatch(a, [&](auto type, auto act, auto gated) {
+  dispatch(a, 1, [&](auto type, auto act, auto gated, auto past) {
     using T = decltype(type);
-    act8_fprop_kernel<T, act.value, gated.value><<<blocks_of(r), kThreads, 0, stream>>>(
+    act8_fprop_kernel<T, act.value, gated.value, past.value><<<blocks_of(r), kThreads, 0, stream>>>(
         r, static_cast<const T*>(a.x), static_cast<T*>(a.y), a.codes, a.scales);
   });
   return hipGetLastError();
@@ -285,9 +288,9 @@ hipError_t launch_act8_fprop(const Act8Args& a, hipStream_t stream) {
 
 hipError_t launch_act8_bprop(const Act8Args& a, hipStream_t stream) {
   const Rows r = rows_of(a);
-  dispatch(a, [&](auto type, auto act, auto gated) {
+  dispatch(a, a.gated ? 2 : 1, [&](auto type, auto act, auto gated, auto past) {
     using T = decltype(type);
-    act8_bprop_kernel<T, act.value, gated.value><<<blocks_of(r), kThreads, 0, stream>>>(
+    act8_bprop_kernel<T, act.value, gated.value, past.value><<<blocks_of(r), kThreads, 0, stream>>>(
         r, static_cast<const T*>(a.dy), a.codes, a.scales, static_cast<T*>(a.y));
   });
   return hipGetLastError();
@@ -295,9 +298,9 @@ hipError_t launch_act8_bprop(const Act8Args& a, hipStream_t stream) {
 
 hipError_t launch_act8_expand(const Act8Args& a, hipStream_t stream) {
   const Rows r = rows_of(a);
-  dispatch(a, [&](auto type, auto act, auto gated) {
+  dispatch(a, 1, [&](auto type, auto act, auto gated, auto past) {
     using T = decltype(type);
-    act8_expand_kernel<T, act.value, gated.value><<<blocks_of(r), kThreads, 0, stream>>>(
+    act8_expand_kernel<T, act.value, gated.value, past.value><<<blocks_of(r), kThreads, 0, stream>>>(
         r, a.codes, a.scales, static_cast<T*>(a.y));
   });
   return hipGetLastError();

@@ -12,21 +12,21 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <int W, typename TI, typename TO>
-__device__ __forceinline__ void move(const TI* from, TO* to, float scale, bool there) {
-  if constexpr (W == 8) {
-    v8f v = {};
-    if (there) v = load8(from) * scale;
-    store8(to, v);
-  } else {
-    v4f v = {};
-    if (there) v = load4(from) * scale;
-    store4(to, v);
-  }
+template <bool STREAM, typename TI>
+__device__ __forceinline__ void move(const TI* from, __bf16* to, float scale, bool there) {
+  v8f v = {};
+  if (there) v = load8(from) * scale;
+  store_run<STREAM>(to, v);
+}
+template <bool STREAM, typename TI>
+__device__ __forceinline__ void move(const TI* from, float* to, float scale, bool there) {
+  v4f v = {};
+  if (there) v = load4(from) * scale;
+  store_run<STREAM>(to, v);
 }
 
 // One row per 2^row_log threads.
-template <typename TI, typename TO>
+template <bool STREAM, typename TI, typename TO>
 __global__ __launch_bounds__(kThreads) void embed_fprop_kernel(const TI* __restrict__ table, const void* __restrict__ ids,
                                                                TO* __restrict__ y, int vocab, int c, int64_t tokens,
                                                                int64_t ld_table, int64_t ld_y, float scale, bool ids64,
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kThreads) void embed_fprop_kernel(const TI* __restr
 #pragma unroll
       for (int r = 0; r < kRuns; ++r) {
         const int col = base + ((r * W) << row_log);
-        if (col < c) move<W>(from + min(col, c - W), to + min(col, c - W), scale, there);
+        if (col < c) move<STREAM>(from + min(col, c - W), to + min(col, c - W), scale, there);
       }
     }
   }
@@ -56,9 +56,10 @@ __global__ __launch_bounds__(kThreads) void embed_fprop_kernel(const TI* __restr
 
 template <typename TI, typename TO>
 void launch(const EmbedArgs& a, int blocks, int row_log, hipStream_t stream) {
-  embed_fprop_kernel<TI, TO><<<blocks, kThreads, 0, stream>>>(static_cast<const TI*>(a.table), a.ids,
-                                                              static_cast<TO*>(a.y), a.vocab, a.c, a.tokens, a.ld_table,
-                                                              a.ld_y, a.scale, a.ids64, row_log);
+  auto* kernel = stream_stores(a.y, a.tokens, a.c, a.ld_y, sizeof(TO)) ? &embed_fprop_kernel<true, TI, TO>
+                                                                       : &embed_fprop_kernel<false, TI, TO>;
+  kernel<<<blocks, kThreads, 0, stream>>>(static_cast<const TI*>(a.table), a.ids, static_cast<TO*>(a.y), a.vocab, a.c,
+                                          a.tokens, a.ld_table, a.ld_y, a.scale, a.ids64, row_log);
 }
 
 }  // namespace

@@ -251,6 +251,23 @@ def test_beyond_32_bit_offsets(device):
     assert torch.equal(back[-1], M.act8_expand(tail, dtype=BF16)[-1]) and (back[65600, :64] == 3).all()
 
 
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_outputs_beyond_the_caches(device, kind, gated):
+    """Outputs of more than 128 MB take other stores: the same bits as of a few rows at a time."""
+    rows, c = 50000, 1472
+    x = torch.randn((rows, c * (2 if gated else 1)), device=device).to(kind)
+    dy = torch.randn((rows, c), device=device).to(kind)
+    y, kept = M.act8_fprop(x, "silu", gated=gated)
+    dx, back = M.act8_bprop(dy, kept), M.act8_expand(kept, apply=True, dtype=kind)
+    for r in (slice(0, 900), slice(31000, 31333), slice(rows - 700, rows)):
+        part = M.Act8(kept.codes[r], kept.scales[r], "silu", gated)
+        y1, k1 = M.act8_fprop(x[r], "silu", gated=gated)
+        assert torch.equal(y[r], y1) and torch.equal(part.codes, k1.codes) and torch.equal(part.scales, k1.scales)
+        assert torch.equal(dx[r], M.act8_bprop(dy[r], part))
+        assert torch.equal(back[r], M.act8_expand(part, apply=True, dtype=kind))
+
+
 # ---- weight gradient --------------------------------------------------------------------------
 
 GRADS = [  # rows, c, k

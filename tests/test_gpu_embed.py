@@ -185,6 +185,15 @@ def test_table_beyond_32_bit_offsets(device):
     assert torch.equal(M.embed_fprop(d, ids[1:4]), torch.stack([dy[1], dy[2] + dy[4], dy[3]]))
 
 
+@pytest.mark.parametrize("out_type", [F32, BF16])
+def test_outputs_beyond_the_caches(device, out_type):
+    table = torch.randn((500, 2048), device=device)
+    ids = torch.randint(-3, 500, (40000,), device=device)
+    got = M.embed_fprop(table, ids, scale=3.0, dtype=out_type)  # 328 and 164 MB
+    want = torch.where((ids >= 0)[:, None], table[ids.clamp(min=0)] * 3.0, torch.zeros((), device=device))
+    assert torch.equal(got, want.to(out_type))
+
+
 def test_other_stream_and_graph_replays(device):
     rng = np.random.default_rng(6)
     vocab, c, tokens = 500, 40, 9000
