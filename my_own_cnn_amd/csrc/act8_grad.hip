@@ -78,11 +78,11 @@ __device__ __forceinline__ void split8(const Raw<float>& r, v8bf (&p)[3]) {
   p[2] = __builtin_convertvector(c, v8bf);
 }
 
-// The permutation of a row's 32-byte units: 256 bytes of LDS, all 64 banks, hold the same unit of
-// eight consecutive rows of 256 bytes or more, or of every second one of 128 bytes.
+// The permutation of a row's 32-byte units: the 32 lanes that a transposing read serves at once take
+// two neighbouring units of four rows, and these eight lie in different banks, 256 bytes in all.
 template <int W>
 __device__ __forceinline__ int turn(int m) {
-  return W >= 128 ? m & 7 : (m >> 1) & 3;
+  return W >= 128 ? ((m & 3) << 1) | ((m >> 2) & 1) : (m & 2) | ((m >> 2) & 1);
 }
 
 template <typename T, typename TO, int P, int TK, int TC, int VK, int VC, int STAGES, int SETS>
@@ -263,10 +263,13 @@ __global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8
   };
 
   // Three stages: a step multiplies its own, reads the next one's first half and writes the third.
-  // Two, where three do not fit: a step reads and multiplies its own and writes the other.  Either
-  // way the values written were loaded SETS steps before.  Past the last step the loads, writes and
-  // reads repeat that step: their values go unused.
-  constexpr int kAhead = STAGES - 1;  // a step writes the values of step t + kAhead
+  // Two, where three do not fit: a step reads and multiplies its own and writes the other.  Five:
+  // a step writes the one three ahead, so that a barrier after every second step is enough: between
+  // two barriers steps t and t + 1 read the stages t to t + 2, all written before, and write t + 3
+  // and t + 4, in place of t - 2 and t - 1.  Either way the values written were loaded SETS steps
+  // before.  Past the last step the loads, writes and reads repeat that step: their values go unused.
+  constexpr int kAhead = STAGES == 5 ? 3 : STAGES - 1;  // a step writes the values of step t + kAhead
+  static_assert(STAGES != 5 || SETS == 2, "the barrier goes by the place in the loop");
   if (fast > 0) {
     Staged first[kAhead], r[SETS];  // step s >= kAhead in r[s % SETS]
     // the sets' loads in order: the waits for one of them do not include the next
@@ -281,36 +284,31 @@ __global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) write(first[i], i);
     __syncthreads();
-    if constexpr (STAGES == 3) read(0, 0, 0);
+    if constexpr (STAGES >= 3) read(0, 0, 0);
     int now = 0;
-    auto step = [&](Staged& set, int t) {
+    auto step = [&](Staged& set, int t, bool barrier) {
       const int next = now == STAGES - 1 ? 0 : now + 1;
-      if constexpr (STAGES == 3) {
-        read(now, 1, 1);
-        write(set, next == STAGES - 1 ? 0 : next + 1);
-      } else {
-        read(now, 0, 0);
-        read(now, 1, 1);
-        write(set, next);
-      }
+      if constexpr (STAGES == 2) read(now, 0, 0);
+      read(now, 1, 1);
+      write(set, now + kAhead >= STAGES ? now + kAhead - STAGES : now + kAhead);
       multiply(0);
       mix();
       __builtin_amdgcn_sched_barrier(0);
       load(set, min(t + kAhead + SETS, fast - 1));
-      if constexpr (STAGES == 3) read(next, 0, 0);
+      if constexpr (STAGES >= 3) read(next, 0, 0);
       multiply(1);
       mix();
-      __syncthreads();
+      if (barrier) __syncthreads();
       now = next;
     };
     int t = 0;
     for (; t + SETS <= fast; t += SETS) {  // no other way round the loop: its waits count on the loads' order
 #pragma unroll
-      for (int u = 0; u < SETS; ++u) step(r[(u + kAhead) % SETS], t + u);
+      for (int u = 0; u < SETS; ++u) step(r[(u + kAhead) % SETS], t + u, STAGES != 5 || u == 1);
     }
 #pragma unroll
     for (int u = 0; u + 1 < SETS; ++u)
-      if (t + u < fast) step(r[(u + kAhead) % SETS], t + u);
+      if (t + u < fast) step(r[(u + kAhead) % SETS], t + u, STAGES != 5);
   }
   for (int t = fast; t < steps; ++t) {
     Staged r;
@@ -456,7 +454,7 @@ template <typename T, typename TO, int P>
 hipError_t launch_product(const Grad& g, const Shape& s, hipStream_t stream) {
   const unsigned blocks = static_cast<unsigned>(static_cast<int64_t>(g.tiles_k) * g.tiles_c * s.splits);
   if constexpr (P == 1) {
-    if (s.tile == 256) return launch_tile<T, TO, P, 256, 256, 4, 2, 3, 2>(g, blocks, stream);
+    if (s.tile == 256) return launch_tile<T, TO, P, 256, 256, 4, 2, 5, 2>(g, blocks, stream);
   } else {
     if (s.tile == 256) return launch_tile<T, TO, P, 256, 256, 4, 2, 2, 1>(g, blocks, stream);
   }
