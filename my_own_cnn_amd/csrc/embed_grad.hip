@@ -336,15 +336,17 @@ __device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
     empty[threadIdx.x] = none;
   }
   __syncthreads();
-  for (int r = 0; r < rows; ++r) {
+  // a row per wave and turn
+  const int lane = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < rows; r += kThreads / 64) {
     if (!empty[r]) continue;
     TO* const row = s.table + (first + r) * s.ld_table;
     constexpr int W = 16 / static_cast<int>(sizeof(TO));
     if (s.c < W) {
-      if (static_cast<int>(threadIdx.x) < s.c) row[threadIdx.x] = static_cast<TO>(0.0f);
+      if (lane < s.c) row[lane] = static_cast<TO>(0.0f);
     } else {
-#pragma unroll 2
-      for (int col = threadIdx.x * W; col < s.c; col += kThreads * W) {
+#pragma unroll 4
+      for (int col = lane * W; col < s.c; col += 64 * W) {
         if constexpr (W == 4) store4(row + min(col, s.c - 4), v4f{});
         else store8(row + min(col, s.c - 8), v8f{});
       }
