@@ -395,20 +395,20 @@ struct Shape {
 };
 
 // The tile (64, 128 or 256 square) and the splits of the rows: the pair with the least estimated
-// time.  Measured on 28 shapes from 128 x 1024 x 1024 to 16384 x 4096 x 4096 (rows, c, k) in each
-// type with every pair, in microseconds: a step of 32 rows takes `alone` with one workgroup on a
-// CU and `each` apiece with several; about 5 to launch, fill and drain; dw and partial sums are
-// written and read at some 6 TB/s; the launch that joins them costs 5 more.  The pair chosen was
-// the fastest or within 5% of it on 24 of the 28, within 20% on all but one.
+// time.  A step of 32 rows takes `alone` us with one workgroup on a CU and `each` apiece with several;
+// 5 us to launch, fill and drain; dw and partial sums are written and read at 5.9 TB/s; the launch
+// that joins them costs 5 us more.  Fitted to every pair's time on 46 problems from 128 x 1024 x 1024
+// to 65536 x 1024 x 1024 (rows, c, k) in both types: the pair chosen is the fastest or within 5% of
+// it on 42 of them, within 18% on all.
 Shape shape_of(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
   struct Rate {
     int tile;
     double alone, each;
   };
-  static constexpr Rate kBf16[3] = {{64, 0.21, 0.15}, {128, 0.43, 0.37}, {256, 0.92, 0.92}};
-  static constexpr Rate kF32[3] = {{64, 0.45, 0.34}, {128, 0.95, 0.95}, {256, 2.6, 2.6}};
+  static constexpr Rate kBf16[3] = {{64, 0.18, 0.16}, {128, 0.47, 0.43}, {256, 1.0, 1.0}};
+  static constexpr Rate kF32[3] = {{64, 0.51, 0.43}, {128, 1.01, 0.96}, {256, 2.62, 2.62}};
   const Rate* rates = dy_bf16 ? kBf16 : kF32;
-  const double values = static_cast<double>(k) * c * 4e-6 / 6;  // us to move one fp32 dw
+  const double values = static_cast<double>(k) * c * 4e-6 / 5.9;  // us to move one fp32 dw
   const double inputs = rows * (k * (dy_bf16 ? 2.0 : 4.0) + c) * 1e-6 / 4.5;
   Shape best{};
   double least = 0.0;
