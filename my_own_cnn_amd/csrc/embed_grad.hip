@@ -2,18 +2,27 @@
 //
 // The (row, position) pairs of the tokens are sorted, stably, so that a row's tokens stand together
 // in order of position; a position without a token has the key `vocab` and sorts to the end.  Up
-// to kRankTokens tokens each token counts the ones before it directly, in one launch; above that
-// the keys go through stable counting passes of up to 10 bits, two launches each.  The sorted list
-// is then cut into chunks of a fixed length: a group of lanes walks one chunk and 512 channels,
-// adds the rows of dy of each run of equal keys in fp32 and writes the runs that lie within its
-// chunk.  A run that reaches over a chunk's end leaves one partial sum per chunk in the workspace,
-// and a last launch adds those in order.  The cuts depend on the number of tokens and channels
-// alone: every call gives the same bits.
+// to kRankTokens tokens each token counts the ones before it directly, in one launch (a call of 4096
+// tokens 24 us, 30 with the counting passes; of 8192 31 and 38); above that the keys go through
+// stable counting passes of up to 10 bits, two launches each.  The sorted list is then cut into
+// chunks of a fixed length: a group of lanes walks one chunk and 512 channels, adds the rows of dy
+// of each run of equal keys in fp32 and writes the runs that lie within its chunk.  A run that
+// reaches over a chunk's end leaves one partial sum per chunk in the workspace, and a last launch
+// adds those in order.  The cuts depend on the number of tokens and channels alone: every call
+// gives the same bits.
 //
 // Rows without a token, most of the table in a common batch, are zeroed by workgroups of the
 // launch that adds.  A row has a token exactly if where[row] is a place of the sorted list that
 // holds its key: the sort writes where[] for the rows that it sees, and what the others hold is
 // tested, not trusted, so nothing has to be cleared.
+//
+// Bound by memory: dy once, the table once.  65536 tokens on 65536 x 2048, bf16 to fp32: 806 MB in
+// 197 us, of them the launch that adds and zeros 160 (5 TB/s; a large copy reaches 4.8), the sort
+// 28, the join 9.  A lane stores runs of 16 bytes next to its neighbours' (two runs of an fp32 row):
+// with 32 bytes per lane the call took 217 us, and 20011 tokens on 50021 x 1001 99 instead of 73.
+// Six workgroups per CU with four rows in flight per lane (five for fp32 rows): 198 us, with eight
+// rows and four workgroups 206.  A chunk's length goes by the tokens and channels, so that a call
+// has some 262144 lanes; zeros after the sums, not among them (61 -> 87 us on the odd table).
 #include "train_device.h"
 
 namespace miq {
@@ -83,10 +92,13 @@ __device__ __forceinline__ unsigned key_of(const void* ids, bool wide, int64_t t
 
 // ---- up to kRankTokens tokens: a token's place is the number of tokens that sort before it -----
 
-// 64 tokens per workgroup, one per lane; the 16 waves share the tokens to compare with.
+// 64 / SHARES tokens per workgroup, each held by SHARES lanes of every wave; these and the 16 waves
+// share the tokens to compare with.
+template <int SHARES>
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const void* __restrict__ ids, bool ids64, int tokens,
                                                           unsigned vocab, unsigned* __restrict__ keys,
                                                           int* __restrict__ order, unsigned* __restrict__ where) {
+  constexpr int kRanked = 64 / SHARES;
   typedef unsigned v4u __attribute__((ext_vector_type(4)));
   __shared__ __attribute__((aligned(16))) unsigned all[kRankTokens];
   __shared__ int counts[16][64];
@@ -95,18 +107,20 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const void* __restrict
   __syncthreads();
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int t0 = blockIdx.x * 64;
-  const int t = t0 + lane;
+  const int share = lane / kRanked;
+  const int t = blockIdx.x * kRanked + lane % kRanked;
   const unsigned mine = all[t];
+  const int t0 = t & ~63;  // the group of 64 that holds the workgroup's tokens
   int n = 0;
-  // waves 0 .. 15 take every 16th group of 64 tokens: equal keys count where they come before
-  for (int g = wave * 64; g < padded; g += 1024) {
-    const unsigned least = g < t0 ? mine : mine - 1;  // all[i] <= least; a key 0 has none before it
+  // equal keys count where they come before; a group's keys in turns that keep the shares in
+  // different banks
+  for (int g = (wave * SHARES + share) * 64; g < padded; g += 1024 * SHARES) {
     if (g != t0) {
+      const unsigned least = g < t0 ? mine : mine - 1;  // all[i] <= least; a key 0 has none below it
       if (g < t0 || mine != 0) {
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {
-          const v4u k = *reinterpret_cast<const v4u*>(&all[g + i]);
+          const v4u k = *reinterpret_cast<const v4u*>(&all[g + ((i + 4 * share) & 63)]);
           n += (k[0] <= least) + (k[1] <= least) + (k[2] <= least) + (k[3] <= least);
         }
       }
@@ -115,16 +129,18 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const void* __restrict
       for (int i = 0; i < 64; i += 4) {
         const v4u k = *reinterpret_cast<const v4u*>(&all[g + i]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) n += k[j] < mine || (k[j] == mine && i + j < lane);
+        for (int j = 0; j < 4; ++j) n += k[j] < mine || (k[j] == mine && g + i + j < t);
       }
     }
   }
   counts[wave][lane] = n;
   __syncthreads();
-  if (wave == 0 && t < tokens) {
+  if (threadIdx.x < kRanked && t < tokens) {
     int place = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) place += counts[w][lane];
+    for (int w = 0; w < 16; ++w)
+#pragma unroll
+      for (int s = 0; s < SHARES; ++s) place += counts[w][s * kRanked + lane];
     keys[place] = mine;
     order[place] = t;
     if (mine < vocab) where[mine] = static_cast<unsigned>(place);
@@ -516,7 +532,13 @@ hipError_t launch(const EmbedGradArgs& a, hipStream_t stream) {
   int* order = reinterpret_cast<int*>(ws + p.order0);
   unsigned* where = reinterpret_cast<unsigned*>(ws + p.where);
   if (a.tokens > 0 && p.passes == 0) {
-    embed_rank_kernel<<<(a.tokens + 63) / 64, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order, where);
+    // two lanes per token where 64 tokens a workgroup leave half of the CUs without one and the work
+    // counts: 8192 tokens 34.0 -> 30.8 us a call, 1024 tokens 16.9 -> 17.4
+    if (a.tokens <= kRankTokens / 2) {
+      embed_rank_kernel<1><<<(a.tokens + 63) / 64, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order, where);
+    } else {
+      embed_rank_kernel<2><<<(a.tokens + 31) / 32, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order, where);
+    }
   } else if (a.tokens > 0) {
     unsigned* keys_to = reinterpret_cast<unsigned*>(ws + p.keys1);
     int* order_to = reinterpret_cast<int*>(ws + p.order1);
