@@ -2,7 +2,14 @@
 //
 // Every kernel is one pass over its tensors.  A lane holds 16 bytes of consecutive channels (8 of
 // bf16, 4 of fp32), so 4 or 8 neighbouring lanes share one exponent byte; a row's chunks are padded
-// to whole groups, which keeps those lanes in one row whatever the row's length.
+// to whole groups, which keeps those lanes in one row whatever the row's length.  The largest
+// magnitude of a group goes round its lanes by two or three exchanges; scaling by a power of two is
+// exact, so the codes depend on no rounding but their own.
+//
+// Bound by memory.  Gated silu on 16384 x 8192 bf16: forward 190 us for 1082 MB (5.7 TB/s), backward
+// 250 us for as much (4.3 TB/s, half of it written); a large copy reaches 4.8.  50176 x 128 fp32
+// kept and expanded: 8.5 and 7.9 us for 32 MB each, some 2 of them the launch.  Stores of 32 bytes per
+// lane of fp32 took 8.7 us there; lanes of 8 fp32 values kept faster (7.6 us) and expanded slower.
 #include "train_device.h"
 
 namespace miq {
