@@ -328,7 +328,7 @@ struct Sum {
         store44(to, apart, acc);
       } else {
         if (accumulate) acc += load8(to);
-        store8(to, acc);
+        store_run<false>(to, acc);
       }
     } else {
       if (accumulate) acc += load44_of(to, apart, c - col);
@@ -363,8 +363,8 @@ __device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
     } else {
 #pragma unroll 4
       for (int col = lane * W; col < s.c; col += 64 * W) {
-        if constexpr (W == 4) store4(row + min(col, s.c - 4), v4f{});
-        else store8(row + min(col, s.c - 8), v8f{});
+        if constexpr (W == 4) store_run<false>(row + min(col, s.c - 4), v4f{});
+        else store_run<false>(row + min(col, s.c - 8), v8f{});
       }
     }
   }

@@ -1,5 +1,5 @@
-// Device helpers shared by the token-network kernels: eight consecutive values of a row as fp32,
-// and the 8-bit form of a group of channels.
+// Device helpers shared by the token-network kernels: runs of a row's values as fp32, codes as fp32,
+// token ids.
 #pragma once
 
 #include "qconv_device.h"
@@ -25,20 +25,7 @@ __device__ __forceinline__ v8f load8(const float* p) {
 __device__ __forceinline__ v8f load8(const __bf16* p) {
   return __builtin_convertvector(*reinterpret_cast<const v8bf_any*>(p), v8f);
 }
-__device__ __forceinline__ void store8(float* p, const v8f& v) {
-  const v4f a{v[0], v[1], v[2], v[3]}, b{v[4], v[5], v[6], v[7]};
-  *reinterpret_cast<v4f_any*>(p) = a;
-  store_gap(a);
-  *reinterpret_cast<v4f_any*>(p + 4) = b;
-  store_gap(b);
-}
-__device__ __forceinline__ void store8(__bf16* p, const v8f& v) {
-  const v8bf b = __builtin_convertvector(v, v8bf);  // to nearest even
-  *reinterpret_cast<v8bf_any*>(p) = b;
-  store_gap(__builtin_bit_cast(v4i, b));
-}
-
-// The first n (0 .. 8) of eight values; the rest read zero and are not stored.
+// The first n (0 .. 8) of eight values; the rest read zero.
 template <typename T>
 __device__ __forceinline__ v8f load8_of(const T* p, int n) {
   if (n >= 8) return load8(p);
@@ -48,19 +35,9 @@ __device__ __forceinline__ v8f load8_of(const T* p, int n) {
     if (i < n) v[i] = static_cast<float>(p[i]);
   return v;
 }
-template <typename T>
-__device__ __forceinline__ void store8_of(T* p, const v8f& v, int n) {
-  if (n >= 8) {
-    store8(p, v);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = static_cast<T>(v[i]);
-}
 
-// store8 and store4 past the caches (STREAM): for outputs that no cache holds until they are read.
-// A launch decides by stream_stores().
+// 16 bytes of a row; past the caches (STREAM) for outputs that no cache holds until they are read, as
+// stream_stores() says.
 template <bool STREAM>
 __device__ __forceinline__ void store_run(__bf16* p, const v8f& v) {
   const v8bf b = __builtin_convertvector(v, v8bf);  // to nearest even
@@ -84,20 +61,13 @@ __device__ __forceinline__ v4f load4(const float* p) { return *reinterpret_cast<
 __device__ __forceinline__ v4f load4(const __bf16* p) {
   return __builtin_convertvector(*reinterpret_cast<const v4bf_any*>(p), v4f);
 }
-__device__ __forceinline__ void store4(float* p, const v4f& v) {
-  *reinterpret_cast<v4f_any*>(p) = v;
-  store_gap(v);
-}
-__device__ __forceinline__ void store4(__bf16* p, const v4f& v) {
-  *reinterpret_cast<v4bf_any*>(p) = __builtin_convertvector(v, v4bf);  // to nearest even
-}
 template <typename T>
 __device__ __forceinline__ v8f load44(const T* p, int apart) {
   return __builtin_shufflevector(load4(p), load4(p + apart), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 __device__ __forceinline__ void store44(float* p, int apart, const v8f& v) {
-  store4(p, __builtin_shufflevector(v, v, 0, 1, 2, 3));
-  store4(p + apart, __builtin_shufflevector(v, v, 4, 5, 6, 7));
+  store_run<false>(p, __builtin_shufflevector(v, v, 0, 1, 2, 3));
+  store_run<false>(p + apart, __builtin_shufflevector(v, v, 4, 5, 6, 7));
 }
 // Of a row that ends n elements after p.
 template <typename T>

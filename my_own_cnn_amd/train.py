@@ -12,7 +12,6 @@ from __future__ import annotations
 import ctypes as C
 from typing import NamedTuple, Optional
 
-from . import _capi
 from ._capi import ACTS, MIQ_BF16, MIQ_F32, MIQ_I32, MIQ_I64, check, lib
 from .conv import _current_device, _stream
 
@@ -362,4 +361,3 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
 
 __all__ = ["Act8", "act8_bprop", "act8_expand", "act8_fprop", "act8_grad", "act8_grad_workspace_size", "act8_keep",
            "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad"]
-_ = _capi

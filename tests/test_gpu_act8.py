@@ -380,22 +380,23 @@ def test_weight_gradient_against_differences(device):
         assert (loss(up) - loss(down)) / 2 == float(dw[j, i])
 
 
-def test_other_stream_and_graph_replays(device):
-    kept, _ = _kept(device, 1, 3000, 64)
-    dy = torch.randn((3000, 100), device=device)
+@pytest.mark.parametrize("rows,c,k,kind", [(3000, 64, 100, F32), (700, 2048, 2048, F32), (700, 2048, 4096, BF16)])
+def test_other_stream_and_graph_replays(device, rows, c, k, kind):
+    kept, _ = _kept(device, 1, rows, c)
+    dy = torch.randn((rows, k), device=device).to(kind)
     want = M.act8_grad(dy, kept)
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
     got = M.act8_grad(dy, kept, stream=side)
     side.synchronize()
     assert torch.equal(got, want)
-    ws = torch.empty(M.act8_grad_workspace_size(3000, 64, 100), dtype=torch.uint8, device=device)
-    out = torch.empty((100, 64), device=device)
+    ws = torch.empty(M.act8_grad_workspace_size(rows, c, k, kind), dtype=torch.uint8, device=device)
+    out = torch.empty((k, c), device=device)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         M.act8_grad(dy, kept, out=out, workspace=ws)
     for seed in range(4):
-        dy.copy_(torch.randn((3000, 100), generator=torch.Generator().manual_seed(seed)).to(device))
+        dy.copy_(torch.randn((rows, k), generator=torch.Generator().manual_seed(seed)).to(device))
         out.fill_(-1)
         graph.replay()
         torch.cuda.synchronize()

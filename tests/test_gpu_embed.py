@@ -48,17 +48,18 @@ def test_lookup_is_the_scaled_row(device, tokens, vocab, c, table_type, out_type
         assert got.dtype == out_type and torch.equal(got, want)
 
 
-def test_lookup_of_row_slices_shapes_and_no_tokens(device):
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_lookup_of_row_slices_shapes_and_no_tokens(device, kind):
     g = torch.Generator().manual_seed(3)
-    wide = torch.randn((50, 40), generator=g).to(device)
-    table = wide[:, 3:36]  # rows 40 apart, every alignment
+    wide = torch.randn((50, 41), generator=g).to(kind).to(device)
+    table = wide[:, 3:36]  # rows 41 apart, every alignment
     ids = torch.randint(0, 50, (2, 3, 5), generator=g).to(device)
-    into = torch.full((2, 3, 5, 48), -7.0, device=device)
+    into = torch.full((2, 3, 5, 49), -7.0, dtype=kind, device=device)
     got = M.embed_fprop(table, ids, out=into[..., 5:38])
     assert torch.equal(got, table[ids])
     assert (into[..., :5] == -7).all() and (into[..., 38:] == -7).all()
     assert M.embed_fprop(table, ids[:0]).shape == (0, 3, 5, 33)
-    empty = torch.empty((0, 9), device=device)
+    empty = torch.empty((0, 9), dtype=kind, device=device)
     assert (M.embed_fprop(empty, ids) == 0).all()
 
 
@@ -127,14 +128,17 @@ def test_gradient_of_integers_is_exact_and_accumulates(device, tokens, vocab, c,
     np.testing.assert_array_equal(out.cpu().numpy(), want)
 
 
-def test_gradient_of_row_slices_and_no_tokens(device):
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_gradient_of_row_slices_and_no_tokens(device, kind):
     rng = np.random.default_rng(9)
-    dy = torch.from_numpy(rng.integers(-3, 4, (4, 25, 50)).astype(np.float32)).to(device)[..., 7:40]
+    dy = torch.from_numpy(rng.integers(-3, 4, (4, 25, 51)).astype(np.float32)).to(kind).to(device)[..., 7:40]
     ids = torch.from_numpy(rng.integers(0, 20, (4, 25))).to(device)
-    into = torch.full((20, 41), -7.0, device=device)
+    into = torch.full((20, 41), -7.0, dtype=kind, device=device)
     M.embed_grad(dy, ids, 20, out=into[:, 5:38])
     want, _, _ = _want(dy.cpu().double().numpy().reshape(100, 33), ids.cpu().numpy().reshape(-1), 20)
-    np.testing.assert_array_equal(into[:, 5:38].cpu().numpy(), want)
+    np.testing.assert_array_equal(into[:, 5:38].cpu().double().numpy(), want)
+    M.embed_grad(dy, ids, 20, out=into[:, 5:38], accumulate=True)  # sums of integers: exact in bf16 to 256
+    np.testing.assert_array_equal(into[:, 5:38].cpu().double().numpy(), 2 * want)
     assert (into[:, :5] == -7).all() and (into[:, 38:] == -7).all()
     none = M.embed_grad(dy[:0], ids[:0], 20)
     assert none.shape == (20, 33) and (none == 0).all()
