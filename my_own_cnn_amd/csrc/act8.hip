@@ -7,7 +7,8 @@
 // exact, so the codes depend on no rounding but their own.
 //
 // Bound by memory.  Gated silu on 16384 x 8192 bf16: forward 190 us for 1082 MB (5.7 TB/s), backward
-// 250 us for as much (4.3 TB/s, half of it written); a large copy reaches 4.8.  50176 x 128 fp32
+// 243 us for as much (4.5 TB/s); a large copy reaches 4.8.  Both one after the other: 453 us, 436 with
+// stores past the caches, 427 with loads past them too.  50176 x 128 fp32
 // kept and expanded: 8.5 and 7.9 us for 32 MB each, some 2 of them the launch.  Stores of 32 bytes per
 // lane of fp32 took 8.7 us there; lanes of 8 fp32 values kept faster (7.6 us) and expanded slower.
 #include "train_device.h"
@@ -63,13 +64,39 @@ struct Vec<4> {
   typedef v4f type;
 };
 
-__device__ __forceinline__ v8f load_all(const __bf16* p) { return load8(p); }
-__device__ __forceinline__ v4f load_all(const float* p) { return load4(p); }
+// Past the caches too where the output is (STREAM): what is read once leaves no room for what is not.
+template <bool STREAM>
+__device__ __forceinline__ v8f load_run(const __bf16* p) {
+  const v8bf_any* const q = reinterpret_cast<const v8bf_any*>(p);
+  if constexpr (STREAM) return __builtin_convertvector(__builtin_nontemporal_load(q), v8f);
+  else return __builtin_convertvector(*q, v8f);
+}
+template <bool STREAM>
+__device__ __forceinline__ v4f load_run(const float* p) {
+  const v4f_any* const q = reinterpret_cast<const v4f_any*>(p);
+  if constexpr (STREAM) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+template <bool STREAM>
+__device__ __forceinline__ void load_codes(const int8_t* p, int (&q)[2]) {
+  const v2i_any* const from = reinterpret_cast<const v2i_any*>(p);
+  v2i w;
+  if constexpr (STREAM) w = __builtin_nontemporal_load(from);
+  else w = *from;
+  q[0] = w[0];
+  q[1] = w[1];
+}
+template <bool STREAM>
+__device__ __forceinline__ void load_codes(const int8_t* p, int (&q)[1]) {
+  const int_any* const from = reinterpret_cast<const int_any*>(p);
+  if constexpr (STREAM) q[0] = __builtin_nontemporal_load(from);
+  else q[0] = *from;
+}
 
 // The first `left` of a lane's channels; the rest read zero and are not stored.
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ typename Vec<kWide<T>>::type load_some(const T* p, int left) {
-  if (left >= kWide<T>) return load_all(p);
+  if (left >= kWide<T>) return load_run<STREAM>(p);
   typename Vec<kWide<T>>::type v = {};
 #pragma unroll
   for (int i = 0; i < kWide<T>; ++i)
@@ -137,17 +164,11 @@ __device__ __forceinline__ void keep(const typename Vec<W>::type& v, int left, i
   if ((threadIdx.x & (kAct8Group / W - 1)) == 0) *scale = static_cast<uint8_t>(byte);
 }
 
-template <int W>
+template <bool STREAM, int W>
 __device__ __forceinline__ typename Vec<W>::type kept(const int8_t* codes, const uint8_t* scale, int left) {
   int q[W / 4] = {};
   if (left >= W) {
-    if constexpr (W == 8) {
-      const v2i w = *reinterpret_cast<const v2i_any*>(codes);
-      q[0] = w[0];
-      q[1] = w[1];
-    } else {
-      q[0] = *reinterpret_cast<const int_any*>(codes);
-    }
+    load_codes<STREAM>(codes, q);
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i)
@@ -178,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void act8_fprop_kernel(Rows r, const T* _
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       const int col = h * r.c + at;
-      v[h] = load_some(x + row * r.ld_x + col, left);
+      v[h] = load_some<STREAM>(x + row * r.ld_x + col, left);
       keep<W>(v[h], left, codes + row * (H * static_cast<int64_t>(r.c)) + col,
               scales + (row * H + h) * r.groups + at / kAct8Group);
     }
@@ -201,11 +222,11 @@ __global__ __launch_bounds__(kThreads) void act8_bprop_kernel(Rows r, const T* _
     int64_t row;
     int at, left;
     if (!place<W>(r, b, &row, &at, &left) || left <= 0) continue;
-    const V d = load_some(dy + row * r.ld_dy + at, left);
+    const V d = load_some<STREAM>(dy + row * r.ld_dy + at, left);
     V v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h)
-      v[h] = kept<W>(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + at,
+      v[h] = kept<STREAM, W>(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + at,
                      scales + (row * H + h) * r.groups + at / kAct8Group, left);
     V g;
 #pragma unroll
@@ -231,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void act8_expand_kernel(Rows r, const int
     V v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h)
-      v[h] = kept<W>(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + at,
+      v[h] = kept<STREAM, W>(codes + row * (H * static_cast<int64_t>(r.c)) + h * r.c + at,
                      scales + (row * H + h) * r.groups + at / kAct8Group, left);
     V out;
 #pragma unroll
