@@ -13,7 +13,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 from ._capi import ACTS, MIQ_BF16, MIQ_F32, MIQ_I32, MIQ_I64, check, lib
-from .conv import _current_device, _stream
+from .conv import _current_device, _raw_stream, _stream
 
 try:
     import torch
@@ -38,6 +38,14 @@ class Act8(NamedTuple):
     gated: bool = False
 
 
+# A call below takes 7 to 11 us on the host, 3.4 of them in the entry point, 1.4 for each tensor it
+# allocates: small layers are bound by it.  So its checks come inline, their messages from a function.
+_here = _current_device if _current_device is not None else (torch.cuda.current_device if torch is not None else None)
+if _raw_stream is None:  # pragma: no cover - older torch
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
+
+
 def _kind(dtype, what: str) -> int:
     kind = _REAL.get(dtype)
     if kind is None:
@@ -55,13 +63,15 @@ def _on_device(t, what: str) -> None:
     at = t.get_device()
     if at < 0:
         raise ValueError(f"{what} must live in device memory")
-    if at != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+    if at != _here():
         raise ValueError(f"{what} must live on the current device")
 
 
 def _rows(t, what: str):
     """(rows, channels, row distance) of a tensor (..., C)."""
-    _on_device(t, what)
+    at = t.get_device()
+    if at < 0 or at != _here():
+        _on_device(t, what)
     shape = t.shape
     if not shape:
         raise ValueError(f"{what} must have a channel dimension")
@@ -88,7 +98,9 @@ def _rows(t, what: str):
 def _dense(t, dtype, what: str) -> int:
     if t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {dtype}")
-    _on_device(t, what)
+    at = t.get_device()
+    if at < 0 or at != _here():
+        _on_device(t, what)
     return t.data_ptr()
 
 
@@ -156,7 +168,8 @@ def embed_fprop(table, ids, *, scale: float = 1.0, dtype=None, out=None, stream=
     y_kind = _kind(dtype, "dtype")
     y, ld_y = _output(out, ids.shape + (c,), dtype, table, stream)
     status = lib().miq_embed_fprop(table.data_ptr(), ids_at, y.data_ptr(), vocab, c, ids.numel(), ld, ld_y, scale, kind,
-                                   _IDS[ids.dtype], y_kind, _stream(stream))
+                                   _IDS[ids.dtype], y_kind,
+                                   _raw_stream(table.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "embed_fprop")
     return y
@@ -192,7 +205,8 @@ def embed_grad(dy, ids, vocab: int, *, scale: float = 1.0, dtype=None, accumulat
     d, ld_d = _output(out, (vocab, c), dtype, dy, stream)
     at, size, held = _workspace(workspace, "miq_embed_grad_workspace_size", (vocab, c, tokens), dy.device, stream)
     status = lib().miq_embed_grad(dy.data_ptr(), ids_at, d.data_ptr(), vocab, c, tokens, ld, ld_d, scale,
-                                  1 if accumulate else 0, kind, _IDS[ids.dtype], d_kind, at, size, _stream(stream))
+                                  1 if accumulate else 0, kind, _IDS[ids.dtype], d_kind, at, size,
+                                  _raw_stream(dy.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "embed_grad")
     return d
@@ -208,37 +222,37 @@ def _halves(width: int, gated: bool) -> int:
     return width // 2
 
 
-def _new_kept(x, c: int, act: str, gated: bool, kept: Optional[Act8], stream) -> Act8:
-    groups = (c + GROUP - 1) // GROUP * (2 if gated else 1)
-    if kept is None:
-        shape = x.shape
-        if stream is None:
-            return Act8(x.new_empty(shape, dtype=torch.int8), x.new_empty(shape[:-1] + (groups,), dtype=torch.uint8), act,
-                        gated)
-        return Act8(_alloc(shape, torch.int8, x.device, stream),
-                    _alloc(shape[:-1] + (groups,), torch.uint8, x.device, stream), act, gated)
-    _dense(kept.codes, torch.int8, "codes")
-    _dense(kept.scales, torch.uint8, "scales")
-    if kept.codes.shape != x.shape or kept.scales.shape != x.shape[:-1] + (groups,):
-        raise ValueError(f"kept must hold codes of shape {tuple(x.shape)} and {groups} scales a row")
-    return Act8(kept.codes, kept.scales, act, gated)
+def _new_kept(x, shape, lead, groups: int, act: str, gated: bool, kept: Optional[Act8], stream) -> Act8:
+    """Storage for x (of `shape`, rows `lead`) kept in 8 bits: `kept`, or new."""
+    if kept is not None:
+        _dense(kept.codes, torch.int8, "codes")
+        _dense(kept.scales, torch.uint8, "scales")
+        if kept.codes.shape != shape or kept.scales.shape != lead + (groups,):
+            raise ValueError(f"kept must hold codes of shape {tuple(shape)} and {groups} scales a row")
+        return Act8(kept.codes, kept.scales, act, gated)
+    if stream is None:
+        return Act8(x.new_empty(shape, dtype=torch.int8), x.new_empty(lead + (groups,), dtype=torch.uint8), act, gated)
+    return Act8(_alloc(shape, torch.int8, x.device, stream), _alloc(lead + (groups,), torch.uint8, x.device, stream), act,
+                gated)
 
 
 def _kept(kept: Act8):
-    """(rows, channels) of a kept tensor."""
+    """(rows, channels, shape of the codes, shape of their rows) of a kept tensor."""
     codes, scales, _, gated = kept
-    _dense(codes, torch.int8, "codes")
-    _dense(scales, torch.uint8, "scales")
+    at = codes.get_device()
+    if (codes.dtype != torch.int8 or scales.dtype != torch.uint8 or at < 0 or at != _here() or
+            scales.get_device() != at or not codes.is_contiguous() or not scales.is_contiguous()):
+        _dense(codes, torch.int8, "codes")
+        _dense(scales, torch.uint8, "scales")
     shape = codes.shape
     if not shape:
         raise ValueError("codes must have a channel dimension")
-    width = shape[-1]
-    c = _halves(width, gated)
-    groups = (c + GROUP - 1) // GROUP * (2 if gated else 1)
+    c = _halves(shape[-1], True) if gated else shape[-1]
+    groups = (c + 31) // GROUP * (2 if gated else 1)
     lead = shape[:-1]
     if scales.shape != lead + (groups,):
         raise ValueError(f"scales must be {tuple(lead) + (groups,)}, got {tuple(scales.shape)}")
-    return lead.numel(), c
+    return lead.numel(), c, shape, lead
 
 
 def act8_fprop(x, act: str = "silu", *, gated: bool = False, out=None, kept: Optional[Act8] = None, stream=None):
@@ -246,13 +260,17 @@ def act8_fprop(x, act: str = "silu", *, gated: bool = False, out=None, kept: Opt
     of what it multiplies, (..., 2C), and the result is act(gate) * up, (..., C).  `act`: 'none',
     'relu', 'silu' or 'gelu'.  The activation is that of x itself, not of the kept values.  `kept`:
     an Act8 to write into."""
-    kind, which = _kind(x.dtype, "x"), _act(act)
+    dtype = x.dtype
+    kind, which = _kind(dtype, "x"), _act(act)
     rows, width, ld = _rows(x, "x")
-    c = _halves(width, gated)
-    y, ld_y = _output(out, x.shape[:-1] + (c,), x.dtype, x, stream)
-    held = _new_kept(x, c, act, gated, kept, stream)
+    shape = x.shape
+    lead = shape[:-1]
+    c = _halves(width, True) if gated else width
+    y, ld_y = _output(out, lead + (c,), dtype, x, stream)
+    held = _new_kept(x, shape, lead, (c + 31) // GROUP * (2 if gated else 1), act, gated, kept, stream)
     status = lib().miq_act8_fprop(x.data_ptr(), y.data_ptr(), held[0].data_ptr(), held[1].data_ptr(), rows, c, ld, ld_y,
-                                  which, 1 if gated else 0, kind, _stream(stream))
+                                  which, 1 if gated else 0, kind,
+                                  _raw_stream(x.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "act8_fprop")
     return y, held
@@ -263,9 +281,10 @@ def act8_keep(x, *, kept: Optional[Act8] = None, stream=None) -> Act8:
     that act8_expand gives back."""
     kind = _kind(x.dtype, "x")
     rows, c, ld = _rows(x, "x")
-    held = _new_kept(x, c, "none", False, kept, stream)
+    shape = x.shape
+    held = _new_kept(x, shape, shape[:-1], (c + 31) // GROUP, "none", False, kept, stream)
     status = lib().miq_act8_fprop(x.data_ptr(), None, held[0].data_ptr(), held[1].data_ptr(), rows, c, ld, c, 0, 0, kind,
-                                  _stream(stream))
+                                  _raw_stream(x.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "act8_keep")
     return held
@@ -274,24 +293,22 @@ def act8_keep(x, *, kept: Optional[Act8] = None, stream=None) -> Act8:
 def act8_expand(kept: Act8, *, apply: bool = False, dtype=None, out=None, stream=None):
     """The kept values as float32 or bfloat16 (`dtype`, default float32; exact in both), or with
     `apply` the activation of them recomputed: act(x') or act(gate') * up'."""
-    rows, c = _kept(kept)
-    codes = kept.codes
+    rows, c, shape, lead = _kept(kept)
+    codes, scales, act, gated = kept
     if dtype is None:
         dtype = out.dtype if out is not None else torch.float32
     kind = _kind(dtype, "dtype")
-    shape = codes.shape
-    gated = kept.gated and apply
-    if gated:
-        shape = shape[:-1] + (c,)
-    elif kept.gated:  # the halves of a gated row are rows of their own
-        rows *= 2
+    halves = gated and not apply  # the halves of a gated row are rows of their own
+    if gated and apply:
+        shape = lead + (c,)
     y, ld_y = _output(out, shape, dtype, codes, stream)
-    if kept.gated and not apply:
+    if halves:
         if not y.is_contiguous():
             raise ValueError("out must be contiguous for the values of gated rows")
-        ld_y = c
-    status = lib().miq_act8_expand(codes.data_ptr(), kept.scales.data_ptr(), y.data_ptr(), rows, c, ld_y,
-                                   _act(kept.act) if apply else 0, 1 if gated else 0, kind, _stream(stream))
+        rows, ld_y = 2 * rows, c
+    status = lib().miq_act8_expand(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), rows, c, ld_y,
+                                   _act(act) if apply else 0, 1 if gated and apply else 0, kind,
+                                   _raw_stream(codes.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "act8_expand")
     return y
@@ -301,14 +318,15 @@ def act8_bprop(dy, kept: Act8, *, out=None, stream=None):
     """The backward pass of act8_fprop at the kept values: dy * act'(x'), or for gated rows
     [dy * up' * act'(gate'), dy * act(gate')]; dy (..., C), float32 or bfloat16."""
     kind = _kind(dy.dtype, "dy")
-    rows, c = _kept(kept)
+    rows, c, shape, lead = _kept(kept)
     codes, scales, act, gated = kept
-    if dy.shape != codes.shape[:-1] + (c,):
-        raise ValueError(f"dy must be {tuple(codes.shape[:-1]) + (c,)}, got {tuple(dy.shape)}")
+    if dy.shape != lead + (c,):
+        raise ValueError(f"dy must be {tuple(lead) + (c,)}, got {tuple(dy.shape)}")
     _, _, ld = _rows(dy, "dy")
-    dx, ld_dx = _output(out, codes.shape, dy.dtype, dy, stream)
+    dx, ld_dx = _output(out, shape, dy.dtype, dy, stream)
     status = lib().miq_act8_bprop(dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), rows, c, ld, ld_dx,
-                                  _act(act), 1 if gated else 0, kind, _stream(stream))
+                                  _act(act), 1 if gated else 0, kind,
+                                  _raw_stream(dy.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "act8_bprop")
     return dx
@@ -341,10 +359,10 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
     kind = _kind(dy.dtype, "dy")
     if kept.gated:
         raise ValueError("act8_grad takes a layer's input, not gated rows")
-    rows, c = _kept(kept)
+    rows, c, _, lead = _kept(kept)
     _, k, ld = _rows(dy, "dy")
-    if dy.shape[:-1] != kept.codes.shape[:-1]:
-        raise ValueError(f"dy and the kept rows differ: {tuple(dy.shape[:-1])} and {tuple(kept.codes.shape[:-1])}")
+    if dy.shape[:-1] != lead:
+        raise ValueError(f"dy and the kept rows differ: {tuple(dy.shape[:-1])} and {tuple(lead)}")
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if dtype is None:
@@ -353,7 +371,8 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
     dw, ld_dw = _output(out, (k, c), dtype, dy, stream)
     at, size, held = _workspace(workspace, "miq_act8_grad_workspace_size", (rows, c, k, kind), dy.device, stream)
     status = lib().miq_act8_grad(dy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), dw.data_ptr(), rows, c, k,
-                                 ld, ld_dw, 1 if accumulate else 0, kind, dw_kind, at, size, _stream(stream))
+                                 ld, ld_dw, 1 if accumulate else 0, kind, dw_kind, at, size,
+                                 _raw_stream(dy.get_device()) if stream is None else _stream(stream))
     if status:
         check(status, "act8_grad")
     return dw
