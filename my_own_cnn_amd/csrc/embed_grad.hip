@@ -17,9 +17,10 @@
 // tested, not trusted, so nothing has to be cleared.
 //
 // Bound by memory: dy once, the table once.  65536 tokens on 65536 x 2048, bf16 to fp32: 806 MB in
-// 197 us, of them the launch that adds and zeros 160 (5 TB/s; a large copy reaches 4.8), the sort
+// 201 us, of them the launch that adds and zeros 162 (5 TB/s; a large copy reaches 4.8), the sort
 // 28, the join 9.  A lane stores runs of 16 bytes next to its neighbours' (two runs of an fp32 row):
-// with 32 bytes per lane the call took 217 us, and 20011 tokens on 50021 x 1001 99 instead of 73.
+// with 32 bytes per lane the call took 217 us, and 20011 tokens on 50021 x 1001 99 instead of 73
+// (into memory that the last-level cache still holds; 87 into other).
 // Six workgroups per CU with four rows in flight per lane (five for fp32 rows): 198 us, with eight
 // rows and four workgroups 206.  A chunk's length goes by the tokens and channels, so that a call
 // has some 262144 lanes; zeros after the sums, not among them (61 -> 87 us on the odd table).
