@@ -38,8 +38,10 @@ class Act8(NamedTuple):
     gated: bool = False
 
 
-# A call below takes 7 to 11 us on the host, 3.4 of them in the entry point, 1.4 for each tensor it
-# allocates: small layers are bound by it.  So its checks come inline, their messages from a function.
+# A call below takes 7 to 9 us on the host, 3.4 of them in the entry point, 1 to 1.5 for each tensor it
+# allocates: small layers are bound by it.  So its checks come inline, their messages from a function,
+# shapes are plain tuples (torch's own take 0.3 us longer to join and to allocate from), and a tensor
+# shaped like another comes from empty_like (1.1 us for 1.7).
 _here = _current_device if _current_device is not None else (torch.cuda.current_device if torch is not None else None)
 if _raw_stream is None:  # pragma: no cover - older torch
     def _raw_stream(device):
@@ -121,8 +123,15 @@ def _output(out, shape, dtype, like, stream):
             return like.new_empty(shape, dtype=dtype), shape[-1]
         return _alloc(shape, dtype, like.device, stream), shape[-1]
     if out.shape != shape or out.dtype != dtype:
-        raise ValueError(f"out must be {dtype} of shape {tuple(shape)}")
+        raise ValueError(f"out must be {dtype} of shape {shape}")
     return out, _rows(out, "out")[2]
+
+
+def _alike(out, like, shape, dtype, stream):
+    """_output for a result of the shape of `like`, which is contiguous."""
+    if out is None and stream is None:
+        return torch.empty_like(like, dtype=dtype), shape[-1]
+    return _output(out, shape, dtype, like, stream)
 
 
 _sizes = {}  # workspace bytes by problem
@@ -166,7 +175,7 @@ def embed_fprop(table, ids, *, scale: float = 1.0, dtype=None, out=None, stream=
     if dtype is None:
         dtype = out.dtype if out is not None else table.dtype
     y_kind = _kind(dtype, "dtype")
-    y, ld_y = _output(out, ids.shape + (c,), dtype, table, stream)
+    y, ld_y = _output(out, tuple(ids.shape) + (c,), dtype, table, stream)
     status = lib().miq_embed_fprop(table.data_ptr(), ids_at, y.data_ptr(), vocab, c, ids.numel(), ld, ld_y, scale, kind,
                                    _IDS[ids.dtype], y_kind,
                                    _raw_stream(table.get_device()) if stream is None else _stream(stream))
@@ -228,10 +237,11 @@ def _new_kept(x, shape, lead, groups: int, act: str, gated: bool, kept: Optional
         _dense(kept.codes, torch.int8, "codes")
         _dense(kept.scales, torch.uint8, "scales")
         if kept.codes.shape != shape or kept.scales.shape != lead + (groups,):
-            raise ValueError(f"kept must hold codes of shape {tuple(shape)} and {groups} scales a row")
+            raise ValueError(f"kept must hold codes of shape {shape} and {groups} scales a row")
         return Act8(kept.codes, kept.scales, act, gated)
     if stream is None:
-        return Act8(x.new_empty(shape, dtype=torch.int8), x.new_empty(lead + (groups,), dtype=torch.uint8), act, gated)
+        codes = torch.empty_like(x, dtype=torch.int8) if x.is_contiguous() else x.new_empty(shape, dtype=torch.int8)
+        return Act8(codes, x.new_empty(lead + (groups,), dtype=torch.uint8), act, gated)
     return Act8(_alloc(shape, torch.int8, x.device, stream), _alloc(lead + (groups,), torch.uint8, x.device, stream), act,
                 gated)
 
@@ -244,15 +254,16 @@ def _kept(kept: Act8):
             scales.get_device() != at or not codes.is_contiguous() or not scales.is_contiguous()):
         _dense(codes, torch.int8, "codes")
         _dense(scales, torch.uint8, "scales")
-    shape = codes.shape
+    shape = tuple(codes.shape)
     if not shape:
         raise ValueError("codes must have a channel dimension")
-    c = _halves(shape[-1], True) if gated else shape[-1]
+    width = shape[-1]
+    c = _halves(width, True) if gated else width
     groups = (c + 31) // GROUP * (2 if gated else 1)
     lead = shape[:-1]
     if scales.shape != lead + (groups,):
-        raise ValueError(f"scales must be {tuple(lead) + (groups,)}, got {tuple(scales.shape)}")
-    return lead.numel(), c, shape, lead
+        raise ValueError(f"scales must be {lead + (groups,)}, got {tuple(scales.shape)}")
+    return (codes.numel() // width if width else codes.shape[:-1].numel()), c, shape, lead
 
 
 def act8_fprop(x, act: str = "silu", *, gated: bool = False, out=None, kept: Optional[Act8] = None, stream=None):
@@ -263,10 +274,13 @@ def act8_fprop(x, act: str = "silu", *, gated: bool = False, out=None, kept: Opt
     dtype = x.dtype
     kind, which = _kind(dtype, "x"), _act(act)
     rows, width, ld = _rows(x, "x")
-    shape = x.shape
+    shape = tuple(x.shape)
     lead = shape[:-1]
     c = _halves(width, True) if gated else width
-    y, ld_y = _output(out, lead + (c,), dtype, x, stream)
+    if gated or not x.is_contiguous():
+        y, ld_y = _output(out, lead + (c,), dtype, x, stream)
+    else:
+        y, ld_y = _alike(out, x, shape, dtype, stream)
     held = _new_kept(x, shape, lead, (c + 31) // GROUP * (2 if gated else 1), act, gated, kept, stream)
     status = lib().miq_act8_fprop(x.data_ptr(), y.data_ptr(), held[0].data_ptr(), held[1].data_ptr(), rows, c, ld, ld_y,
                                   which, 1 if gated else 0, kind,
@@ -281,7 +295,7 @@ def act8_keep(x, *, kept: Optional[Act8] = None, stream=None) -> Act8:
     that act8_expand gives back."""
     kind = _kind(x.dtype, "x")
     rows, c, ld = _rows(x, "x")
-    shape = x.shape
+    shape = tuple(x.shape)
     held = _new_kept(x, shape, shape[:-1], (c + 31) // GROUP, "none", False, kept, stream)
     status = lib().miq_act8_fprop(x.data_ptr(), None, held[0].data_ptr(), held[1].data_ptr(), rows, c, ld, c, 0, 0, kind,
                                   _raw_stream(x.get_device()) if stream is None else _stream(stream))
@@ -300,8 +314,9 @@ def act8_expand(kept: Act8, *, apply: bool = False, dtype=None, out=None, stream
     kind = _kind(dtype, "dtype")
     halves = gated and not apply  # the halves of a gated row are rows of their own
     if gated and apply:
-        shape = lead + (c,)
-    y, ld_y = _output(out, shape, dtype, codes, stream)
+        y, ld_y = _output(out, lead + (c,), dtype, codes, stream)
+    else:
+        y, ld_y = _alike(out, codes, shape, dtype, stream)
     if halves:
         if not y.is_contiguous():
             raise ValueError("out must be contiguous for the values of gated rows")
@@ -321,9 +336,9 @@ def act8_bprop(dy, kept: Act8, *, out=None, stream=None):
     rows, c, shape, lead = _kept(kept)
     codes, scales, act, gated = kept
     if dy.shape != lead + (c,):
-        raise ValueError(f"dy must be {tuple(lead) + (c,)}, got {tuple(dy.shape)}")
+        raise ValueError(f"dy must be {lead + (c,)}, got {tuple(dy.shape)}")
     _, _, ld = _rows(dy, "dy")
-    dx, ld_dx = _output(out, shape, dy.dtype, dy, stream)
+    dx, ld_dx = _alike(out, codes, shape, dy.dtype, stream)
     status = lib().miq_act8_bprop(dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), dx.data_ptr(), rows, c, ld, ld_dx,
                                   _act(act), 1 if gated else 0, kind,
                                   _raw_stream(dy.get_device()) if stream is None else _stream(stream))
@@ -362,7 +377,7 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
     rows, c, _, lead = _kept(kept)
     _, k, ld = _rows(dy, "dy")
     if dy.shape[:-1] != lead:
-        raise ValueError(f"dy and the kept rows differ: {tuple(dy.shape[:-1])} and {tuple(lead)}")
+        raise ValueError(f"dy and the kept rows differ: {tuple(dy.shape[:-1])} and {lead}")
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if dtype is None:
