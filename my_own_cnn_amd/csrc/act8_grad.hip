@@ -29,7 +29,6 @@ constexpr int kThreads = 256;
 constexpr int kStep = 32;  // rows m per step
 
 typedef short v4s __attribute__((ext_vector_type(4)));
-typedef short v8s __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef v4i v4i_any __attribute__((aligned(1)));
 
@@ -106,7 +105,7 @@ __global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8
   constexpr int NB = kStep * TC / CB / kThreads;
   constexpr int WK = TK / VK, WC = TC / VC;              // a wave's part
   constexpr int IA = WK / 32, IB = WC / 32;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+  extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int tiles = g.tiles_k * g.tiles_c;
   const int at = xcd_tile(blockIdx.x, gridDim.x);
@@ -127,7 +126,7 @@ __global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8
   const int wave = tid >> 6;
   const int wk = (wave / VC) * WK, wc = (wave % VC) * WC;
 
-  // a thread's chunks: rows a0 + i * (256 * 8 / TK), always the same columns
+  // a thread's chunks: rows a_row + i * kRowsA and b_row + i * kRowsB, always the same columns
   const int a_row = tid / (TK / 8), a_col = (tid % (TK / 8)) * 8;
   const int b_row = tid / (TC / CB), b_col = (tid % (TC / CB)) * CB;
   constexpr int kRowsA = kThreads * 8 / TK, kRowsB = kThreads * CB / TC;
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8
   // which reach only sums that are not stored) among them: inside the range, and not so near the
   // tensors' ends that such a column lies beyond them.
   auto whole = [&](int64_t ld, int64_t width, int64_t first, int64_t span) {
-    const int64_t last = (g.rows - 1) * ld + width - first - span;  // row 0's reads may start here at most
+    const int64_t last = (g.rows - 1) * ld + width - first - span;  // where a row's reads may start at most
     return last < 0 ? int64_t{0} : last / ld + 1;
   };
   // Spreads a half step's other instructions between its matrix instructions: left alone, the
@@ -156,11 +155,11 @@ __global__ __launch_bounds__(VK* VC * 64, TK* TC >= 256 * 256 ? 1 : 2) void act8
     constexpr int kReads = 2 * (P * IA + IB), kWrites = P * NA + NB * CB / 8;
 #pragma unroll
     for (int i = 0; i < kMul; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                          // matrix
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                 // matrix
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * ((kReads + kMul - 1) / kMul), 0);  // LDS reads
-      __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);                          // vector ALU
-      __builtin_amdgcn_sched_group_barrier(0x200, (kWrites + kMul - 1) / kMul, 0);  // LDS writes
-      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                          // loads
+      __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);                                 // vector ALU
+      __builtin_amdgcn_sched_group_barrier(0x200, (kWrites + kMul - 1) / kMul, 0);       // LDS writes
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                                 // loads
     }
   };
   const int64_t safe = min(min(whole(g.ld_dy, g.k, k0, TK), whole(g.c, g.c, c0, TC)),
