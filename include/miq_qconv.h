@@ -458,7 +458,7 @@ int miq_embed_fprop(const void* table, const void* ids, void* y, int64_t vocab, 
                     int64_t ld_table, int64_t ld_y, float scale, int32_t table_type, int32_t id_type, int32_t y_type,
                     void* stream);
 
-/* Bytes of device workspace miq_embed_grad needs (no GPU access). */
+/* Bytes of device workspace miq_embed_grad needs, 0 for few tokens (no GPU access). */
 int miq_embed_grad_workspace_size(int64_t vocab, int32_t c, int64_t tokens, size_t* bytes);
 
 /* The table's gradient: d[v, :] = scale * (sum of dy[t, :] over the t with ids[t] == v), the tokens

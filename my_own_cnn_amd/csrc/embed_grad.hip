@@ -1,8 +1,8 @@
 // The embedding table's gradient by sorted tokens (miq_embed_grad).
 //
 // The (row, position) pairs of the tokens are sorted, stably, so that a row's tokens stand together
-// in order of position; a position without a token has the key `vocab` and sorts to the end.  Up
-// to kRankTokens tokens each token counts the ones before it directly, in one launch (a call of 4096
+// in order of position; a position without a token has the key `vocab` and sorts to the end.  Up to
+// kRankTokens tokens each token counts the ones before it directly, in one launch (a call of 4096
 // tokens 24 us, 30 with the counting passes; of 8192 31 and 38); above that the keys go through
 // stable counting passes of up to 10 bits, two launches each.  The sorted list is then cut into
 // chunks of a fixed length: a group of lanes walks one chunk and 512 channels, adds the rows of dy
@@ -10,6 +10,10 @@
 // reaches over a chunk's end leaves one partial sum per chunk in the workspace, and a last launch
 // adds those in order.  The cuts depend on the number of tokens and channels alone: every call
 // gives the same bits.
+//
+// Up to kDirectTokens tokens nothing is sorted: one launch in which each token's workgroup looks at
+// all tokens and adds its row if it is the row's first (1 to 256 tokens of 512 channels 8 us instead
+// of 12 to 16).
 //
 // Rows without a token, most of the table in a common batch, are zeroed by workgroups of the
 // launch that adds.  A row has a token exactly if where[row] is a place of the sorted list that
@@ -30,6 +34,8 @@ namespace miq {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kDirectTokens = 1024; // most tokens that take no sort
+constexpr int kDirectUnits = 2048;  // and most workgroups that add them
 constexpr int kRankTokens = 8192;   // most tokens that are ranked by counting
 constexpr int kDigitBits = 10;      // most bits of a counting pass
 constexpr int kDigits = 1 << kDigitBits;
@@ -44,6 +50,7 @@ constexpr int kAhead = 4;           // rows of dy in flight per lane
 struct Plan {
   int bits, passes, digit_bits, blocks, per_block;  // counting passes
   int lanes, col_tiles, len, chunks;                // lanes per chunk, chunk length
+  bool direct;                                      // no sort
   size_t keys0, keys1, order0, order1, hist, where, part, total;
 };
 
@@ -65,6 +72,9 @@ Plan make_plan(int32_t vocab, int32_t c, int32_t tokens) {
   p.lanes = 8;
   while (p.lanes < 64 && p.lanes * 8 < c) p.lanes *= 2;
   p.col_tiles = (c + kCols - 1) / kCols;
+  // the last bound keeps the grid below 2^32 threads, with the workgroups that zero
+  p.direct = t <= kDirectTokens && t * p.col_tiles <= kDirectUnits && vocab <= 1 << 27;
+  if (p.direct) return p;  // without a workspace
   // chunks enough for about 1024 lanes on each of the 256 CUs
   const int64_t want = 262144 / (static_cast<int64_t>(p.col_tiles) * p.lanes);
   int64_t len = (t + (want < 1 ? 1 : want) - 1) / (want < 1 ? 1 : want);
@@ -338,24 +348,12 @@ struct Sum {
   }
 };
 
-// Zeros in the rows [first, first + kZeroRows) that no token names.
-template <typename TI, typename TO>
-__device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
-  __shared__ int empty[kZeroRows];
+// Zeros in the rows from `first` on that are marked empty, a row per wave and turn.
+template <int THREADS, typename TI, typename TO>
+__device__ __forceinline__ void zero_marked(const Sum<TI, TO>& s, int64_t first, const int* empty) {
   const int rows = static_cast<int>(min(static_cast<int64_t>(kZeroRows), s.vocab - first));
-  if (static_cast<int>(threadIdx.x) < rows) {
-    bool none = true;
-    if (s.tokens > 0) {  // else there is no workspace
-      const unsigned row = static_cast<unsigned>(first) + threadIdx.x;
-      const unsigned at = s.where[row];
-      none = at >= static_cast<unsigned>(s.tokens) || s.keys[at] != row;
-    }
-    empty[threadIdx.x] = none;
-  }
-  __syncthreads();
-  // a row per wave and turn
   const int lane = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < rows; r += kThreads / 64) {
+  for (int r = threadIdx.x >> 6; r < rows; r += THREADS / 64) {
     if (!empty[r]) continue;
     TO* const row = s.table + (first + r) * s.ld_table;
     constexpr int W = 16 / static_cast<int>(sizeof(TO));
@@ -369,6 +367,19 @@ __device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
       }
     }
   }
+}
+
+// The rows [first, first + kZeroRows) that no token names.
+template <typename TI, typename TO>
+__device__ __forceinline__ void zero_rows(const Sum<TI, TO>& s, int64_t first) {
+  __shared__ int empty[kZeroRows];
+  if (threadIdx.x < kZeroRows && first + threadIdx.x < s.vocab) {
+    const unsigned row = static_cast<unsigned>(first) + threadIdx.x;
+    const unsigned at = s.where[row];
+    empty[threadIdx.x] = at >= static_cast<unsigned>(s.tokens) || s.keys[at] != row;
+  }
+  __syncthreads();
+  zero_marked<kThreads>(s, first, empty);
 }
 
 // A lane's eight values of a row of dy, as loaded.
@@ -468,6 +479,95 @@ __device__ __forceinline__ void sum_chunk(const Sum<TI, TO>& s, int chunk, int t
   }
 }
 
+// ---- up to kDirectTokens tokens: no sort -----------------------------------------------------------
+
+// A workgroup per token and 512 channels: every thread looks at KEYS of the tokens, so that the ones
+// of this token's row are found in order at once, and where the token is the row's first the
+// workgroup adds them, its waves a contiguous part each and the parts in order.  The workgroups after
+// these zero the rows that no token names, kZeroRows each.
+//
+// Bound by launch and latency.  257 to 1024 tokens take workgroups of 512 threads: 1024 tokens on
+// 16384 x 512, fp32, in 9.9 us with all tokens apart, 12.4 with skewed ids and 27.4 with one id (with
+// the sort 15.6, 18.5 and 29.4; of 256 threads 8.3, 17.2 and 54; of 1024 17.1, 16.8 and 27.3).  At most
+// kDirectUnits workgroups: 1024 tokens of 1024 channels 11 us instead of 15, of 2048 channels 21 to 27
+// instead of 16.
+template <int THREADS, int KEYS, typename TI, typename TO>
+__global__ __launch_bounds__(THREADS, 8) void embed_direct_kernel(Sum<TI, TO> s, const void* __restrict__ ids, bool ids64) {
+  constexpr int kWaves = THREADS / 64;
+  constexpr int kRows = sizeof(TI) == 2 ? 8 : 6;  // of dy in flight per lane
+  __shared__ uint64_t found[KEYS * kWaves];
+  __shared__ int pos[KEYS * THREADS];
+  __shared__ v8f parts[kWaves][64];
+  __shared__ int empty[kZeroRows];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int token = blockIdx.x / s.col_tiles;
+  const unsigned mine = token < s.tokens ? key_of(ids, ids64, token, s.vocab) : s.vocab;
+  unsigned key[KEYS];
+#pragma unroll
+  for (int k = 0; k < KEYS; ++k) {
+    const int t = k * THREADS + threadIdx.x;
+    key[k] = t < s.tokens ? key_of(ids, ids64, t, s.vocab) : s.vocab;
+  }
+  if (token >= s.tokens) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x - s.sum_blocks) * kZeroRows;
+    if (threadIdx.x < kZeroRows) empty[threadIdx.x] = 1;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k)
+      if (key[k] >= first && key[k] < first + kZeroRows && key[k] < s.vocab) empty[key[k] - first] = 0;
+    __syncthreads();
+    zero_marked<THREADS>(s, first, empty);
+    return;
+  }
+  if (mine >= s.vocab) return;
+  uint64_t same[KEYS];
+#pragma unroll
+  for (int k = 0; k < KEYS; ++k) {
+    same[k] = __ballot(key[k] == mine);
+    if (lane == 0) found[k * kWaves + wave] = same[k];
+  }
+  __syncthreads();
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < KEYS * kWaves; ++w) {
+    const int here = __popcll(found[w]);
+    if (w % kWaves == wave && key[w / kWaves] == mine)
+      pos[n + __popcll(same[w / kWaves] & ((uint64_t{1} << lane) - 1))] = w * 64 + lane;
+    n += here;
+  }
+  __syncthreads();
+  if (pos[0] != token) return;  // another token is the row's first
+  const int tile = blockIdx.x % s.col_tiles;
+  int col, apart;
+  bool whole;
+  const bool there = s.place(tile, lane, &col, &apart, &whole);
+  const int each = (n + kWaves - 1) / kWaves;
+  const int from = min(wave * each, n), to = min(from + each, n);
+  v8f acc = {};
+  if (there && whole) {
+    for (int i = from; i < to; i += kRows) {
+      Raw8<TI> row[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        load_raw<Sum<TI, TO>::kPairs>(row[j], s.dy + pos[min(i + j, to - 1)] * s.ld_dy + col, apart);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        if (i + j < to) acc += value(row[j]);
+    }
+  } else if (there) {
+    for (int i = from; i < to; ++i) acc += load44_of(s.dy + pos[i] * s.ld_dy + col, apart, s.c - col);
+  }
+  if (n > 1) {
+    parts[wave][lane] = acc;
+    __syncthreads();
+    acc = parts[0][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) acc += parts[w][lane];
+  }
+  if (wave == 0 && there) s.finish(mine, col, apart, whole, acc);
+}
+
 template <typename TI, typename TO>
 __global__ __launch_bounds__(kThreads, sizeof(TI) == 2 ? 6 : 5) void embed_sum_kernel(Sum<TI, TO> s) {
   if (static_cast<int>(blockIdx.x) >= s.sum_blocks) {
@@ -527,28 +627,51 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(Sum<TI, TO> s) {
 template <typename TI, typename TO>
 hipError_t launch(const EmbedGradArgs& a, hipStream_t stream) {
   const Plan p = make_plan(a.vocab, a.c, a.tokens);
+  const int64_t zero_blocks = a.accumulate ? 0 : (static_cast<int64_t>(a.vocab) + kZeroRows - 1) / kZeroRows;
+  Sum<TI, TO> s{};
+  s.dy = static_cast<const TI*>(a.dy);
+  s.table = static_cast<TO*>(a.dtable);
+  s.ld_dy = a.ld_dy;
+  s.ld_table = a.ld_dtable;
+  s.tokens = a.tokens;
+  s.c = a.c;
+  s.lanes = p.lanes;
+  s.col_tiles = p.col_tiles;
+  s.len = p.len;
+  s.chunks = p.chunks;
+  s.vocab = static_cast<unsigned>(a.vocab);
+  s.scale = a.scale;
+  s.accumulate = a.accumulate;
+  if (p.direct) {
+    s.lanes = 64;
+    s.sum_blocks = a.tokens * p.col_tiles;
+    const unsigned blocks = static_cast<unsigned>(s.sum_blocks + zero_blocks);
+    if (a.tokens <= 256) embed_direct_kernel<256, 1><<<blocks, 256, 0, stream>>>(s, a.ids, a.ids64);
+    else embed_direct_kernel<512, kDirectTokens / 512><<<blocks, 512, 0, stream>>>(s, a.ids, a.ids64);
+    return hipGetLastError();
+  }
   char* ws = static_cast<char*>(a.ws);
   const unsigned vocab = static_cast<unsigned>(a.vocab);
   unsigned* keys = reinterpret_cast<unsigned*>(ws + p.keys0);
   int* order = reinterpret_cast<int*>(ws + p.order0);
   unsigned* where = reinterpret_cast<unsigned*>(ws + p.where);
-  if (a.tokens > 0 && p.passes == 0) {
+  if (p.passes == 0) {
     // two lanes per token where 64 tokens a workgroup leave half of the CUs without one and the work
-    // counts: 8192 tokens 34.0 -> 30.8 us a call, 1024 tokens 16.9 -> 17.4
+    // counts: 8192 tokens 34.0 -> 30.8 us a call, 1024 tokens 16.9 -> 17.4 (sorted)
     if (a.tokens <= kRankTokens / 2) {
       embed_rank_kernel<1><<<(a.tokens + 63) / 64, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order, where);
     } else {
       embed_rank_kernel<2><<<(a.tokens + 31) / 32, 1024, 0, stream>>>(a.ids, a.ids64, a.tokens, vocab, keys, order, where);
     }
-  } else if (a.tokens > 0) {
+  } else {
     unsigned* keys_to = reinterpret_cast<unsigned*>(ws + p.keys1);
     int* order_to = reinterpret_cast<int*>(ws + p.order1);
     unsigned* hist = reinterpret_cast<unsigned*>(ws + p.hist);
     for (int i = 0; i < p.passes; ++i) {
-      Pass s{i == 0 ? nullptr : keys, i == 0 ? nullptr : order, a.ids, a.ids64, vocab, a.tokens, p.per_block, p.blocks,
-             i * p.digit_bits, 1 << p.digit_bits};
-      embed_hist_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s, hist);
-      embed_scatter_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s, hist, keys_to, order_to,
+      Pass pass{i == 0 ? nullptr : keys, i == 0 ? nullptr : order, a.ids, a.ids64, vocab, a.tokens, p.per_block, p.blocks,
+                i * p.digit_bits, 1 << p.digit_bits};
+      embed_hist_kernel<<<p.blocks, kSortThreads, 0, stream>>>(pass, hist);
+      embed_scatter_kernel<<<p.blocks, kSortThreads, 0, stream>>>(pass, hist, keys_to, order_to,
                                                                   i == p.passes - 1 ? where : nullptr);
       unsigned* k = keys;
       keys = keys_to;
@@ -558,28 +681,13 @@ hipError_t launch(const EmbedGradArgs& a, hipStream_t stream) {
       order_to = o;
     }
   }
-  Sum<TI, TO> s{};
-  s.dy = static_cast<const TI*>(a.dy);
-  s.table = static_cast<TO*>(a.dtable);
   s.keys = keys;
   s.order = order;
   s.where = where;
   s.part = reinterpret_cast<float*>(ws + p.part);
-  s.ld_dy = a.ld_dy;
-  s.ld_table = a.ld_dtable;
-  s.tokens = a.tokens;
-  s.c = a.c;
-  s.lanes = p.lanes;
-  s.col_tiles = p.col_tiles;
-  s.len = p.len;
-  s.chunks = p.chunks;
-  s.vocab = vocab;
-  s.scale = a.scale;
-  s.accumulate = a.accumulate;
   const int64_t units = static_cast<int64_t>(p.chunks) * p.col_tiles;
   const int64_t per = kThreads / p.lanes;
   s.sum_blocks = static_cast<int>((units + per - 1) / per);
-  const int64_t zero_blocks = a.accumulate ? 0 : (static_cast<int64_t>(a.vocab) + kZeroRows - 1) / kZeroRows;
   embed_sum_kernel<TI, TO><<<static_cast<unsigned>(s.sum_blocks + zero_blocks), kThreads, 0, stream>>>(s);
   if (p.chunks > 1)
     embed_join_kernel<TI, TO><<<static_cast<unsigned>((p.chunks - 1) * p.col_tiles), kThreads, 0, stream>>>(s);

@@ -85,6 +85,8 @@ GRADS = [  # tokens, vocab, c, how the ids fall
     (64, 64, 65, "skewed"), (65, 1000, 32, "even"), (300, 3, 513, "even"), (257, 40, 1001, "skewed"),
     (4096, 5000, 24, "skewed"), (8191, 100, 16, "skewed"), (8192, 70000, 8, "even"), (8193, 300, 16, "skewed"),
     (8193, 5, 512, "same"), (20000, 50021, 40, "skewed"), (20011, 1, 33, "even"), (40000, 1 << 21, 8, "skewed"),
+    (256, 300, 16, "same"), (1024, 7, 512, "same"), (1024, 60000, 4, "even"), (1000, 90, 1024, "skewed"),
+    (682, 50, 1536, "skewed"), (683, 50, 1536, "skewed"), (1025, 90, 72, "skewed"), (1024, 9, 1, "none"),
     (600, 70, 48, "none"), (9000, 70, 48, "none"), (100000, 1030, 64, "skewed"),
 ]
 
@@ -242,5 +244,6 @@ def test_refusals(device):
         M.embed_grad(dy, ids, 4, accumulate=True)
     with pytest.raises(ValueError, match="ids.shape"):
         M.embed_grad(dy[:2], ids, 4)
+    dy, ids = torch.zeros((2000, 8), device=device), torch.zeros(2000, dtype=torch.int64, device=device)
     with pytest.raises(M.MiqError, match="workspace is smaller"):
         M.embed_grad(dy, ids, 4, workspace=torch.empty(16, dtype=torch.uint8, device=device))

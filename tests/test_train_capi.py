@@ -52,8 +52,8 @@ REFUSED = [
     ("miq_embed_grad", GRAD, dict(ld_dy=7), BAD, "row distance"),
     ("miq_embed_grad", GRAD, dict(dtable=None), NULL, "output"),
     ("miq_embed_grad", GRAD, dict(dy=None), NULL, "dy"),
-    ("miq_embed_grad", GRAD, dict(ws=None), NULL, "workspace"),
-    ("miq_embed_grad", GRAD, dict(ws_bytes=8), BAD, "workspace is smaller"),
+    ("miq_embed_grad", GRAD, dict(tokens=2000, ws=None), NULL, "workspace"),
+    ("miq_embed_grad", GRAD, dict(tokens=2000, ws_bytes=8), BAD, "workspace is smaller"),
     ("miq_embed_grad", GRAD, dict(ws=P + 8), BAD, "16 bytes"),
     ("miq_act8_fprop", ACT, dict(rows=-1), BAD, ">= 0"),
     ("miq_act8_fprop", ACT, dict(rows=1 << 41), BAD, "2^40"),
@@ -111,7 +111,8 @@ def test_nothing_to_do_enqueues_nothing(entry, defaults, change):
 
 def test_workspace_sizes():
     assert M.embed_grad_workspace_size(1000, 64, 0) == 0
-    small, large = M.embed_grad_workspace_size(1000, 64, 100), M.embed_grad_workspace_size(1000, 64, 10 ** 6)
+    assert M.embed_grad_workspace_size(1000, 64, 1024) == 0  # few tokens are not sorted
+    small, large = M.embed_grad_workspace_size(1000, 64, 1025), M.embed_grad_workspace_size(1000, 64, 10 ** 6)
     assert 0 < small < large < 10 ** 6 * 16 + (64 << 20)
     assert M.embed_grad_workspace_size(1 << 28, 1 << 20, (1 << 31) - 65) > 0
     assert M.act8_grad_workspace_size(64, 4096, 4096) == 0
