@@ -148,6 +148,37 @@ def test_gradient_of_row_slices_and_no_tokens(device, kind):
     assert (M.embed_grad(dy[:0], ids[:0], 20, accumulate=True, out=kept) == 3).all()
 
 
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("tokens,c", [(1500, 33), (1500, 1030), (9000, 33)])
+def test_sorted_gradient_of_row_slices_with_nan_where_no_token_is(device, kind, tokens, c):
+    rng = np.random.default_rng(tokens + c)
+    ids = rng.integers(-300, 600, tokens)  # a third without a token
+    values = rng.integers(-2, 3, (tokens, c + 9)).astype(np.float32)
+    values[ids < 0] = np.nan
+    dy = torch.from_numpy(values).to(kind).to(device)[:, 7:7 + c]
+    idd = torch.from_numpy(ids).to(device)
+    into = torch.full((600, c + 4), -7.0, dtype=kind, device=device)
+    out = into[:, 3:3 + c]
+    M.embed_grad(dy, idd, 600, out=out)
+    want, _, _ = _want(np.nan_to_num(values[:, 7:7 + c]).astype(np.float64), ids, 600)
+    np.testing.assert_array_equal(out.cpu().double().numpy(), want)
+    M.embed_grad(dy, idd, 600, out=out, accumulate=True)  # sums of integers: exact in bf16 to 256
+    np.testing.assert_array_equal(out.cpu().double().numpy(), 2 * want)
+    assert (into[:, :3] == -7).all() and (into[:, 3 + c:] == -7).all()
+
+
+def test_gradient_rows_beyond_32_bit_offsets(device):
+    tokens, c = 70000, 32768  # 2.3e9 values of dy
+    dy = torch.zeros((tokens, c), dtype=BF16, device=device)
+    ids = torch.full((tokens,), -1, device=device)
+    for t, row in [(0, 1), (65537, 3), (69998, 1), (69999, 4)]:
+        dy[t] = torch.randint(-3, 4, (c,), device=device).to(BF16)
+        ids[t] = row
+    d = M.embed_grad(dy, ids, 6, dtype=BF16)
+    assert torch.equal(d[1], dy[0] + dy[69998]) and torch.equal(d[3], dy[65537]) and torch.equal(d[4], dy[69999])
+    assert (d[[0, 2, 5]] == 0).all()
+
+
 def test_gradient_against_differences(device):
     """The lookup is linear in its table: with values of few bits its differences are exact."""
     rng = np.random.default_rng(4)
