@@ -461,6 +461,11 @@ int miq_embed_fprop(const void* table, const void* ids, void* y, int64_t vocab, 
 /* Bytes of device workspace miq_embed_grad needs, 0 for few tokens (no GPU access). */
 int miq_embed_grad_workspace_size(int64_t vocab, int32_t c, int64_t tokens, size_t* bytes);
 
+/* How miq_embed_grad runs a problem: plan[0] the launches that sort the tokens, plan[1] the parts
+ * that the sorted tokens are cut into; zeros where nothing is sorted (one launch without a
+ * workspace) or there is nothing to do.  No GPU access. */
+int miq_plan_embed_grad(int64_t vocab, int32_t c, int64_t tokens, int32_t plan[2]);
+
 /* The table's gradient: d[v, :] = scale * (sum of dy[t, :] over the t with ids[t] == v), the tokens
  * of a row added in an order that depends on the ids alone.  accumulate == 0 overwrites the whole
  * table (rows without a token are zeros); accumulate != 0 adds to dtable and touches only the rows

@@ -11,7 +11,7 @@ from .conv import (BlockConv2DParams, bmm_i32, bmm_matmul_i32, conv2d_nhwc_f32, 
                    fprop_nhwc_qi32_algo, plan_qi32, plan_block_qi32, qi32_workspace_size,
                    make_desc, plan, plan_f32, plan_f32_split, qconv2d_nhwc_i8, qconv2d_nhwc_i8_acc32, qconv2d_nhwc_i8_dequant, qparams_array)
 from .train import (Act8, act8_bprop, act8_expand, act8_fprop, act8_grad, act8_grad_workspace_size, act8_keep, embed_fprop,
-                    embed_grad, embed_grad_workspace_size, plan_act8_grad)
+                    embed_grad, embed_grad_workspace_size, plan_act8_grad, plan_embed_grad)
 from ._capi import LIB_PATH, lib
 from .workloads import HEADLINE, WORKLOADS, Workload
 
@@ -22,6 +22,6 @@ __all__ = [
     "fprop_nhwc_qi32_algo", "plan_qi32", "plan_block_qi32", "qi32_workspace_size",
     "make_desc", "plan", "plan_f32", "plan_f32_split", "qconv2d_nhwc_i8", "qconv2d_nhwc_i8_acc32", "qconv2d_nhwc_i8_dequant", "qparams_array",
     "Act8", "act8_bprop", "act8_expand", "act8_fprop", "act8_grad", "act8_grad_workspace_size", "act8_keep",
-    "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad",
+    "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad", "plan_embed_grad",
     "LIB_PATH", "lib", "HEADLINE", "WORKLOADS", "Workload",
 ]

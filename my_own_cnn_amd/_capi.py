@@ -155,6 +155,7 @@ SIGNATURES = {
     "miq_plan_block_f32": (C.c_int, [_I, _I, _I, _I, _I, _I, _I, _I, C.POINTER(BlockConv2DParams), _I, _PI]),
     "miq_embed_fprop": (C.c_int, [_P, _P, _P, _L, _I, _L, _L, _L, C.c_float, _I, _I, _I, _P]),
     "miq_embed_grad_workspace_size": (C.c_int, [_L, _I, _L, C.POINTER(C.c_size_t)]),
+    "miq_plan_embed_grad": (C.c_int, [_L, _I, _L, _PI]),
     "miq_embed_grad": (
         C.c_int, [_P, _P, _P, _L, _I, _L, _L, _L, C.c_float, _I, _I, _I, _I, _P, C.c_size_t, _P]),
     "miq_act8_fprop": (C.c_int, [_P, _P, _P, _P, _L, _I, _L, _L, _I, _I, _I, _P]),

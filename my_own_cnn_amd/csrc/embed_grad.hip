@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kDirectTokens = 1024; // most tokens that take no sort
+constexpr int kDirectShort = 256;   // most of them in workgroups of 256 threads
 constexpr int kDirectUnits = 2048;  // and most workgroups that add them
 constexpr int kRankTokens = 8192;   // most tokens that are ranked by counting
 constexpr int kDigitBits = 10;      // most bits of a counting pass
@@ -72,8 +73,10 @@ Plan make_plan(int32_t vocab, int32_t c, int32_t tokens) {
   p.lanes = 8;
   while (p.lanes < 64 && p.lanes * 8 < c) p.lanes *= 2;
   p.col_tiles = (c + kCols - 1) / kCols;
-  // the last bound keeps the grid below 2^32 threads, with the workgroups that zero
-  p.direct = t <= kDirectTokens && t * p.col_tiles <= kDirectUnits && vocab <= 1 << 27;
+  // The last bound keeps the grid of workgroups of 512 threads below 2^32 threads, with the 2^23 of
+  // them that zero 2^28 rows; of 256 threads it is below for every table, so that a call without
+  // tokens, which has no workspace, never comes to the sort.
+  p.direct = t <= kDirectTokens && t * p.col_tiles <= kDirectUnits && (t <= kDirectShort || vocab <= 1 << 27);
   if (p.direct) return p;  // without a workspace
   // chunks enough for about 1024 lanes on each of the 256 CUs
   const int64_t want = 262144 / (static_cast<int64_t>(p.col_tiles) * p.lanes);
@@ -646,7 +649,7 @@ hipError_t launch(const EmbedGradArgs& a, hipStream_t stream) {
     s.lanes = 64;
     s.sum_blocks = a.tokens * p.col_tiles;
     const unsigned blocks = static_cast<unsigned>(s.sum_blocks + zero_blocks);
-    if (a.tokens <= 256) embed_direct_kernel<256, 1><<<blocks, 256, 0, stream>>>(s, a.ids, a.ids64);
+    if (a.tokens <= kDirectShort) embed_direct_kernel<kDirectShort, 1><<<blocks, kDirectShort, 0, stream>>>(s, a.ids, a.ids64);
     else embed_direct_kernel<512, kDirectTokens / 512><<<blocks, 512, 0, stream>>>(s, a.ids, a.ids64);
     return hipGetLastError();
   }
@@ -698,6 +701,12 @@ hipError_t launch(const EmbedGradArgs& a, hipStream_t stream) {
 
 size_t embed_grad_workspace_bytes(int32_t vocab, int32_t c, int32_t tokens) {
   return make_plan(vocab, c, tokens).total;
+}
+
+void plan_embed_grad(int32_t vocab, int32_t c, int32_t tokens, int32_t* sorts, int32_t* chunks) {
+  const Plan p = make_plan(vocab, c, tokens);
+  *sorts = p.direct ? 0 : p.passes == 0 ? 1 : 2 * p.passes;
+  *chunks = p.chunks;
 }
 
 hipError_t launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream) {

@@ -103,6 +103,17 @@ int miq_embed_grad_workspace_size(int64_t vocab, int32_t c, int64_t tokens, size
   return MIQ_OK;
 }
 
+int miq_plan_embed_grad(int64_t vocab, int32_t c, int64_t tokens, int32_t plan[2]) {
+  if (plan == nullptr) return null("plan pointer is NULL");
+  const int st = check_embed_sizes(vocab, c, tokens);
+  if (st != MIQ_OK) return st;
+  plan[0] = plan[1] = 0;
+  if (vocab > 0 && c > 0) {
+    miq::plan_embed_grad(static_cast<int32_t>(vocab), c, static_cast<int32_t>(tokens), &plan[0], &plan[1]);
+  }
+  return MIQ_OK;
+}
+
 int miq_embed_grad(const void* dy, const void* ids, void* dtable, int64_t vocab, int32_t c, int64_t tokens,
                    int64_t ld_dy, int64_t ld_dtable, float scale, int32_t accumulate, int32_t dy_type, int32_t id_type,
                    int32_t dtable_type, void* workspace, size_t workspace_bytes, void* stream) {

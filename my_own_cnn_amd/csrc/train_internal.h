@@ -33,6 +33,7 @@ struct EmbedGradArgs {
   bool accumulate, dy_bf16, ids64, dtable_bf16;
 };
 size_t embed_grad_workspace_bytes(int32_t vocab, int32_t c, int32_t tokens);
+void plan_embed_grad(int32_t vocab, int32_t c, int32_t tokens, int32_t* sorts, int32_t* chunks);
 hipError_t launch_embed_grad(const EmbedGradArgs& a, hipStream_t stream);
 
 // x, y: act8_fprop; dy, y (= dx): act8_bprop; y: act8_expand.

@@ -191,6 +191,14 @@ def embed_grad_workspace_size(vocab: int, c: int, tokens: int) -> int:
     return out.value
 
 
+def plan_embed_grad(vocab: int, c: int, tokens: int):
+    """(launches that sort the tokens, parts that the sorted tokens are cut into) of embed_grad, zeros
+    where nothing is sorted: one launch without a workspace (no GPU access)."""
+    out = (C.c_int32 * 2)()
+    check(lib().miq_plan_embed_grad(vocab, c, tokens, out), "plan_embed_grad")
+    return out[0], out[1]
+
+
 def embed_grad(dy, ids, vocab: int, *, scale: float = 1.0, dtype=None, accumulate: bool = False, out=None,
                workspace=None, stream=None):
     """The gradient of embed_fprop with respect to the table: (vocab, C), float32 or bfloat16
@@ -394,4 +402,4 @@ def act8_grad(dy, kept: Act8, *, dtype=None, accumulate: bool = False, out=None,
 
 
 __all__ = ["Act8", "act8_bprop", "act8_expand", "act8_fprop", "act8_grad", "act8_grad_workspace_size", "act8_keep",
-           "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad"]
+           "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad", "plan_embed_grad"]
