@@ -458,7 +458,9 @@ int miq_embed_fprop(const void* table, const void* ids, void* y, int64_t vocab, 
                     int64_t ld_table, int64_t ld_y, float scale, int32_t table_type, int32_t id_type, int32_t y_type,
                     void* stream);
 
-/* Bytes of device workspace miq_embed_grad needs, 0 for few tokens (no GPU access). */
+/* Bytes of device workspace miq_embed_grad needs: 0 exactly where it sorts nothing, that is for up to
+ * 256 tokens, or up to 1024 on at most 2^27 rows, while tokens * ceil(c / 512) <= 2048, and where
+ * there is nothing to do (no GPU access). */
 int miq_embed_grad_workspace_size(int64_t vocab, int32_t c, int64_t tokens, size_t* bytes);
 
 /* How miq_embed_grad runs a problem: plan[0] the launches that sort the tokens, plan[1] the parts
@@ -467,7 +469,7 @@ int miq_embed_grad_workspace_size(int64_t vocab, int32_t c, int64_t tokens, size
 int miq_plan_embed_grad(int64_t vocab, int32_t c, int64_t tokens, int32_t plan[2]);
 
 /* The table's gradient: d[v, :] = scale * (sum of dy[t, :] over the t with ids[t] == v), the tokens
- * of a row added in an order that depends on the ids alone.  accumulate == 0 overwrites the whole
+ * of a row added in an order that depends on the ids and the sizes alone.  accumulate == 0 overwrites the whole
  * table (rows without a token are zeros); accumulate != 0 adds to dtable and touches only the rows
  * that have a token.  Ids outside [0, vocab) contribute nothing.  dy: tokens x c of dy_type;
  * dtable: vocab x c of dtable_type. */

@@ -8,12 +8,11 @@
 // chunks of a fixed length: a group of lanes walks one chunk and 512 channels, adds the rows of dy
 // of each run of equal keys in fp32 and writes the runs that lie within its chunk.  A run that
 // reaches over a chunk's end leaves one partial sum per chunk in the workspace, and a last launch
-// adds those in order.  The cuts depend on the number of tokens and channels alone: every call
-// gives the same bits.
+// adds those in order.  The cuts depend on the sizes alone: every call gives the same bits.
 //
-// Up to kDirectTokens tokens nothing is sorted: one launch in which each token's workgroup looks at
-// all tokens and adds its row if it is the row's first (1 to 256 tokens of 512 channels 8 us instead
-// of 12 to 16).
+// Up to kDirectTokens tokens (kDirectShort on the largest tables) nothing is sorted: one launch in
+// which each token's workgroup looks at all tokens and adds its row if it is the row's first (1 to
+// 256 tokens of 512 channels 8 us instead of 12 to 16).
 //
 // Rows without a token, most of the table in a common batch, are zeroed by workgroups of the
 // launch that adds.  A row has a token exactly if where[row] is a place of the sorted list that
@@ -491,7 +490,8 @@ __device__ __forceinline__ void sum_chunk(const Sum<TI, TO>& s, int chunk, int t
 //
 // Bound by launch and latency.  257 to 1024 tokens take workgroups of 512 threads: 1024 tokens on
 // 16384 x 512, fp32, in 9.9 us with all tokens apart, 12.4 with skewed ids and 27.4 with one id (with
-// the sort 15.6, 18.5 and 29.4; of 256 threads 8.3, 17.2 and 54; of 1024 17.1, 16.8 and 27.3).  At most
+// the sort 15.6, 18.5 and 29.4; of 256 threads 8.3, 17.2 and 54; of 1024 17.1, 16.8 and 27.3).  2048
+// tokens apart would take 21 to 31 us, 17 with the sort: kDirectTokens ends before.  At most
 // kDirectUnits workgroups: 1024 tokens of 1024 channels 11 us instead of 15, of 2048 channels 21 to 27
 // instead of 16.
 template <int THREADS, int KEYS, typename TI, typename TO>

@@ -203,7 +203,7 @@ def embed_grad(dy, ids, vocab: int, *, scale: float = 1.0, dtype=None, accumulat
                workspace=None, stream=None):
     """The gradient of embed_fprop with respect to the table: (vocab, C), float32 or bfloat16
     (`dtype`, default float32), row v the sum of scale * dy over the positions whose id is v, in an
-    order fixed by the ids.  `accumulate` adds it to `out` and touches only rows that have a token.
+    order fixed by the ids and the sizes.  `accumulate` adds it to `out` and touches only rows that have a token.
     `workspace`: a device buffer of at least embed_grad_workspace_size() bytes, not used by another
     call in flight; None allocates one from PyTorch for this call."""
     kind = _kind(dy.dtype, "dy")
