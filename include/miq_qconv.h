@@ -491,7 +491,7 @@ int miq_embed_grad(const void* dy, const void* ids, void* dtable, int64_t vocab,
 typedef enum miq_act {
   MIQ_ACT_NONE = 0,
   MIQ_ACT_RELU = 1,
-  MIQ_ACT_SILU = 2, /* v / (1 + exp(-v)) */
+  MIQ_ACT_SILU = 2, /* v / (1 + exp(-v)), -0 where exp(-v) overflows (v < -88.7, below 3e-37) */
   MIQ_ACT_GELU = 3  /* v * (1 + erf(v / sqrt 2)) / 2 */
 } miq_act;
 
@@ -502,7 +502,8 @@ int miq_act8_fprop(const void* x, void* y, int8_t* codes, uint8_t* scales, int64
                    int64_t ld_y, int32_t act, int32_t gated, int32_t type, void* stream);
 
 /* The activation's backward pass at the kept values x': dx = dy * act'(x'), or, gated, the row
- * [dy * up' * act'(gate'), dy * act(gate')].  dy: rows x c, dx: rows x c (2c gated), of `type`. */
+ * [dy * up' * act'(gate'), dy * act(gate')].  These are products: an infinite dy at a slope of 0 (relu
+ * at x' <= 0) gives NaN.  dy: rows x c, dx: rows x c (2c gated), of `type`. */
 int miq_act8_bprop(const void* dy, const int8_t* codes, const uint8_t* scales, void* dx, int64_t rows, int32_t c,
                    int64_t ld_dy, int64_t ld_dx, int32_t act, int32_t gated, int32_t type, void* stream);
 
