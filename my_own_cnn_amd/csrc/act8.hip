@@ -6,11 +6,18 @@
 // magnitude of a group goes round its lanes by two or three exchanges; scaling by a power of two is
 // exact, so the codes depend on no rounding but their own.
 //
-// Bound by memory.  Gated silu on 16384 x 8192 bf16: forward 190 us for 1082 MB (5.7 TB/s), backward
-// 243 us for as much (4.5 TB/s); a large copy reaches 4.8.  Both one after the other: 453 us, 436 with
-// stores past the caches, 427 with loads past them too.  50176 x 128 fp32
-// kept and expanded: 8.5 and 7.9 us for 32 MB each, some 2 of them the launch.  Stores of 32 bytes per
-// lane of fp32 took 8.7 us there; lanes of 8 fp32 values kept faster (7.6 us) and expanded slower.
+// Bound by memory in fp32 and with relu: 4.8 TB/s, what a large copy reaches, and more.  bf16 moves
+// half the bytes a value, so there the exponential, the division and erfc of silu and gelu take the
+// longer: ungated on 16384 x 8192, forward and backward, relu 5.9 and 5.9 TB/s, silu 4.4 and 4.1, gelu
+// 3.4 and 2.8 (243 us); gated 6.1 and 6.4, 5.3 and 4.5, 4.5 and 3.7.  Vector instructions per value,
+// forward and backward: relu 20 and 16, silu 43 and 41, gelu 69 and 79; ungated silu and gelu issue one
+// each 3.4 to 4.8 cycles and SIMD at 2.4 GHz, and are bound by that.  fp32 on 8192 x 8192, gelu: 4.7 and
+// 4.2 TB/s ungated, 5.7 and 5.4 gated.
+//
+// Gated silu on 16384 x 8192 bf16, one after the other: 453 us, 436 with stores past the caches, 427 to
+// 435 with loads past them too.  50176 x 128 fp32 kept and expanded: 8.7 and 7.8 us for 32 MB each,
+// some 2 of them the launch.  Stores of 32 bytes per lane of fp32 took 8.7 us to expand; lanes of 8 fp32
+// values kept faster (7.6 us) and expanded slower.
 #include "train_device.h"
 
 namespace miq {
@@ -127,7 +134,8 @@ __device__ __forceinline__ bool place(const Rows& r, int64_t block, int64_t* row
   return base + threadIdx.x < r.total;
 }
 
-// The exponent byte of a group, from its largest magnitude (as fp32 bits) in all four lanes.
+// The exponent byte of a group, from its largest magnitude (as fp32 bits) in all of its lanes (4 of
+// bf16, 8 of fp32).
 __device__ __forceinline__ int exponent_byte(unsigned top) {
   const int e = static_cast<int>(top >> 23) - 6 + ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0);
   return top >= 0x7f800000u ? 255 : min(max(e, 1), 248);

@@ -12,14 +12,16 @@
 // the transposing LDS read gives a lane four m of its column at once.  The rows of LDS are permuted
 // in units of 16 columns (32 bytes) by their m, so that a read meets no bank twice.
 //
-// Bound by the matrix instructions and the power they draw: 4096 x 4096 over 16384 bf16 rows takes
-// 460 us, 1195 TFLOP/s, at some 2.0 GHz, the matrix units busy 56% of the cycles (a library product
-// of the same operands in bf16: 552 us).  What it took, in us: 128-square tiles and transposed
-// 2-byte LDS stores 7386; this layout 629; loads without branches, two steps of them in flight and
-// the conversions spread between the matrix instructions 485; eight waves of 64 x 128 instead of four
-// of 128 x 128 472; no bank conflicts, and five stages with a barrier every second step 460.
-// fp32, 4096 cubed: 349 us, 394 TFLOP/s (1180 of bf16), on two stages.  512 x 128 over 50176 fp32 rows,
-// the reading of 110 MB: 38 us, 32 in the product (3.4 TB/s) and 6 in the join of 63 partial sums.
+// Bound by the matrix instructions and the power they draw: 4096 x 4096 over 16384 bf16 rows takes 460
+// to 471 us from card to card, 1168 to 1195 TFLOP/s, at some 2.0 GHz, the matrix units busy 56% of the
+// cycles (a library product of the same operands in bf16: 552 us).  What it took, in us: 128-square
+// tiles and transposed 2-byte LDS stores 7386; this layout 629; loads without branches, two steps of
+// them in flight and the conversions spread between the matrix instructions 485; eight waves of
+// 64 x 128 instead of four of 128 x 128 472; no bank conflicts, and five stages with a barrier every
+// second step 460.  fp32, 4096 cubed: 349 to 360 us, 381 to 394 TFLOP/s (three times that of bf16),
+// on two stages.  512 x 128 over 50176 fp32 rows, the reading of 110 MB: 39 us, 32 in the product
+// (3.4 TB/s) and 6 in the join of 63 partial sums.  The smaller tiles do less: 2048 cubed in bf16 33 to
+// 37 us, 470 to 520 TFLOP/s.
 #include "train_device.h"
 
 namespace miq {
@@ -408,7 +410,7 @@ struct Shape {
 // 5 us to launch, fill and drain; dw and partial sums are written and read at 5.9 TB/s; the launch
 // that joins them costs 5 us more.  Fitted to every pair's time on 46 problems from 128 x 1024 x 1024
 // to 65536 x 1024 x 1024 (rows, c, k) in both types: the pair chosen is the fastest or within 5% of
-// it on 42 of them, within 18% on all.
+// it on 44 of them, within 18% on all.
 Shape shape_of(int32_t rows, int32_t c, int32_t k, bool dy_bf16) {
   struct Rate {
     int tile;
