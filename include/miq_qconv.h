@@ -528,6 +528,85 @@ int miq_act8_grad(const void* dy, const int8_t* codes, const uint8_t* scales, vo
                   int32_t k, int64_t ld_dy, int64_t ld_dw, int32_t accumulate, int32_t dy_type, int32_t dw_type,
                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- layers of token networks on 8-bit rows -------------------------------------------- */
+/* No reference counterpart: the norm with the residual's addition, activations as 8-bit rows, and
+ * int8 products with a scale for each row and each output channel, one or many (a layer of
+ * experts).  The conventions of the section above hold here too.
+ *
+ * An 8-bit row of c values: int8 codes and one fp32 scale; a value stands for code * scale.  With
+ * m the row's largest magnitude, held to 2^-110 from below, scale = m / 127 and the codes are
+ * v * (127 / m) rounded to nearest even, |code| <= 127.  A row that holds an infinity or a NaN has
+ * codes 0 and a NaN scale, and stands for NaN.  Codes are dense: row r starts at codes + r * c. */
+
+/* y = s * gain / sqrt(mean(s^2) + eps) by rows of c.  s = x, or with `add` (not NULL) x + add, rounded
+ * to `type` and written to `sum`, which comes with add and may be x or add itself (with its row
+ * distance).  x, add, sum, y: rows x c of `type`; gain: c of gain_type.  Sums of squares are fp32, and
+ * summed again over scaled values where they overflow.  eps in 1e-30 .. 1e30. */
+int miq_rms_fprop(const void* x, const void* add, const void* gain, void* sum, void* y, int64_t rows, int32_t c,
+                  int64_t ld_x, int64_t ld_add, int64_t ld_sum, int64_t ld_y, float eps, int32_t type,
+                  int32_t gain_type, void* stream);
+
+/* miq_rms_fprop with y as 8-bit rows.  |s * gain| has to be finite in fp32, else the row stands for NaN. */
+int miq_rms_row8(const void* x, const void* add, const void* gain, void* sum, int8_t* codes, float* scales, int64_t rows,
+                 int32_t c, int64_t ld_x, int64_t ld_add, int64_t ld_sum, float eps, int32_t type, int32_t gain_type,
+                 void* stream);
+
+/* Bytes of device workspace miq_rms_bprop needs (no GPU access). */
+int miq_rms_bprop_workspace_size(int64_t rows, int32_t c, size_t* bytes);
+
+/* The backward pass of miq_rms_fprop at x (the sum, where it had an addend): with n = x / sqrt(mean(x^2) +
+ * eps) and dn = dy * gain, dx = (dn - n * mean(dn * n)) / sqrt(mean(x^2) + eps), plus dsum (or NULL), the
+ * gradient that reaches the sum by another way; and dgain = the sum over the rows of dy * n, added to
+ * dgain where accumulate != 0.  The gradient of x and of add are both dx.  dy, x, dsum, dx: rows x c
+ * of `type`; dgain: c of dgain_type.  rows == 0 gives a dgain of zeros. */
+int miq_rms_bprop(const void* dy, const void* x, const void* gain, const void* dsum, void* dx, void* dgain, int64_t rows,
+                  int32_t c, int64_t ld_dy, int64_t ld_x, int64_t ld_dsum, int64_t ld_dx, float eps, int32_t accumulate,
+                  int32_t type, int32_t gain_type, int32_t dgain_type, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* act(x) by rows of c, or act(gate) * up for gated rows [gate, up] of 2c, as 8-bit rows.  MIQ_ACT_NONE
+ * makes 8-bit rows of x itself: of a layer's weights, k rows of c. */
+int miq_act_row8(const void* x, int8_t* codes, float* scales, int64_t rows, int32_t c, int64_t ld_x, int32_t act,
+                 int32_t gated, int32_t type, void* stream);
+
+/* What 8-bit rows stand for: y = code * scale, rows x c of `type`. */
+int miq_row8_expand(const int8_t* codes, const float* scales, void* y, int64_t rows, int32_t c, int64_t ld_y,
+                    int32_t type, void* stream);
+
+/* Bytes of device workspace miq_row8_linear needs (no GPU access). */
+int miq_row8_linear_workspace_size(int64_t rows, int32_t c, int32_t k, size_t* bytes);
+
+/* y[m, j] = (sum over i < c of codes[m, i] * w_codes[j, i]) * scales[m] * w_scales[j] + bias[j] + add[m, j]:
+ * a linear layer on 8-bit rows and 8-bit weights, k rows of c.  The sum of products is exact; it
+ * is rounded to fp32, as is each of the operations after it in this order, and the result to
+ * `type`.  bias: k fp32, or NULL; add: rows x k of `type`, or NULL, may be y itself (with its row
+ * distance).  rows up to 2^31 - 65, c up to 131071, k up to 2^22. */
+int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
+                    const float* bias, const void* add, void* y, int64_t rows, int32_t c, int32_t k, int64_t ld_add,
+                    int64_t ld_y, int32_t type, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The products of a layer of experts: rows offsets[e] .. offsets[e + 1] - 1 of y by the weights of expert e
+ * (w_codes: experts x k x c, w_scales and bias: experts x k).  Row i of y takes row index[i] of the
+ * x_rows 8-bit rows, or row i where index is NULL; an index outside 0 .. x_rows - 1 stands for a row
+ * of zeros.  offsets (experts + 1, on the device, rising, at most `rows`) may leave experts without
+ * a row; rows of y outside them are left as they were.  experts up to 4096. */
+int miq_row8_experts(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
+                     const float* bias, const int32_t* offsets, const int32_t* index, void* y, int64_t x_rows,
+                     int64_t rows, int32_t c, int32_t k, int32_t experts, int64_t ld_y, int32_t type, void* stream);
+
+/* The (token, slot) pairs of ids (tokens x slots) sorted by expert, in their order within an expert:
+ * offsets[e] (experts + 1) is where expert e's pairs start, rows[i] (tokens * slots) the token of sorted
+ * pair i, -1 behind the last, and places[t, s] where a pair went, -1 for an id outside 0 .. experts - 1. */
+int miq_experts_plan(const void* ids, int32_t* offsets, int32_t* rows, int32_t* places, int64_t tokens, int32_t slots,
+                     int32_t experts, int32_t id_type, void* stream);
+
+/* out[t] = add[t] + sum over s of share[t, s] * y[places[t, s]], in fp32 and in the order of s; places
+ * outside 0 .. rows - 1 add nothing.  y: rows x c, add (or NULL) and out: tokens x c, of `type`; add may
+ * be out itself (with its row distance); share: fp32, or NULL for ones. */
+int miq_experts_join(const void* y, const int32_t* places, const float* share, const void* add, void* out, int64_t rows,
+                     int64_t tokens, int32_t slots, int32_t c, int64_t ld_y, int64_t ld_add, int64_t ld_out, int32_t type,
+                     void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

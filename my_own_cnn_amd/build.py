@@ -48,6 +48,12 @@ SOURCES = [
     "embed_grad.hip",
     "act8.hip",
     "act8_grad.hip",
+    "row8_capi.cpp",
+    "rms.hip",
+    "rms_grad.hip",
+    "row8.hip",
+    "row8_linear.hip",
+    "experts.hip",
     "conv_quant_host.cpp",
     "verify.cpp",
     "bench.cpp",

@@ -25,30 +25,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-enum Act : int { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
-
-// act(v).  NaN stays NaN.
-template <int ACT>
-__device__ __forceinline__ float act_of(float v) {
-  if constexpr (ACT == kRelu) return v < 0.0f ? 0.0f : v;
-  if constexpr (ACT == kSilu) return v / (1.0f + expf(-v));
-  if constexpr (ACT == kGelu) return 0.5f * v * erfcf(v * -0.70710678118654752f);
-  return v;
-}
-
-// act'(v); 0 at relu's corner.
-template <int ACT>
-__device__ __forceinline__ float slope_of(float v) {
-  if constexpr (ACT == kRelu) return v > 0.0f ? 1.0f : (v <= 0.0f ? 0.0f : v);
-  if constexpr (ACT == kSilu) {
-    const float s = 1.0f / (1.0f + expf(-v));
-    return s * (1.0f + v * (1.0f - s));
-  }
-  if constexpr (ACT == kGelu)
-    return 0.5f * erfcf(v * -0.70710678118654752f) + v * expf(-0.5f * v * v) * 0.39894228040143268f;
-  return 1.0f;
-}
-
 struct Rows {
   int64_t total;     // chunks of a lane's channels, rows padded to whole groups
   int64_t ld_x, ld_dy, ld_y;
@@ -56,34 +32,6 @@ struct Rows {
   FastDivM div;            // by per_row
 };
 
-// A lane's channels: 16 bytes of the tensor's type.
-template <typename T>
-constexpr int kWide = 16 / static_cast<int>(sizeof(T));
-
-template <int W>
-struct Vec;
-template <>
-struct Vec<8> {
-  typedef v8f type;
-};
-template <>
-struct Vec<4> {
-  typedef v4f type;
-};
-
-// Past the caches too where the output is (STREAM): what is read once leaves no room for what is not.
-template <bool STREAM>
-__device__ __forceinline__ v8f load_run(const __bf16* p) {
-  const v8bf_any* const q = reinterpret_cast<const v8bf_any*>(p);
-  if constexpr (STREAM) return __builtin_convertvector(__builtin_nontemporal_load(q), v8f);
-  else return __builtin_convertvector(*q, v8f);
-}
-template <bool STREAM>
-__device__ __forceinline__ v4f load_run(const float* p) {
-  const v4f_any* const q = reinterpret_cast<const v4f_any*>(p);
-  if constexpr (STREAM) return __builtin_nontemporal_load(q);
-  else return *q;
-}
 template <bool STREAM>
 __device__ __forceinline__ void load_codes(const int8_t* p, int (&q)[2]) {
   const v2i_any* const from = reinterpret_cast<const v2i_any*>(p);
@@ -98,27 +46,6 @@ __device__ __forceinline__ void load_codes(const int8_t* p, int (&q)[1]) {
   const int_any* const from = reinterpret_cast<const int_any*>(p);
   if constexpr (STREAM) q[0] = __builtin_nontemporal_load(from);
   else q[0] = *from;
-}
-
-// The first `left` of a lane's channels; the rest read zero and are not stored.
-template <bool STREAM, typename T>
-__device__ __forceinline__ typename Vec<kWide<T>>::type load_some(const T* p, int left) {
-  if (left >= kWide<T>) return load_run<STREAM>(p);
-  typename Vec<kWide<T>>::type v = {};
-#pragma unroll
-  for (int i = 0; i < kWide<T>; ++i)
-    if (i < left) v[i] = static_cast<float>(p[i]);
-  return v;
-}
-template <bool STREAM, typename T>
-__device__ __forceinline__ void store_some(T* p, const typename Vec<kWide<T>>::type& v, int left) {
-  if (left >= kWide<T>) {
-    store_run<STREAM>(p, v);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < kWide<T>; ++i)
-    if (i < left) p[i] = static_cast<T>(v[i]);
 }
 
 // (row, channel, channels left) of this thread's chunk of W; false past the end

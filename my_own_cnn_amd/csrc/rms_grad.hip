@@ -1,0 +1,223 @@
+// The backward pass of the root-mean-square norm (miq_rms_bprop).
+//
+//   n = s * r, r = 1 / sqrt(mean s^2 + eps), dn = dy * gain
+//   ds = r * (dn - n * mean(dn * n)) + dsum,   dgain = sum over the rows of dy * n
+//
+// One read of s, dy and dsum and one write of ds: a row stays in the registers of a wave or a
+// workgroup, both sums of a row (s^2 and dn * s) meet once, and dgain's terms are added in registers over
+// the rows that a workgroup takes.  The workgroups' sums go to the workspace and are added by a second
+// launch, both in an order fixed by the sizes.
+#include <algorithm>
+
+#include "row8_device.h"
+
+namespace miq {
+namespace {
+
+constexpr int kParts = 1024;  // workgroups, and rows of the workspace, at most
+
+template <int W, typename G>
+__device__ __forceinline__ typename Vec<W>::type load_gain(const G* p, int left) {
+  typename Vec<W>::type v = {};
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    if (i < left) v[i] = static_cast<float>(p[i]);
+  return v;
+}
+
+template <typename T, typename G, int THREADS, int V>
+__global__ __launch_bounds__(kRowBlock<THREADS>) void rms_grad_kernel(RmsGradArgs a) {
+  constexpr int W = kWide<T>;
+  constexpr int kThreads = kRowBlock<THREADS>, kRows = kThreads / THREADS;
+  typedef typename Vec<W>::type Run;
+  __shared__ RowSums<THREADS> lds;
+  __shared__ float sums[kRows > 1 ? kRows * THREADS * V * W : 1];
+  const int t = static_cast<int>(threadIdx.x) % THREADS;
+  const int own = static_cast<int>(threadIdx.x) / THREADS;
+  Run g[V], total[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int col = (j * THREADS + t) * W;
+    g[j] = load_gain<W>(static_cast<const G*>(a.gain) + col, a.c - col);
+    total[j] = Run{};
+  }
+  int turn = 0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own; row < a.rows;
+       row += static_cast<int64_t>(gridDim.x) * kRows) {
+    Run s[V], d[V];
+    float squares = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int col = (j * THREADS + t) * W;
+      s[j] = load_some<false>(static_cast<const T*>(a.x) + row * a.ld_x + col, a.c - col);
+      d[j] = load_some<false>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.c - col);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        squares += s[j][i] * s[j][i];
+        dot += d[j][i] * g[j][i] * s[j][i];
+      }
+    reduce_row<THREADS>(lds, turn, &squares, &dot, nullptr);
+    turn ^= 1;
+    float eps = a.eps, down = 1.0f;
+    if (overflowed(squares)) {  // the same for all of the row's threads
+      squares = dot = 0.0f;
+      down = kDown;
+      eps = eps * kDown * kDown;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s[j] *= kDown;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          squares += s[j][i] * s[j][i];
+          dot += d[j][i] * g[j][i] * s[j][i];
+        }
+      }
+      reduce_row<THREADS>(lds, turn, &squares, &dot, nullptr);
+      turn ^= 1;
+    }
+    const float r = inverse_rms(squares, a.c, eps);
+    const float along = dot * r / static_cast<float>(a.c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int col = (j * THREADS + t) * W;
+      const Run n = s[j] * r;
+      total[j] += d[j] * n;
+      Run dx = (d[j] * g[j] - n * along) * (r * down);
+      if (a.dsum != nullptr) dx += load_some<false>(static_cast<const T*>(a.dsum) + row * a.ld_dsum + col, a.c - col);
+      store_some<false>(static_cast<T*>(a.dx) + row * a.ld_dx + col, dx, a.c - col);
+    }
+  }
+  // The workgroup's row of the workspace.
+  float* const out = a.ws + static_cast<int64_t>(blockIdx.x) * a.c;
+  if constexpr (kRows > 1) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) sums[own * (THREADS * V * W) + (j * THREADS + t) * W + i] = total[j][i];
+    __syncthreads();
+    for (int col = threadIdx.x; col < a.c; col += kThreads) {
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) s += sums[k * (THREADS * V * W) + col];
+      out[col] = s;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int col = (j * THREADS + t) * W;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i < a.c - col) out[col + i] = total[j][i];
+    }
+  }
+}
+
+// Rows longer than the registers of a workgroup: read again for ds and dgain; dgain's terms are added
+// in the workgroup's row of the workspace, each by the thread that reads it next.
+template <typename T, typename G>
+__global__ __launch_bounds__(1024) void rms_grad_long_kernel(RmsGradArgs a) {
+  constexpr int W = kWide<T>, kThreads = 1024;
+  typedef typename Vec<W>::type Run;
+  __shared__ RowSums<kThreads> lds;
+  float* const out = a.ws + static_cast<int64_t>(blockIdx.x) * a.c;
+  int turn = 0;
+  bool first = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* const x = static_cast<const T*>(a.x) + row * a.ld_x;
+    const T* const dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
+    const G* const gain = static_cast<const G*>(a.gain);
+    float squares = 0.0f, dot = 0.0f, down = 1.0f, eps = a.eps;
+    for (int again = 0; again < 2; ++again) {
+      squares = dot = 0.0f;
+      for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.c; at += kThreads * W) {
+        const int left = static_cast<int>(a.c - at);
+        const Run s = load_some<false>(x + at, left) * down, d = load_some<false>(dy + at, left);
+        const Run g = load_gain<W>(gain + at, left);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          squares += s[i] * s[i];
+          dot += d[i] * g[i] * s[i];
+        }
+      }
+      reduce_row<kThreads>(lds, turn, &squares, &dot, nullptr);
+      turn ^= 1;
+      if (!overflowed(squares) || again) break;
+      down = kDown;
+      eps = a.eps * kDown * kDown;
+    }
+    const float r = inverse_rms(squares, a.c, eps);
+    const float along = dot * r / static_cast<float>(a.c);
+    for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.c; at += kThreads * W) {
+      const int left = static_cast<int>(a.c - at);
+      const Run n = load_some<false>(x + at, left) * down * r, d = load_some<false>(dy + at, left);
+      const Run g = load_gain<W>(gain + at, left);
+      Run dx = (d * g - n * along) * (r * down);
+      if (a.dsum != nullptr) dx += load_some<false>(static_cast<const T*>(a.dsum) + row * a.ld_dsum + at, left);
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i < left) out[at + i] = (first ? 0.0f : out[at + i]) + d[i] * n[i];
+      store_some<false>(static_cast<T*>(a.dx) + row * a.ld_dx + at, dx, left);
+    }
+    first = false;
+  }
+}
+
+// dgain[col] = the sum of the workspace's rows, 32 columns a workgroup, 32 threads a column.
+template <typename D>
+__global__ __launch_bounds__(1024) void rms_grad_join_kernel(const float* __restrict__ ws, D* __restrict__ dgain, int c,
+                                                             int parts, bool accumulate) {
+  __shared__ float lds[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  for (int base = blockIdx.x * 32; base < c; base += gridDim.x * 32) {
+    float s = 0.0f;
+    if (base + x < c)
+      for (int p = y; p < parts; p += 32) s += ws[static_cast<int64_t>(p) * c + base + x];
+    lds[y][x] = s;
+    __syncthreads();
+    if (y == 0 && base + x < c) {
+      float total = accumulate ? static_cast<float>(dgain[base + x]) : 0.0f;
+      for (int i = 0; i < 32; ++i) total += lds[i][x];
+      dgain[base + x] = static_cast<D>(total);
+    }
+    __syncthreads();
+  }
+}
+
+// A workgroup for at least four rows (sixteen, a wave a row), so that the workspace stays small beside
+// the rows.
+int64_t parts_of(int64_t rows) { return std::min<int64_t>(kParts, (rows + 3) / 4); }
+
+template <typename T, typename G>
+void launch(const RmsGradArgs& a, int64_t parts, hipStream_t stream) {
+  by_shape(row_shape(a.c, kWide<T>, a.rows), [&](auto threads, auto runs) {
+    constexpr int THREADS = threads.value, V = runs.value;
+    if constexpr (V == 0) {
+      rms_grad_long_kernel<T, G><<<static_cast<unsigned>(parts), 1024, 0, stream>>>(a);
+    } else {
+      rms_grad_kernel<T, G, THREADS, V><<<static_cast<unsigned>(parts), kRowBlock<THREADS>, 0, stream>>>(a);
+    }
+  });
+}
+
+}  // namespace
+
+size_t rms_grad_workspace_bytes(int64_t rows, int32_t c) { return static_cast<size_t>(parts_of(rows)) * c * sizeof(float); }
+
+hipError_t launch_rms_grad(const RmsGradArgs& a, hipStream_t stream) {
+  const int64_t parts = parts_of(a.rows);
+  if (parts > 0) {
+    if (a.bf16) a.gain_bf16 ? launch<__bf16, __bf16>(a, parts, stream) : launch<__bf16, float>(a, parts, stream);
+    else a.gain_bf16 ? launch<float, __bf16>(a, parts, stream) : launch<float, float>(a, parts, stream);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(a.c) + 31) / 32, 1 << 20));
+  const int n = static_cast<int>(parts);
+  if (a.dgain_bf16) rms_grad_join_kernel<<<grid, 1024, 0, stream>>>(a.ws, static_cast<__bf16*>(a.dgain), a.c, n, a.accumulate);
+  else rms_grad_join_kernel<<<grid, 1024, 0, stream>>>(a.ws, static_cast<float*>(a.dgain), a.c, n, a.accumulate);
+  return hipGetLastError();
+}
+
+}  // namespace miq
