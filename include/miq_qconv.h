@@ -573,9 +573,6 @@ int miq_act_row8(const void* x, int8_t* codes, float* scales, int64_t rows, int3
 int miq_row8_expand(const int8_t* codes, const float* scales, void* y, int64_t rows, int32_t c, int64_t ld_y,
                     int32_t type, void* stream);
 
-/* Bytes of device workspace miq_row8_linear needs (no GPU access). */
-int miq_row8_linear_workspace_size(int64_t rows, int32_t c, int32_t k, size_t* bytes);
-
 /* y[m, j] = (sum over i < c of codes[m, i] * w_codes[j, i]) * scales[m] * w_scales[j] + bias[j] + add[m, j]:
  * a linear layer on 8-bit rows and 8-bit weights, k rows of c.  The sum of products is exact; it
  * is rounded to fp32, as is each of the operations after it in this order, and the result to
@@ -583,7 +580,12 @@ int miq_row8_linear_workspace_size(int64_t rows, int32_t c, int32_t k, size_t* b
  * distance).  rows up to 2^31 - 65, c up to 131071, k up to 2^22. */
 int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
                     const float* bias, const void* add, void* y, int64_t rows, int32_t c, int32_t k, int64_t ld_add,
-                    int64_t ld_y, int32_t type, void* workspace, size_t workspace_bytes, void* stream);
+                    int64_t ld_y, int32_t type, void* stream);
+
+/* How miq_row8_linear (experts 1) and miq_row8_experts run a problem: plan[0] is 1 where the weights go straight
+ * to the matrix instructions (few rows) and 0 where tiles of both operands go through LDS, plan[1] and
+ * plan[2] are a tile's rows and channels; zeros where there is nothing to do.  No GPU access. */
+int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]);
 
 /* The products of a layer of experts: rows offsets[e] .. offsets[e + 1] - 1 of y by the weights of expert e
  * (w_codes: experts x k x c, w_scales and bias: experts x k).  Row i of y takes row index[i] of the

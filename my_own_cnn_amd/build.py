@@ -52,7 +52,9 @@ SOURCES = [
     "rms.hip",
     "rms_grad.hip",
     "row8.hip",
-    "row8_linear.hip",
+    "row8_linear.cpp",
+    "row8_tile.hip",
+    "row8_few.hip",
     "experts.hip",
     "conv_quant_host.cpp",
     "verify.cpp",

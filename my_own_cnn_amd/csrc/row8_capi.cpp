@@ -219,19 +219,19 @@ int miq_row8_expand(const int8_t* codes, const float* scales, void* y, int64_t r
   return done(miq::launch_row8_expand(a, static_cast<hipStream_t>(stream)));
 }
 
-int miq_row8_linear_workspace_size(int64_t rows, int32_t c, int32_t k, size_t* bytes) {
-  if (bytes == nullptr) return null("bytes pointer is NULL");
-  const int st = check_product(rows, c, k, 1);
+int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]) {
+  if (plan == nullptr) return null("plan pointer is NULL");
+  const int st = check_product(rows, c, k, experts);
   if (st != MIQ_OK) return st;
-  *bytes = rows == 0 || k == 0 ? 0 : miq::row8_linear_workspace_bytes(static_cast<int32_t>(rows), c, k);
+  plan[0] = plan[1] = plan[2] = 0;
+  if (rows > 0 && k > 0) miq::plan_row8_linear(static_cast<int32_t>(rows), c, k, experts, plan);
   return MIQ_OK;
 }
 
 int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
                     const float* bias, const void* add, void* y, int64_t rows, int32_t c, int32_t k, int64_t ld_add,
-                    int64_t ld_y, int32_t type, void* workspace, size_t workspace_bytes, void* stream) {
-  size_t need = 0;
-  const int st = miq_row8_linear_workspace_size(rows, c, k, &need);
+                    int64_t ld_y, int32_t type, void* stream) {
+  const int st = check_product(rows, c, k, 1);
   if (st != MIQ_OK) return st;
   if (!real_type(type)) return bad("type must be MIQ_F32 or MIQ_BF16");
   if (!stride_ok(ld_y, k) || (add != nullptr && !stride_ok(ld_add, k))) return bad(kShortRows);
@@ -240,11 +240,9 @@ int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_co
     return null("codes or scales pointer is NULL");
   }
   if (y == nullptr) return null("output pointer is NULL");
-  if (need > 0 && workspace == nullptr) return null("workspace pointer is NULL");
-  if (workspace_bytes < need) return bad("workspace is smaller than miq_row8_linear_workspace_size reports");
   if (!aligned(scales, 4) || !aligned(w_scales, 4) || !aligned(bias, 4) || !aligned(add, size_of(type)) ||
-      !aligned(y, size_of(type)) || !aligned(workspace, 16)) {
-    return bad("a pointer is not aligned to its element, or the workspace to 16 bytes");
+      !aligned(y, size_of(type))) {
+    return bad(kUnaligned);
   }
   miq::Row8LinearArgs a{};
   a.x = codes;
@@ -254,7 +252,6 @@ int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_co
   a.bias = bias;
   a.add = add;
   a.y = y;
-  a.ws = workspace;
   a.ld_add = ld_add;
   a.ld_y = ld_y;
   a.x_rows = a.rows = static_cast<int32_t>(rows);

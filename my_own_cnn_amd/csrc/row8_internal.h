@@ -1,5 +1,5 @@
 // Internal interface between row8_capi.cpp and the kernels of 8-bit rows (rms.hip, rms_grad.hip,
-// row8.hip, row8_linear.hip, experts.hip).
+// row8.hip, row8_linear.cpp, row8_few.hip, row8_tile.hip, experts.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -73,13 +73,14 @@ struct Row8LinearArgs {
   const int32_t* offsets;
   const int32_t* index;
   void* y;
-  void* ws;
   int64_t ld_add, ld_y;
   int32_t x_rows, rows, c, k, experts;
   bool bf16;
 };
-size_t row8_linear_workspace_bytes(int32_t rows, int32_t c, int32_t k);
-void plan_row8_linear(int32_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[4]);
+hipError_t launch_row8_few(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream);
+hipError_t launch_row8_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream);
+// plan: whether the weights go straight to the matrix instructions (few rows), and a tile's rows and channels.
+void plan_row8_linear(int32_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]);
 hipError_t launch_row8_linear(const Row8LinearArgs& a, hipStream_t stream);
 
 struct ExpertsPlanArgs {

@@ -1,0 +1,322 @@
+// Products of 8-bit rows with 8-bit weights in tiles held by LDS (row8_linear.cpp has the formula).
+//
+// A workgroup computes BM rows by BN channels of y, 64 codes of the reduction a step.  Both operands lie
+// in LDS as rows of 64 bytes, STAGES steps of them; a step's bytes travel straight from global memory to
+// LDS (DMA; through registers where rows do not start on 16 bytes), two or more steps ahead.  A wave
+// reads the fragments of the next step while its matrix instructions run on this one's, so one barrier a
+// step is all that a wave waits for.
+#include <algorithm>
+
+#include "row8_product.h"
+
+namespace miq {
+namespace {
+
+constexpr int kStep = 64;  // codes, and bytes of a row of LDS
+
+struct Tiling {
+  int from, high, wide;  // the launch's first row tile and their number (the most, of experts), channel tiles
+};
+
+// The 16-byte units of a row of LDS are permuted by its number: an LDS read serves in one cycle the lanes
+// 0-3, 12-15, 20-23, 24-27 of a half-wave or the other 16, that is rows 0-3 and 12-15 at one unit and 4-11
+// at the next one, or the other way round, and these lie in different banks.
+__device__ __forceinline__ int unit(int row, int at) {
+  const int g = (row >> 2) & 3;
+  return at ^ (((g ^ (g >> 1)) & 1) << 1 | g >> 1);
+}
+
+// The channel in row p of LDS.  Matrix instruction f of a group of 64 rows of LDS leaves its rows 4q .. 4q + 3
+// in lane group q: for 16-byte stores whose four lanes lie side by side a lane's channels are 8q .. 8q + 7 of
+// 32 (bf16, of two instructions), or 4q .. 4q + 3 of 16.
+template <typename T>
+__device__ __forceinline__ int channel_of(int p) {
+  if constexpr (sizeof(T) == 4) return p;
+  return (p & ~31) + ((p >> 2) & 3) * 8 + ((p >> 4) & 1) * 4 + (p & 3);
+}
+
+template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) void row8_tile_kernel(Row8LinearArgs a, Tiling tiling) {
+  constexpr int kWaves = WM * WN;
+  constexpr int NX = BM / 16 / kWaves, NW = BN / 16 / kWaves;  // runs of 16 rows that a wave stages
+  constexpr int kStage = (BM + BN) * kStep;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;  // a wave's fragments
+  static_assert(NX >= 1 && NW >= 1 && FN % 2 == 0, "whole runs and groups of 32 channels");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // Tiles in bands of eight rows of tiles: neighbours share their rows and channels in an L2.
+  constexpr int kBand = 8;
+  const int at = xcd_tile(blockIdx.x, gridDim.x);
+  const int band = at / (kBand * tiling.wide);
+  const int band_high = min(kBand, tiling.high - band * kBand);
+  const int in = at - band * kBand * tiling.wide;
+  const int row_tile = tiling.from + band * kBand + in % band_high, n0 = in / band_high * BN;
+  RowTile r = {0, row_tile * BM, a.rows - row_tile * BM < BM ? a.rows : (row_tile + 1) * BM};
+  if (a.offsets != nullptr) {
+    r = find_tile(a.offsets, a.experts, a.rows, BM, row_tile);
+    if (r.expert < 0) return;
+  }
+  const int rows = r.end - r.row0, channels = min(BN, a.k - n0);
+  const int64_t w_at = (static_cast<int64_t>(r.expert) * a.k + n0) * a.c;
+
+  // The output stage takes U runs of a lane's channels of each row, W values each.  Its scales are loaded first,
+  // where registers are left for them.
+  constexpr int W = kWide<T>, U = FN * 4 / W;
+  constexpr bool kEarly = FM * FN < 32;
+  const int wm = wave / WN, wn = wave % WN;
+  const int f_row = lane & 15, f_at = lane >> 4;
+  const int64_t w_of0 = static_cast<int64_t>(r.expert) * a.k;
+  const int k0 = n0 + wn * FN * 16 + f_at * W;  // of run u: k0 + u * 4 * W
+  float x_scale[FM];
+  typename Vec<W>::type w_scale[U];
+  auto load_scales = [&]() {
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int row = (wm * FM + j) * 16 + f_row;
+      int from = row < rows ? r.row0 + row : -1;
+      if (a.index != nullptr && from >= 0) from = a.index[from];
+      x_scale[j] = from >= 0 && from < a.x_rows ? a.x_scales[from] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) w_scale[u] = load_floats<W>(a.w_scales + w_of0 + k0 + u * 4 * W, a.k - (k0 + u * 4 * W));
+  };
+  if constexpr (kEarly) load_scales();
+
+  // A wave's runs: lane l stages unit l & 3 of row l >> 2 of each.  Rows and channels beyond the tile's read
+  // another's or zeros: they reach no sum that is stored.
+  const int s_row = lane >> 2;
+  int x_row[NX], w_row[NW];
+#pragma unroll
+  for (int i = 0; i < NX; ++i) {
+    const int row = (wave * NX + i) * 16 + s_row;
+    x_row[i] = row < rows ? row : 0;
+    if (a.index != nullptr) {
+      const int from = a.index[r.row0 + x_row[i]];
+      x_row[i] = from >= 0 && from < a.x_rows ? from : 0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NW; ++i) w_row[i] = min(channel_of<T>((wave * NW + i) * 16 + s_row), channels - 1);
+  const int8_t* const x_base = a.index != nullptr ? a.x : a.x + static_cast<int64_t>(r.row0) * a.c;
+  const int8_t* const w_base = a.w + w_at;
+  const int steps = (a.c + kStep - 1) / kStep;
+
+  // DMA: offsets of a wave's runs; past the tensor's end they read zeros.
+  unsigned x_of[NX], w_of[NW];
+  __amdgpu_buffer_rsrc_t x_rsrc, w_rsrc;
+  // registers: where a wave's runs start, and two steps of them on their way
+  const int8_t* x_from[NX];
+  const int8_t* w_from[NW];
+  v4i x_set[2][NX], w_set[2][NW];
+  const int s_at = unit(s_row, lane & 3) * 16;
+  if constexpr (DMA) {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) x_of[i] = static_cast<unsigned>(x_row[i]) * static_cast<unsigned>(a.c) + s_at;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) w_of[i] = static_cast<unsigned>(w_row[i]) * static_cast<unsigned>(a.c) + s_at;
+    x_rsrc = make_rsrc(x_base, static_cast<int>(static_cast<unsigned>(a.index != nullptr ? a.x_rows : rows) *
+                                                static_cast<unsigned>(a.c)));
+    w_rsrc = make_rsrc(w_base, channels * a.c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) x_from[i] = x_base + static_cast<int64_t>(x_row[i]) * a.c;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) w_from[i] = w_base + static_cast<int64_t>(w_row[i]) * a.c;
+  }
+  auto stage = [&](int step, int buffer) {
+    const unsigned k = static_cast<unsigned>(min(step, steps - 1)) * kStep;
+    char* const to = lds + buffer * kStage;
+#pragma unroll
+    for (int i = 0; i < NX; ++i)
+      load_lds16(x_rsrc, reinterpret_cast<v4i*>(to + (wave * NX + i) * 1024), x_of[i], k);
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+      load_lds16(w_rsrc, reinterpret_cast<v4i*>(to + BM * kStep + (wave * NW + i) * 1024), w_of[i], k);
+  };
+  auto load = [&](int step, int set) {
+    const int k = min(step, steps - 1) * kStep + s_at;
+    if (step < steps - 1) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) x_set[set][i] = load16<false>(x_from[i] + k);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) w_set[set][i] = load16<false>(w_from[i] + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) x_set[set][i] = load_codes16(x_from[i], k, a.c);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) w_set[set][i] = load_codes16(w_from[i], k, a.c);
+    }
+  };
+  auto write = [&](int set, int buffer) {
+    char* const to = lds + buffer * kStage + lane * 16;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) *reinterpret_cast<v4i*>(to + (wave * NX + i) * 1024) = x_set[set][i];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) *reinterpret_cast<v4i*>(to + BM * kStep + (wave * NW + i) * 1024) = w_set[set][i];
+  };
+
+  typedef __attribute__((address_space(3))) const char lds_char;
+  typedef __attribute__((address_space(3))) const v4i lds_v4i;
+  lds_char* const f_from = (lds_char*)lds + f_row * kStep + unit(f_row, f_at) * 16;  // an address-space cast
+  lds_char* const x_part = f_from + wm * FM * 1024;
+  lds_char* const w_part = f_from + BM * kStep + wn * FN * 1024;
+  v4i fx[2][FM], fw[2][FN];
+  auto read = [&](int buffer, int set) {
+    lds_char* const x = x_part + buffer * kStage;
+    lds_char* const w = w_part + buffer * kStage;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) fw[set][i] = *reinterpret_cast<lds_v4i*>(w + i * 1024);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fx[set][i] = *reinterpret_cast<lds_v4i*>(x + i * 1024);
+  };
+  v4i acc[FN][FM] = {};
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[set][i], fx[set][j], acc[i][j], 0, 0, 0);
+  };
+
+  // Step t multiplies the fragments read in step t - 1 and reads those of t + 1.  Past the last step the
+  // loads and reads repeat it.
+  // DMA: it starts the loads of t + STAGES - 1 into the buffer of t - 1, which every wave has read before the
+  // step's barrier; before the barrier a wave waits for its own loads of t + 1, and the STAGES - 3 steps
+  // after that stay in flight.
+  // Registers: at its end it writes t + 2, in place of t - 2, and loads t + 4.
+  constexpr int kLoads = NX + NW;
+  static_assert(STAGES == 4 && (STAGES - 2) * kLoads <= 15, "the buffers' numbers, and the counter's bits in use");
+  int now = 0;  // buffer of step t
+  if constexpr (DMA) {
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) stage(i, i);
+    wait_vmcnt((STAGES - 2) * kLoads);
+    barrier_only();
+  } else {
+    load(0, 0);
+    load(1, 1);
+    write(0, 0);
+    write(1, 1);
+    load(2, 0);
+    load(3, 1);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    barrier_only();
+  }
+  read(0, 0);
+  auto step = [&](int t, int set) {
+    if constexpr (DMA) wait_vmcnt((STAGES - 3) * kLoads);
+    else __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): its writes of t + 1
+    barrier_only();
+    if constexpr (DMA) stage(t + STAGES - 1, now == 0 ? STAGES - 1 : now - 1);
+    now = now + 1 == STAGES ? 0 : now + 1;
+    read(now, set ^ 1);
+    multiply(set);
+    // a read or a load after each matrix instruction
+#pragma unroll
+    for (int i = 0; i < FN * FM; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // matrix
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);            // LDS reads
+      if constexpr (DMA) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // loads
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!DMA) {
+      write(set, now + 1 == STAGES ? 0 : now + 1);
+      load(t + 4, set);
+    }
+  };
+  int t = 0;
+  for (; t + 2 < steps; t += 2) {
+    step(t, 0);
+    step(t + 1, 1);
+  }
+  if (t + 1 < steps) {
+    step(t, 0);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) fx[0][j] = fx[1][j];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) fw[0][i] = fw[1][i];
+  }
+  // the last step: codes past the rows' end do not count
+  const bool there = (steps - 1) * kStep + f_at * 16 < a.c;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) fx[0][j] = there ? fx[0][j] : v4i{};
+  multiply(0);
+  wait_vmcnt(0);  // no load into LDS outlives the workgroup
+
+  if constexpr (!kEarly) load_scales();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = k0 + u * 4 * W, left = a.k - k;
+    if (left <= 0) continue;
+    typename Vec<W>::type bias = {};
+    if (a.bias != nullptr) bias = load_floats<W>(a.bias + w_of0 + k, left);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int row = (wm * FM + j) * 16 + f_row;
+      if (row >= rows) continue;
+      typename Vec<W>::type v;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[i] = scaled(acc[(u * W + i) / 4][j][i % 4], x_scale[j], w_scale[u][i]);
+      if (a.bias != nullptr) v += bias;
+      const int64_t y_row = r.row0 + row;
+      if (a.add != nullptr) v += load_some<false>(static_cast<const T*>(a.add) + y_row * a.ld_add + k, left);
+      store_some<false>(static_cast<T*>(a.y) + y_row * a.ld_y + k, v, left);
+    }
+  }
+}
+
+template <typename T, bool DMA, int BM, int BN, int WM, int WN>
+hipError_t launch(const Row8LinearArgs& a, hipStream_t stream) {
+  constexpr int kStages = 4, kSize = kStages * (BM + BN) * kStep;
+  const int wide = (a.k + BN - 1) / BN;
+  const int64_t high = a.offsets != nullptr ? most_tiles(a.rows, a.experts, BM)
+                                            : (static_cast<int64_t>(a.rows) + BM - 1) / BM;
+  auto* const kernel = row8_tile_kernel<T, DMA, BM, BN, WM, WN, kStages>;
+  if (kSize > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kSize);
+    if (e != hipSuccess) return e;
+  }
+  // at most 2^22 tiles a launch, whole row tiles each
+  const int64_t most = std::max<int64_t>((int64_t{1} << 22) / wide, 1);
+  for (int64_t from = 0; from < high; from += most) {
+    const Tiling t{static_cast<int>(from), static_cast<int>(std::min(most, high - from)), wide};
+    kernel<<<static_cast<unsigned>(static_cast<int64_t>(t.high) * wide), WM * WN * 64, kSize, stream>>>(a, t);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T, bool DMA>
+hipError_t by_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream) {
+  if constexpr (DMA) {
+    // two steps of it in registers spill: 128 x 256 where they would be
+    if (rows == 256) return launch<T, DMA, 256, 256, 2, 4>(a, stream);
+  }
+  if (rows == 64) {
+    if (channels == 64) return launch<T, DMA, 64, 64, 2, 2>(a, stream);
+    return launch<T, DMA, 64, 128, 2, 2>(a, stream);
+  }
+  if (channels == 128) return launch<T, DMA, 128, 128, 2, 2>(a, stream);
+  return launch<T, DMA, 128, 256, 2, 4>(a, stream);
+}
+
+template <typename T>
+hipError_t by_way(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream) {
+  // straight to LDS: rows that start on 16 bytes, and rows of an index within 32-bit offsets
+  if (codes_on(a, 16) && (a.index == nullptr || static_cast<int64_t>(a.x_rows) * a.c < (int64_t{1} << 32) - (1 << 20))) {
+    return by_tile<T, true>(a, rows, channels, stream);
+  }
+  // Through registers a load from an odd address costs less than the second load and the shifts that few rows
+  // take (1003 x 2051 x 1537: 20 us and 30).
+  return by_tile<T, false>(a, rows, channels, stream);
+}
+
+}  // namespace
+
+hipError_t launch_row8_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream) {
+  return a.bf16 ? by_way<__bf16>(a, rows, channels, stream) : by_way<float>(a, rows, channels, stream);
+}
+
+}  // namespace miq

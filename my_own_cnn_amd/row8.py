@@ -233,19 +233,18 @@ def row8_expand(x: Row8, *, dtype=None, out=None, stream=None):
 
 # ---- products ---------------------------------------------------------------------------------------
 
-def row8_linear_workspace_size(rows: int, c: int, k: int) -> int:
-    """Bytes of device workspace row8_linear(..., workspace=...) needs (no GPU access)."""
-    out = C.c_size_t()
-    check(lib().miq_row8_linear_workspace_size(rows, c, k, C.byref(out)), "row8_linear_workspace_size")
-    return out.value
+def plan_row8_linear(rows: int, c: int, k: int, experts: int = 1):
+    """(few, rows, channels) of row8_linear and, with `experts`, row8_experts: whether the weights go
+    straight to the matrix instructions, and a tile's rows and channels (no GPU access)."""
+    out = (C.c_int32 * 3)()
+    check(lib().miq_plan_row8_linear(rows, c, k, experts, out), "plan_row8_linear")
+    return bool(out[0]), out[1], out[2]
 
 
-def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, workspace=None, stream=None):
+def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, stream=None):
     """A linear layer of 8-bit rows x (..., C) by 8-bit weights w (K, C): the exact int8 product times the
     row's and the channel's scale, plus `bias` (K,), float32, plus `add` (..., K), of the result's
-    type; (..., K), float32 or bfloat16 (`dtype`, default bfloat16).  `out` may be `add`.
-    `workspace`: a device buffer of at least row8_linear_workspace_size() bytes, not used by another
-    call in flight; None allocates one from PyTorch for this call."""
+    type; (..., K), float32 or bfloat16 (`dtype`, default bfloat16).  `out` may be `add`."""
     lead, c = _row8(x, "x")
     w_lead, w_c = _row8(w, "w")
     if len(w_lead) != 1 or w_c != c:
@@ -263,9 +262,8 @@ def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, 
     codes, scales = x
     rows = scales.numel()
     y, ld_y = _output(out, lead + (k,), dtype, codes, stream)
-    at, size, held = _workspace(workspace, "miq_row8_linear_workspace_size", (rows, c, k), codes.device, stream)
     status = lib().miq_row8_linear(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), bias_at, add_at,
-                                   y.data_ptr(), rows, c, k, ld_add, ld_y, kind, at, size, _handle(codes, stream))
+                                   y.data_ptr(), rows, c, k, ld_add, ld_y, kind, _handle(codes, stream))
     if status:
         check(status, "row8_linear")
     return y
@@ -359,5 +357,5 @@ def experts_join(y, places, share=None, *, add=None, out=None, stream=None):
     return to
 
 
-__all__ = ["ExpertsPlan", "Row8", "act_row8", "experts_join", "experts_plan", "rms_bprop", "rms_bprop_workspace_size",
-           "rms_fprop", "rms_row8", "row8_expand", "row8_experts", "row8_linear", "row8_linear_workspace_size"]
+__all__ = ["ExpertsPlan", "Row8", "act_row8", "experts_join", "experts_plan", "plan_row8_linear", "rms_bprop",
+           "rms_bprop_workspace_size", "rms_fprop", "rms_row8", "row8_expand", "row8_experts", "row8_linear"]

@@ -20,7 +20,7 @@ BACK = dict(dy=P, x=P, gain=P, dsum=P, dx=P, dgain=P, rows=4, c=8, ld_dy=8, ld_x
 ACT = dict(x=P, codes=P, scales=P, rows=4, c=8, ld_x=8, act=2, gated=0, type=0, stream=None)
 EXPAND = dict(codes=P, scales=P, y=P, rows=4, c=8, ld_y=8, type=0, stream=None)
 LINEAR = dict(codes=P, scales=P, w_codes=P, w_scales=P, bias=P, add=P, y=P, rows=4, c=8, k=8, ld_add=8, ld_y=8, type=0,
-              ws=P, ws_bytes=BIG, stream=None)
+              stream=None)
 EXPERTS = dict(codes=P, scales=P, w_codes=P, w_scales=P, bias=P, offsets=P, index=P, y=P, x_rows=4, rows=4, c=8, k=8,
                experts=2, ld_y=8, type=0, stream=None)
 PLAN = dict(ids=P, offsets=P, rows=P, places=P, tokens=4, slots=2, experts=3, id_type=2, stream=None)
@@ -87,7 +87,6 @@ REFUSED = [
     ("miq_row8_linear", LINEAR, dict(y=None), NULL, "output"),
     ("miq_row8_linear", LINEAR, dict(bias=P + 2), BAD, "aligned"),
     ("miq_row8_linear", LINEAR, dict(add=P + 1, type=1), BAD, "aligned"),
-    ("miq_row8_linear", LINEAR, dict(ws=P + 8), BAD, "16 bytes"),
     ("miq_row8_experts", EXPERTS, dict(experts=0), BAD, "4096"),
     ("miq_row8_experts", EXPERTS, dict(experts=4097), BAD, "4096"),
     ("miq_row8_experts", EXPERTS, dict(x_rows=-1), BAD, "x_rows"),
@@ -149,10 +148,7 @@ def test_workspace_sizes():
     assert M.rms_bprop_workspace_size(1 << 17, 1 << 29) > 1 << 32
     with pytest.raises(M.MiqError, match="2\\^46"):
         M.rms_bprop_workspace_size(1 << 40, 1 << 10)
-    with pytest.raises(M.MiqError, match="131071"):
-        M.row8_linear_workspace_size(1, 131072, 1)
     assert M.lib().miq_rms_bprop_workspace_size(1, 1, None) == NULL
-    assert M.lib().miq_row8_linear_workspace_size(1, 1, 1, None) == NULL
 
 
 def test_host_tensors_are_refused():
@@ -167,7 +163,7 @@ def test_host_tensors_are_refused():
             call()
 
 
-@pytest.mark.parametrize("src", ["rms.hip", "rms_grad.hip", "row8.hip", "row8_linear.hip", "experts.hip"])
+@pytest.mark.parametrize("src", ["rms.hip", "rms_grad.hip", "row8.hip", "row8_few.hip", "row8_tile.hip", "experts.hip"])
 def test_every_wide_store_is_followed_by_two_wait_states(src, tmp_path):
     dst = tmp_path / "k.s"
     subprocess.run([B.hipcc(), *B.common_flags(), "--cuda-device-only", "-S", str(B.CSRC / src), "-o", str(dst)],
