@@ -19,11 +19,23 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(ExpertsPlanA
   const int64_t each = (runs + kPlanWaves - 1) / kPlanWaves;
   const int64_t from = min(wave * each, runs) * 64;
   const int64_t to = min((wave + 1) * each, runs) * 64;
+  // four runs of 64 at a time, loaded together
+  auto load = [&](int64_t base, ID (&id)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = base + u * 64 + lane;
+      id[u] = i < to && i < a.n ? ids[i] : -1;
+    }
+  };
   int less = 0, same = 0;
-  for (int64_t i = from + lane; i < to; i += 64) {
-    const ID id = i < a.n ? ids[i] : -1;
-    less += id >= 0 && id < expert;
-    same += id == expert;
+  for (int64_t base = from; base < to; base += 256) {
+    ID id[4];
+    load(base, id);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      less += id[u] >= 0 && id[u] < expert;
+      same += id[u] == expert;
+    }
   }
   for (int step = 1; step < 64; step *= 2) {
     less += __shfl_xor(less, step);
@@ -41,17 +53,21 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(ExpertsPlanA
     count += own[w];
   }
   at += start;
-  for (int64_t base = from; base < to; base += 64) {
-    const int64_t i = base + lane;
-    const ID id = i < a.n ? ids[i] : -1;
-    const uint64_t mine = __ballot(i < a.n && id == expert);
-    if (mine >> lane & 1) {
-      const int place = at + __popcll(mine & ((uint64_t{1} << lane) - 1));
-      a.rows[place] = fdiv(static_cast<int>(i), by_slots);
-      a.places[i] = place;
+  for (int64_t base = from; base < to; base += 256) {
+    ID id[4];
+    load(base, id);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = base + u * 64 + lane;
+      const uint64_t mine = __ballot(id[u] == expert);
+      if (mine >> lane & 1) {
+        const int place = at + __popcll(mine & ((uint64_t{1} << lane) - 1));
+        a.rows[place] = fdiv(static_cast<int>(i), by_slots);
+        a.places[i] = place;
+      }
+      if (expert == 0 && i < to && i < a.n && (id[u] < 0 || id[u] >= a.experts)) a.places[i] = -1;
+      at += __popcll(mine);
     }
-    if (expert == 0 && i < a.n && (id < 0 || id >= a.experts)) a.places[i] = -1;
-    at += __popcll(mine);
   }
   if (threadIdx.x == 0) a.offsets[expert] = start;
   if (expert == a.experts - 1) {

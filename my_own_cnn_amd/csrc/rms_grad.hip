@@ -14,7 +14,31 @@
 namespace miq {
 namespace {
 
-constexpr int kParts = 1024;  // workgroups, and rows of the workspace, at most
+constexpr int kParts = 512;                // workgroups, and rows of the workspace, at most
+constexpr int64_t kWorkspace = 1 << 25;  // values of it, while that leaves a workgroup
+
+// 16 bytes of a row as they lie in memory, zeros past its end.
+template <typename T>
+struct RawOf;
+template <>
+struct RawOf<__bf16> {
+  typedef v8bf type;
+  typedef v8bf_any any;
+};
+template <>
+struct RawOf<float> {
+  typedef v4f type;
+  typedef v4f_any any;
+};
+template <typename T>
+__device__ __forceinline__ typename RawOf<T>::type load_raw(const T* p, int left) {
+  if (left >= kWide<T>) return *reinterpret_cast<const typename RawOf<T>::any*>(p);
+  typename RawOf<T>::type v = {};
+#pragma unroll
+  for (int i = 0; i < kWide<T>; ++i)
+    if (i < left) v[i] = p[i];
+  return v;
+}
 
 template <int W, typename G>
 __device__ __forceinline__ typename Vec<W>::type load_gain(const G* p, int left) {
@@ -26,7 +50,7 @@ __device__ __forceinline__ typename Vec<W>::type load_gain(const G* p, int left)
 }
 
 template <typename T, typename G, int THREADS, int V>
-__global__ __launch_bounds__(kRowBlock<THREADS>) void rms_grad_kernel(RmsGradArgs a) {
+__global__ __launch_bounds__(kRowBlock<THREADS>, THREADS == 1024 ? 4 : 2) void rms_grad_kernel(RmsGradArgs a) {
   constexpr int W = kWide<T>;
   constexpr int kThreads = kRowBlock<THREADS>, kRows = kThreads / THREADS;
   typedef typename Vec<W>::type Run;
@@ -41,10 +65,31 @@ __global__ __launch_bounds__(kRowBlock<THREADS>) void rms_grad_kernel(RmsGradArg
     g[j] = load_gain<W>(static_cast<const G*>(a.gain) + col, a.c - col);
     total[j] = Run{};
   }
+  // the next row's values travel while this one is summed
+  typename RawOf<T>::type next_s[V], next_d[V], next_e[V];
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int col = (j * THREADS + t) * W;
+      next_s[j] = load_raw(static_cast<const T*>(a.x) + row * a.ld_x + col, a.c - col);
+      next_d[j] = load_raw(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.c - col);
+      if (a.dsum != nullptr) next_e[j] = load_raw(static_cast<const T*>(a.dsum) + row * a.ld_dsum + col, a.c - col);
+    }
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own;
+  if (row < a.rows) load(row);
   int turn = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own; row < a.rows;
-       row += static_cast<int64_t>(gridDim.x) * kRows) {
+  for (; row < a.rows; row += step) {
     Run s[V], d[V];
+    typename RawOf<T>::type e[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s[j] = __builtin_convertvector(next_s[j], Run);
+      d[j] = __builtin_convertvector(next_d[j], Run);
+      e[j] = next_e[j];
+    }
+    if (row + step < a.rows) load(row + step);
     float squares = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -86,7 +131,7 @@ __global__ __launch_bounds__(kRowBlock<THREADS>) void rms_grad_kernel(RmsGradArg
       const Run n = s[j] * r;
       total[j] += d[j] * n;
       Run dx = (d[j] * g[j] - n * along) * (r * down);
-      if (a.dsum != nullptr) dx += load_some<false>(static_cast<const T*>(a.dsum) + row * a.ld_dsum + col, a.c - col);
+      if (a.dsum != nullptr) dx += __builtin_convertvector(e[j], Run);
       store_some<false>(static_cast<T*>(a.dx) + row * a.ld_dx + col, dx, a.c - col);
     }
   }
@@ -173,8 +218,11 @@ __global__ __launch_bounds__(1024) void rms_grad_join_kernel(const float* __rest
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   for (int base = blockIdx.x * 32; base < c; base += gridDim.x * 32) {
     float s = 0.0f;
-    if (base + x < c)
-      for (int p = y; p < parts; p += 32) s += ws[static_cast<int64_t>(p) * c + base + x];
+    if (base + x < c) {
+      const float* from = ws + base + x;
+#pragma unroll 8
+      for (int p = y; p < parts; p += 32) s += from[static_cast<int64_t>(p) * c];
+    }
     lds[y][x] = s;
     __syncthreads();
     if (y == 0 && base + x < c) {
@@ -186,9 +234,10 @@ __global__ __launch_bounds__(1024) void rms_grad_join_kernel(const float* __rest
   }
 }
 
-// A workgroup for at least four rows (sixteen, a wave a row), so that the workspace stays small beside
-// the rows.
-int64_t parts_of(int64_t rows) { return std::min<int64_t>(kParts, (rows + 3) / 4); }
+// Workgroups, each with a row of the workspace: two a CU while there are rows for them.
+int64_t parts_of(int64_t rows, int64_t c) {
+  return std::min({rows, static_cast<int64_t>(kParts), std::max<int64_t>(kWorkspace / c, 1)});
+}
 
 template <typename T, typename G>
 void launch(const RmsGradArgs& a, int64_t parts, hipStream_t stream) {
@@ -204,10 +253,10 @@ void launch(const RmsGradArgs& a, int64_t parts, hipStream_t stream) {
 
 }  // namespace
 
-size_t rms_grad_workspace_bytes(int64_t rows, int32_t c) { return static_cast<size_t>(parts_of(rows)) * c * sizeof(float); }
+size_t rms_grad_workspace_bytes(int64_t rows, int32_t c) { return static_cast<size_t>(parts_of(rows, c)) * c * sizeof(float); }
 
 hipError_t launch_rms_grad(const RmsGradArgs& a, hipStream_t stream) {
-  const int64_t parts = parts_of(a.rows);
+  const int64_t parts = parts_of(a.rows, a.c);
   if (parts > 0) {
     if (a.bf16) a.gain_bf16 ? launch<__bf16, __bf16>(a, parts, stream) : launch<__bf16, float>(a, parts, stream);
     else a.gain_bf16 ? launch<float, __bf16>(a, parts, stream) : launch<float, float>(a, parts, stream);

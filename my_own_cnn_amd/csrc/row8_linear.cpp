@@ -25,8 +25,8 @@ struct Tile {
 constexpr Tile kTiles[] = {{64, 64, 0.18, 0.13, 0.4},
                            {64, 128, 0.205, 0.21, 0.7},
                            {128, 128, 0.24, 0.31, 1.3},
-                           {128, 256, 0.36, 0.5, 2.5},
-                           {256, 256, 0.55, 0.8, 6}};
+                           {128, 256, 0.36, 0.57, 2.5},
+                           {256, 256, 0.55, 0.84, 7}};
 // Rows that do not start on 16 bytes go through registers.
 constexpr double kThroughRegisters = 1.5;
 // Few rows: bound by what a CU takes in, 38 KB a us (21 where rows do not start on 4 bytes); us for a tile's
@@ -62,7 +62,9 @@ Shape shape_of(int64_t rows, int64_t c, int64_t k, int64_t experts) {
   const double steps = static_cast<double>(over(c, 64)) * (c % 16 == 0 ? 1.0 : kThroughRegisters);
   for (const Tile& t : kTiles) {
     if (c < 16 || (t.rows == 256 && c % 16 != 0)) continue;
-    const int64_t tiles = groups * over(part, t.rows) * over(k, t.channels), rounds = over(tiles, 256);
+    // of experts the last row tile is half full
+    const double high = groups == 1 ? over(part, t.rows) : std::max(1.0, static_cast<double>(part) / t.rows + 0.5);
+    const int64_t tiles = static_cast<int64_t>(groups * high) * over(k, t.channels), rounds = over(tiles, 256);
     take({false, t.rows, t.channels}, kLaunch + steps * std::max(t.alone, t.each * rounds) + t.output * rounds);
   }
   return best;

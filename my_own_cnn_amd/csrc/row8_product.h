@@ -13,16 +13,32 @@ struct RowTile {
   int expert, row0, end;
 };
 
-// Tile number `tile` of the experts' row tiles of `high` rows, in their order: every wave looks for it by
-// itself, 64 experts at a time.  Offsets are held to 0 .. rows and to rising order.
+// An expert's rows, held to 0 .. rows and to rising order, and its row tiles of `high` rows.
+struct ExpertRows {
+  int lo, hi, tiles;
+};
+__device__ __forceinline__ ExpertRows expert_rows(const int32_t* offsets, int experts, int rows, int high, int expert) {
+  const int e = min(expert, experts - 1);
+  const int lo = min(max(offsets[e], 0), rows);
+  const int hi = min(max(offsets[e + 1], lo), rows);
+  return {lo, hi, expert < experts && hi > lo ? (hi - lo - 1) / high + 1 : 0};
+}
+
+// All experts' row tiles; every wave counts them by itself, 64 experts at a time.
+__device__ __forceinline__ int count_tiles(const int32_t* offsets, int experts, int rows, int high) {
+  int count = 0;
+  for (int base = 0; base < experts; base += 64)
+    count += expert_rows(offsets, experts, rows, high, base + (static_cast<int>(threadIdx.x) & 63)).tiles;
+  for (int step = 1; step < 64; step *= 2) count += __shfl_xor(count, step);
+  return __builtin_amdgcn_readfirstlane(count);
+}
+
+// Tile number `tile` of the experts' row tiles, in their order.
 __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int experts, int rows, int high, int tile) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
   for (int base = 0; base < experts; base += 64) {
-    const int e = min(base + lane, experts - 1);
-    const int lo = min(max(offsets[e], 0), rows);
-    const int hi = min(max(offsets[e + 1], lo), rows);
-    const int count = base + lane < experts && hi > lo ? (hi - lo - 1) / high + 1 : 0;
-    int upto = count;  // this expert's tiles and those before it
+    const ExpertRows e = expert_rows(offsets, experts, rows, high, base + lane);
+    int upto = e.tiles;  // this expert's tiles and those before it
     for (int step = 1; step < 64; step *= 2) {
       const int other = __shfl_up(upto, step);
       if (lane >= step) upto += other;
@@ -30,8 +46,8 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int experts
     const uint64_t past = __ballot(upto > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      const int row0 = __shfl(lo, at) + (tile - (__shfl(upto, at) - __shfl(count, at))) * high;
-      const int last = __shfl(hi, at), end = last - row0 < high ? last : row0 + high;
+      const int row0 = __shfl(e.lo, at) + (tile - (__shfl(upto, at) - __shfl(e.tiles, at))) * high;
+      const int last = __shfl(e.hi, at), end = last - row0 < high ? last : row0 + high;
       return {__builtin_amdgcn_readfirstlane(base + at), __builtin_amdgcn_readfirstlane(row0),
               __builtin_amdgcn_readfirstlane(end)};
     }

@@ -35,6 +35,30 @@ __device__ __forceinline__ int channel_of(int p) {
   return (p & ~31) + ((p >> 2) & 3) * 8 + ((p >> 4) & 1) * 4 + (p & 3);
 }
 
+// Tile `id` of a launch: tiles go in bands of eight rows of tiles, so that neighbours share their rows and
+// channels in an L2.  Experts' tiles are dealt to the XCDs by their real number (`high` row tiles), not by
+// the most that the launch allows for.
+struct Place {
+  RowTile r;
+  int n0;
+};
+template <int BM, int BN>
+__device__ __forceinline__ Place place_of(const Row8LinearArgs& a, const Tiling& tiling, int high, int id) {
+  constexpr int kBand = 8;
+  const int at = xcd_tile(id, high * tiling.wide);
+  const int band = at / (kBand * tiling.wide);
+  const int band_high = min(kBand, high - band * kBand);
+  const int in = at - band * kBand * tiling.wide;
+  const int row_tile = tiling.from + band * kBand + in % band_high, n0 = in / band_high * BN;
+  if (a.offsets != nullptr) return {find_tile(a.offsets, a.experts, a.rows, BM, row_tile), n0};
+  return {{0, row_tile * BM, a.rows - row_tile * BM < BM ? a.rows : (row_tile + 1) * BM}, n0};
+}
+template <int BM>
+__device__ __forceinline__ int row_tiles(const Row8LinearArgs& a, const Tiling& tiling) {
+  if (a.offsets == nullptr) return tiling.high;
+  return min(tiling.high, count_tiles(a.offsets, a.experts, a.rows, BM) - tiling.from);
+}
+
 template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) void row8_tile_kernel(Row8LinearArgs a, Tiling tiling) {
   constexpr int kWaves = WM * WN;
@@ -45,18 +69,11 @@ __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 :
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // Tiles in bands of eight rows of tiles: neighbours share their rows and channels in an L2.
-  constexpr int kBand = 8;
-  const int at = xcd_tile(blockIdx.x, gridDim.x);
-  const int band = at / (kBand * tiling.wide);
-  const int band_high = min(kBand, tiling.high - band * kBand);
-  const int in = at - band * kBand * tiling.wide;
-  const int row_tile = tiling.from + band * kBand + in % band_high, n0 = in / band_high * BN;
-  RowTile r = {0, row_tile * BM, a.rows - row_tile * BM < BM ? a.rows : (row_tile + 1) * BM};
-  if (a.offsets != nullptr) {
-    r = find_tile(a.offsets, a.experts, a.rows, BM, row_tile);
-    if (r.expert < 0) return;
-  }
+  const int high = row_tiles<BM>(a, tiling);
+  if (static_cast<int>(blockIdx.x) >= high * tiling.wide) return;
+  const Place place = place_of<BM, BN>(a, tiling, high, blockIdx.x);
+  const RowTile r = place.r;
+  const int n0 = place.n0;
   const int rows = r.end - r.row0, channels = min(BN, a.k - n0);
   const int64_t w_at = (static_cast<int64_t>(r.expert) * a.k + n0) * a.c;
 

@@ -20,8 +20,9 @@ CASES = [
     (8200, 67, 130, 1, (False, 64, 64)),
     (1, 64, 16400, 1, (False, 64, 128)), (5, 112, 4100, 4, (False, 64, 128)), (50, 68, 4099, 4, (False, 64, 128)),
     (5, 67, 4100, 4, (False, 64, 128)),
-    (257, 336, 4100, 4, (False, 128, 128)), (200, 68, 8201, 1, (False, 128, 128)), (257, 67, 4100, 4, (False, 128, 128)),
-    (257, 336, 8199, 4, (False, 128, 256)), (257, 324, 8200, 4, (False, 128, 256)), (257, 323, 8200, 4, (False, 128, 256)),
+    (400, 80, 6150, 4, (False, 128, 128)), (200, 68, 8201, 1, (False, 128, 128)), (257, 67, 6150, 4, (False, 128, 128)),
+    (200, 656, 16397, 1, (False, 128, 256)), (700, 80, 8199, 4, (False, 128, 256)), (700, 68, 8200, 4, (False, 128, 256)),
+    (700, 67, 8200, 4, (False, 128, 256)),
     (700, 656, 16397, 1, (False, 256, 256)), (1500, 592, 8200, 2, (False, 256, 256)),
 ]
 
