@@ -12,8 +12,11 @@ from typing import NamedTuple, Optional
 
 from ._capi import check, lib
 from .conv import _stream
-from .train import (_IDS, _act, _alike, _alloc, _dense, _halves, _here, _kind, _on_device, _output, _raw_stream, _rows,
-                    _workspace, torch)
+from .train import (_IDS, _REAL, _act, _alike, _alloc, _dense, _halves, _here, _kind, _on_device, _output, _raw_stream,
+                    _rows, _workspace, torch)
+
+if torch is not None:
+    _I8, _I32, _F32, _BF16 = torch.int8, torch.int32, torch.float32, torch.bfloat16
 
 
 class Row8(NamedTuple):
@@ -34,6 +37,10 @@ class ExpertsPlan(NamedTuple):
     places: "torch.Tensor"
 
 
+# The calls' checks are inline, like train.py's: on small tensors a call is bound by its time on the host.
+_MAKE = tuple.__new__
+
+
 def _new_row8(lead, c: int, like, kept: Optional[Row8], stream) -> Row8:
     """Storage for 8-bit rows (*lead, c): `kept`, or new."""
     if kept is not None:
@@ -43,33 +50,34 @@ def _new_row8(lead, c: int, like, kept: Optional[Row8], stream) -> Row8:
             raise ValueError(f"kept must hold codes of shape {lead + (c,)} and scales of shape {lead}")
         return Row8(kept[0], kept[1])
     if stream is None:
-        return Row8(like.new_empty(lead + (c,), dtype=torch.int8), like.new_empty(lead, dtype=torch.float32))
-    return Row8(_alloc(lead + (c,), torch.int8, like.device, stream), _alloc(lead, torch.float32, like.device, stream))
+        shape = lead + (c,)
+        if like.shape == shape and like.is_contiguous():
+            return _MAKE(Row8, (torch.empty_like(like, dtype=_I8), like.new_empty(lead, dtype=_F32)))
+        return _MAKE(Row8, (like.new_empty(shape, dtype=_I8), like.new_empty(lead, dtype=_F32)))
+    return Row8(_alloc(lead + (c,), _I8, like.device, stream), _alloc(lead, _F32, like.device, stream))
 
 
 def _row8(x, what: str):
-    """(shape of the rows, channels) of 8-bit rows."""
+    """Shape of 8-bit rows (..., C)."""
     codes, scales = x
     at = codes.get_device()
-    if (codes.dtype != torch.int8 or scales.dtype != torch.float32 or at < 0 or at != _here() or
-            scales.get_device() != at or not codes.is_contiguous() or not scales.is_contiguous()):
-        _dense(codes, torch.int8, f"{what} codes")
-        _dense(scales, torch.float32, f"{what} scales")
-    shape = tuple(codes.shape)
-    if not shape:
-        raise ValueError(f"{what} codes must have a channel dimension")
-    if scales.shape != shape[:-1]:
-        raise ValueError(f"{what} scales must be {shape[:-1]}, got {tuple(scales.shape)}")
-    return shape[:-1], shape[-1]
+    shape = codes.shape
+    if (at < 0 or at != _here() or codes.dtype is not _I8 or scales.dtype is not _F32 or scales.get_device() != at or
+            not codes.is_contiguous() or not scales.is_contiguous() or scales.shape != shape[:-1] or not shape):
+        _dense(codes, _I8, f"{what} codes")
+        _dense(scales, _F32, f"{what} scales")
+        if not shape:
+            raise ValueError(f"{what} codes must have a channel dimension")
+        raise ValueError(f"{what} scales must be {tuple(shape[:-1])}, got {tuple(scales.shape)}")
+    return shape
 
 
 def _vector(v, size: int, what: str):
     """(address, kind) of a real vector of `size` values."""
-    kind = _kind(v.dtype, what)
-    at = v.get_device()
-    if at < 0 or at != _here():
+    kind = _REAL.get(v.dtype)
+    if kind is None or v.get_device() != _here() or v.shape != (size,) or not v.is_contiguous():
+        _kind(v.dtype, what)
         _on_device(v, what)
-    if v.shape != (size,) or not v.is_contiguous():
         raise ValueError(f"{what} must be contiguous, of shape {(size,)}")
     return v.data_ptr(), kind
 
@@ -81,10 +89,6 @@ def _f32_of(v, shape, what: str):
     if v.shape != shape:
         raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(v.shape)}")
     return _dense(v, torch.float32, what)
-
-
-def _ints(v, what: str):
-    return _dense(v, torch.int32, what)
 
 
 def _handle(like, stream):
@@ -102,8 +106,8 @@ def _added(x, add, total, shape, stream):
     if add.shape != shape or add.dtype != x.dtype:
         raise ValueError(f"add must be {x.dtype} of shape {shape}")
     ld_add = _rows(add, "add")[2]
-    if x.is_contiguous():
-        total, ld = _alike(total, x, shape, x.dtype, stream)
+    if total is None and stream is None and ld_add == shape[-1] and x.is_contiguous():
+        total, ld = torch.empty_like(x), ld_add
     else:
         total, ld = _output(total, shape, x.dtype, x, stream)
     return add.data_ptr(), ld_add, total, total.data_ptr(), ld
@@ -218,14 +222,19 @@ def act_row8(x, act: str = "none", *, gated: bool = False, kept: Optional[Row8] 
 
 def row8_expand(x: Row8, *, dtype=None, out=None, stream=None):
     """What 8-bit rows stand for, code * scale, as float32 or bfloat16 (`dtype`, default float32)."""
-    lead, c = _row8(x, "x")
+    shape = _row8(x, "x")
     codes, scales = x
     if dtype is None:
-        dtype = out.dtype if out is not None else torch.float32
-    kind = _kind(dtype, "dtype")
-    y, ld_y = _alike(out, codes, lead + (c,), dtype, stream)
-    status = lib().miq_row8_expand(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), scales.numel(), c, ld_y, kind,
-                                   _handle(codes, stream))
+        dtype = out.dtype if out is not None else _F32
+    kind = _REAL.get(dtype)
+    if kind is None:
+        _kind(dtype, "dtype")
+    c = shape[-1]
+    if out is None and stream is None:
+        y, ld_y, handle = torch.empty_like(codes, dtype=dtype), c, _raw_stream(codes.get_device())
+    else:
+        (y, ld_y), handle = _output(out, tuple(shape), dtype, codes, stream), _handle(codes, stream)
+    status = lib().miq_row8_expand(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), scales.numel(), c, ld_y, kind, handle)
     if status:
         check(status, "row8_expand")
     return y
@@ -245,25 +254,31 @@ def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, 
     """A linear layer of 8-bit rows x (..., C) by 8-bit weights w (K, C): the exact int8 product times the
     row's and the channel's scale, plus `bias` (K,), float32, plus `add` (..., K), of the result's
     type; (..., K), float32 or bfloat16 (`dtype`, default bfloat16).  `out` may be `add`."""
-    lead, c = _row8(x, "x")
-    w_lead, w_c = _row8(w, "w")
-    if len(w_lead) != 1 or w_c != c:
-        raise ValueError(f"w must be (output channels, {c}), got {w_lead + (w_c,)}")
-    k = w_lead[0]
+    shape = _row8(x, "x")
+    w_shape = _row8(w, "w")
+    c = shape[-1]
+    if len(w_shape) != 2 or w_shape[1] != c:
+        raise ValueError(f"w must be (output channels, {c}), got {tuple(w_shape)}")
+    k = w_shape[0]
     if dtype is None:
-        dtype = out.dtype if out is not None else (add.dtype if add is not None else torch.bfloat16)
-    kind = _kind(dtype, "dtype")
-    bias_at = _f32_of(bias, (k,), "bias")
+        dtype = out.dtype if out is not None else (add.dtype if add is not None else _BF16)
+    kind = _REAL.get(dtype)
+    if kind is None:
+        _kind(dtype, "dtype")
+    y_shape = (shape[0], k) if len(shape) == 2 else tuple(shape[:-1]) + (k,)
     add_at, ld_add = None, 0
     if add is not None:
-        if add.shape != lead + (k,) or add.dtype != dtype:
-            raise ValueError(f"add must be {dtype} of shape {lead + (k,)}")
+        if add.shape != y_shape or add.dtype is not dtype:
+            raise ValueError(f"add must be {dtype} of shape {y_shape}")
         add_at, ld_add = add.data_ptr(), _rows(add, "add")[2]
     codes, scales = x
-    rows = scales.numel()
-    y, ld_y = _output(out, lead + (k,), dtype, codes, stream)
-    status = lib().miq_row8_linear(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), bias_at, add_at,
-                                   y.data_ptr(), rows, c, k, ld_add, ld_y, kind, _handle(codes, stream))
+    if out is None and stream is None:
+        y, ld_y, handle = codes.new_empty(y_shape, dtype=dtype), k, _raw_stream(codes.get_device())
+    else:
+        (y, ld_y), handle = _output(out, y_shape, dtype, codes, stream), _handle(codes, stream)
+    status = lib().miq_row8_linear(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(),
+                                   None if bias is None else _f32_of(bias, (k,), "bias"), add_at, y.data_ptr(),
+                                   scales.numel(), c, k, ld_add, ld_y, kind, handle)
     if status:
         check(status, "row8_linear")
     return y
@@ -280,18 +295,20 @@ def experts_plan(ids, experts: int, *, stream=None) -> ExpertsPlan:
     if len(shape) not in (1, 2):
         raise ValueError("ids must be (tokens, slots) or (tokens,)")
     slots = shape[1] if len(shape) == 2 else 1
+    if experts < 1:
+        raise ValueError("experts must be at least 1")
     ids_at = _dense(ids, ids.dtype, "ids")
     if stream is None:
-        offsets = ids.new_empty((experts + 1,), dtype=torch.int32)
-        rows = ids.new_empty((ids.numel(),), dtype=torch.int32)
-        places = torch.empty_like(ids, dtype=torch.int32)
+        offsets = ids.new_empty(experts + 1, dtype=_I32)
+        rows = ids.new_empty(ids.numel(), dtype=_I32)
+        places = torch.empty_like(ids, dtype=_I32)
     else:
         offsets, rows, places = (_alloc(s, torch.int32, ids.device, stream) for s in ((experts + 1,), (ids.numel(),), shape))
     status = lib().miq_experts_plan(ids_at, offsets.data_ptr(), rows.data_ptr(), places.data_ptr(), shape[0], slots,
                                     experts, _IDS[ids.dtype], _handle(ids, stream))
     if status:
         check(status, "experts_plan")
-    return ExpertsPlan(offsets, rows, places)
+    return _MAKE(ExpertsPlan, (offsets, rows, places))
 
 
 def row8_experts(x: Row8, w: Row8, offsets, *, rows=None, bias=None, dtype=None, out=None, stream=None):
@@ -300,30 +317,35 @@ def row8_experts(x: Row8, w: Row8, offsets, *, rows=None, bias=None, dtype=None,
     `rows`; an entry of `rows` outside x stands for a row of zeros.  offsets (experts + 1,) and
     `rows` are int32 tensors on the device, as experts_plan gives them; offsets rise and end within
     the rows.  Rows of the result behind the last expert's are not written."""
-    lead, c = _row8(x, "x")
-    w_lead, w_c = _row8(w, "w")
-    if len(lead) != 1:
+    shape = _row8(x, "x")
+    w_shape = _row8(w, "w")
+    if len(shape) != 2:
         raise ValueError("x must be (rows, channels)")
-    if len(w_lead) != 2 or w_c != c:
-        raise ValueError(f"w must be (experts, output channels, {c}), got {w_lead + (w_c,)}")
-    experts, k = w_lead
+    n, c = shape
+    if len(w_shape) != 3 or w_shape[2] != c:
+        raise ValueError(f"w must be (experts, output channels, {c}), got {tuple(w_shape)}")
+    experts, k, _ = w_shape
     if offsets.shape != (experts + 1,):
         raise ValueError(f"offsets must be {(experts + 1,)}, got {tuple(offsets.shape)}")
-    offsets_at = _ints(offsets, "offsets")
-    n, rows_at = lead[0], None
+    offsets_at = _dense(offsets, _I32, "offsets")
+    x_rows, rows_at = n, None
     if rows is not None:
         if rows.dim() != 1:
             raise ValueError("rows must have one dimension")
-        n, rows_at = rows.shape[0], _ints(rows, "rows")
+        n, rows_at = rows.numel(), _dense(rows, _I32, "rows")
     if dtype is None:
-        dtype = out.dtype if out is not None else torch.bfloat16
-    kind = _kind(dtype, "dtype")
-    bias_at = _f32_of(bias, (experts, k), "bias")
+        dtype = out.dtype if out is not None else _BF16
+    kind = _REAL.get(dtype)
+    if kind is None:
+        _kind(dtype, "dtype")
     codes, scales = x
-    y, ld_y = _output(out, (n, k), dtype, codes, stream)
-    status = lib().miq_row8_experts(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), bias_at,
-                                    offsets_at, rows_at, y.data_ptr(), lead[0], n, c, k, experts, ld_y, kind,
-                                    _handle(codes, stream))
+    if out is None and stream is None:
+        y, ld_y, handle = codes.new_empty((n, k), dtype=dtype), k, _raw_stream(codes.get_device())
+    else:
+        (y, ld_y), handle = _output(out, (n, k), dtype, codes, stream), _handle(codes, stream)
+    status = lib().miq_row8_experts(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(),
+                                    None if bias is None else _f32_of(bias, (experts, k), "bias"), offsets_at, rows_at,
+                                    y.data_ptr(), x_rows, n, c, k, experts, ld_y, kind, handle)
     if status:
         check(status, "row8_experts")
     return y
@@ -342,7 +364,7 @@ def experts_join(y, places, share=None, *, add=None, out=None, stream=None):
     if len(shape) not in (1, 2):
         raise ValueError("places must be (tokens, slots) or (tokens,)")
     slots = shape[1] if len(shape) == 2 else 1
-    places_at = _ints(places, "places")
+    places_at = _dense(places, _I32, "places")
     share_at = _f32_of(share, shape, "share")
     add_at, ld_add = None, 0
     if add is not None:
