@@ -580,12 +580,17 @@ int miq_row8_expand(const int8_t* codes, const float* scales, void* y, int64_t r
  * distance).  rows up to 2^31 - 65, c up to 131071, k up to 2^22. */
 int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
                     const float* bias, const void* add, void* y, int64_t rows, int32_t c, int32_t k, int64_t ld_add,
-                    int64_t ld_y, int32_t type, void* stream);
+                    int64_t ld_y, int32_t type, void* workspace, size_t workspace_bytes, void* stream);
 
-/* How miq_row8_linear (experts 1) and miq_row8_experts run a problem: plan[0] is 1 where the weights go straight
- * to the matrix instructions (few rows) and 0 where tiles of both operands go through LDS, plan[1] and
- * plan[2] are a tile's rows and channels; zeros where there is nothing to do.  No GPU access. */
-int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]);
+/* Bytes of device workspace miq_row8_linear (x_rows == rows, experts 1) and miq_row8_experts need: 0 wherever c is a
+ * multiple of 16, and for few rows (no GPU access). */
+int miq_row8_workspace_size(int64_t x_rows, int64_t rows, int32_t c, int32_t k, int32_t experts, size_t* bytes);
+
+/* How miq_row8_linear (experts 1) and miq_row8_experts (on as many rows of x) run a problem: plan[0] is 1 where the
+ * weights go straight to the matrix instructions (few rows) and 0 where tiles of both operands go through
+ * LDS, plan[1] and plan[2] are a tile's rows and channels, plan[3] is 1 where rows of codes are first copied to
+ * the workspace, each to whole lines; zeros where there is nothing to do.  No GPU access. */
+int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[4]);
 
 /* The products of a layer of experts: rows offsets[e] .. offsets[e + 1] - 1 of y by the weights of expert e
  * (w_codes: experts x k x c, w_scales and bias: experts x k).  Row i of y takes row index[i] of the
@@ -594,7 +599,8 @@ int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, in
  * a row; rows of y outside them are left as they were.  experts up to 4096. */
 int miq_row8_experts(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
                      const float* bias, const int32_t* offsets, const int32_t* index, void* y, int64_t x_rows,
-                     int64_t rows, int32_t c, int32_t k, int32_t experts, int64_t ld_y, int32_t type, void* stream);
+                     int64_t rows, int32_t c, int32_t k, int32_t experts, int64_t ld_y, int32_t type, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 /* The (token, slot) pairs of ids (tokens x slots) sorted by expert, in their order within an expert:
  * offsets[e] (experts + 1) is where expert e's pairs start, rows[i] (tokens * slots) the token of sorted

@@ -13,7 +13,7 @@ from .conv import (BlockConv2DParams, bmm_i32, bmm_matmul_i32, conv2d_nhwc_f32, 
 from .train import (Act8, act8_bprop, act8_expand, act8_fprop, act8_grad, act8_grad_workspace_size, act8_keep, embed_fprop,
                     embed_grad, embed_grad_workspace_size, plan_act8_grad, plan_embed_grad)
 from .row8 import (ExpertsPlan, Row8, act_row8, experts_join, experts_plan, plan_row8_linear, rms_bprop,
-                   rms_bprop_workspace_size, rms_fprop, rms_row8, row8_expand, row8_experts, row8_linear)
+                   rms_bprop_workspace_size, rms_fprop, rms_row8, row8_expand, row8_experts, row8_linear, row8_workspace_size)
 from ._capi import LIB_PATH, lib
 from .workloads import HEADLINE, WORKLOADS, Workload
 
@@ -27,5 +27,6 @@ __all__ = [
     "embed_fprop", "embed_grad", "embed_grad_workspace_size", "plan_act8_grad", "plan_embed_grad",
     "ExpertsPlan", "Row8", "act_row8", "experts_join", "experts_plan", "plan_row8_linear", "rms_bprop",
     "rms_bprop_workspace_size", "rms_fprop", "rms_row8", "row8_expand", "row8_experts", "row8_linear",
+    "row8_workspace_size",
     "LIB_PATH", "lib", "HEADLINE", "WORKLOADS", "Workload",
 ]

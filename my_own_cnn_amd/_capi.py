@@ -172,10 +172,12 @@ SIGNATURES = {
         C.c_int, [_P, _P, _P, _P, _P, _P, _L, _I, _L, _L, _L, _L, C.c_float, _I, _I, _I, _I, _P, C.c_size_t, _P]),
     "miq_act_row8": (C.c_int, [_P, _P, _P, _L, _I, _L, _I, _I, _I, _P]),
     "miq_row8_expand": (C.c_int, [_P, _P, _P, _L, _I, _L, _I, _P]),
-    "miq_row8_linear": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _L, _L, _I, _P]),
+    "miq_row8_workspace_size": (C.c_int, [_L, _L, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    "miq_row8_linear": (
+        C.c_int, [_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _L, _L, _I, _P, C.c_size_t, _P]),
     "miq_plan_row8_linear": (C.c_int, [_L, _I, _I, _I, _PI]),
     "miq_row8_experts": (
-        C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _L, _I, _P]),
+        C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _L, _I, _P, C.c_size_t, _P]),
     "miq_experts_plan": (C.c_int, [_P, _P, _P, _P, _L, _I, _I, _I, _P]),
     "miq_experts_join": (C.c_int, [_P, _P, _P, _P, _P, _L, _L, _I, _I, _L, _L, _L, _I, _P]),
 }

@@ -2,7 +2,7 @@
 //
 // v = act(x), or act(gate) * up; m = max(max |v|, 2^-110); code = rint(v * (127 / m)), scale = m / 127.
 // A row stays in the registers of a wave or a workgroup: one read, one write.
-#include "row8_device.h"
+#include "row8_product.h"
 
 namespace miq {
 namespace {
@@ -162,6 +162,29 @@ __global__ __launch_bounds__(256) void row8_expand_kernel(Expand e, const int8_t
   }
 }
 
+// Rows of codes to rows of whole lines, 16 bytes a lane.
+struct Pad {
+  int64_t total, x_rows;  // lanes
+  int c, per_row;
+  FastDivM div;  // by per_row
+};
+__global__ __launch_bounds__(256) void row8_pad_kernel(Pad p, const int8_t* __restrict__ x, const int8_t* __restrict__ w,
+                                                       int8_t* __restrict__ to) {
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 256; base < p.total; base += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t lane = base + threadIdx.x;
+    if (lane >= p.total) continue;
+    const int64_t row0 = base / p.per_row;  // the workgroup's, one division
+    const int at = static_cast<int>(base - row0 * p.per_row) + static_cast<int>(threadIdx.x);
+    const int over = fdiv(at, p.div);
+    const int64_t row = row0 + over;
+    const int col = (at - over * p.per_row) * 16;
+    const int8_t* const from = row < p.x_rows ? x + row * p.c : w + (row - p.x_rows) * p.c;
+    const v4i v = col + 16 <= p.c ? load16<true>(from + col) : load_codes16(from, col, p.c);
+    reinterpret_cast<v4i*>(to)[lane] = v;
+    store_gap(v);
+  }
+}
+
 template <typename T, int ACT, bool GATED>
 void launch_act(const ActRow8Args& a, hipStream_t stream) {
   const RowShape shape = row_shape(a.c, kWide<T>, a.rows);
@@ -195,6 +218,20 @@ void by_act(const ActRow8Args& a, hipStream_t stream) {
 
 hipError_t launch_act_row8(const ActRow8Args& a, hipStream_t stream) {
   a.bf16 ? by_act<__bf16>(a, stream) : by_act<float>(a, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_row8_pad(const int8_t* x, int64_t x_rows, const int8_t* w, int64_t w_rows, int32_t c, int32_t width,
+                           int8_t* to, hipStream_t stream) {
+  Pad p{};
+  p.c = c;
+  p.x_rows = x_rows;
+  p.per_row = width / 16;
+  p.total = (x_rows + w_rows) * p.per_row;
+  p.div = fastdiv_m(static_cast<uint32_t>(p.per_row));
+  const int64_t blocks = (p.total + 255) / 256;
+  const unsigned grid = static_cast<unsigned>(blocks < (1 << 23) ? blocks : (1 << 23));
+  row8_pad_kernel<<<grid, 256, 0, stream>>>(p, x, w, to);
   return hipGetLastError();
 }
 

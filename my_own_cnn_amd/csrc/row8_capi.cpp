@@ -219,19 +219,31 @@ int miq_row8_expand(const int8_t* codes, const float* scales, void* y, int64_t r
   return done(miq::launch_row8_expand(a, static_cast<hipStream_t>(stream)));
 }
 
-int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]) {
+int miq_plan_row8_linear(int64_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[4]) {
   if (plan == nullptr) return null("plan pointer is NULL");
   const int st = check_product(rows, c, k, experts);
   if (st != MIQ_OK) return st;
-  plan[0] = plan[1] = plan[2] = 0;
+  plan[0] = plan[1] = plan[2] = plan[3] = 0;
   if (rows > 0 && k > 0) miq::plan_row8_linear(static_cast<int32_t>(rows), c, k, experts, plan);
+  return MIQ_OK;
+}
+
+int miq_row8_workspace_size(int64_t x_rows, int64_t rows, int32_t c, int32_t k, int32_t experts, size_t* bytes) {
+  if (bytes == nullptr) return null("bytes pointer is NULL");
+  const int st = check_product(rows, c, k, experts);
+  if (st != MIQ_OK) return st;
+  if (x_rows < 0 || x_rows > kMaxPositions) return bad("x_rows must lie in 0 .. 2^31 - 65");
+  *bytes = rows == 0 || k == 0 ? 0
+                               : miq::row8_workspace_bytes(static_cast<int32_t>(x_rows), static_cast<int32_t>(rows), c, k,
+                                                           experts);
   return MIQ_OK;
 }
 
 int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
                     const float* bias, const void* add, void* y, int64_t rows, int32_t c, int32_t k, int64_t ld_add,
-                    int64_t ld_y, int32_t type, void* stream) {
-  const int st = check_product(rows, c, k, 1);
+                    int64_t ld_y, int32_t type, void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  const int st = miq_row8_workspace_size(rows, rows, c, k, 1, &need);
   if (st != MIQ_OK) return st;
   if (!real_type(type)) return bad("type must be MIQ_F32 or MIQ_BF16");
   if (!stride_ok(ld_y, k) || (add != nullptr && !stride_ok(ld_add, k))) return bad(kShortRows);
@@ -240,9 +252,11 @@ int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_co
     return null("codes or scales pointer is NULL");
   }
   if (y == nullptr) return null("output pointer is NULL");
+  if (need > 0 && workspace == nullptr) return null("workspace pointer is NULL");
+  if (workspace_bytes < need) return bad("workspace is smaller than miq_row8_workspace_size reports");
   if (!aligned(scales, 4) || !aligned(w_scales, 4) || !aligned(bias, 4) || !aligned(add, size_of(type)) ||
-      !aligned(y, size_of(type))) {
-    return bad(kUnaligned);
+      !aligned(y, size_of(type)) || !aligned(workspace, 16)) {
+    return bad("a pointer is not aligned to its element, or the workspace to 16 bytes");
   }
   miq::Row8LinearArgs a{};
   a.x = codes;
@@ -252,6 +266,7 @@ int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_co
   a.bias = bias;
   a.add = add;
   a.y = y;
+  a.ws = workspace;
   a.ld_add = ld_add;
   a.ld_y = ld_y;
   a.x_rows = a.rows = static_cast<int32_t>(rows);
@@ -264,10 +279,11 @@ int miq_row8_linear(const int8_t* codes, const float* scales, const int8_t* w_co
 
 int miq_row8_experts(const int8_t* codes, const float* scales, const int8_t* w_codes, const float* w_scales,
                      const float* bias, const int32_t* offsets, const int32_t* index, void* y, int64_t x_rows,
-                     int64_t rows, int32_t c, int32_t k, int32_t experts, int64_t ld_y, int32_t type, void* stream) {
-  const int st = check_product(rows, c, k, experts);
+                     int64_t rows, int32_t c, int32_t k, int32_t experts, int64_t ld_y, int32_t type,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  const int st = miq_row8_workspace_size(x_rows, rows, c, k, experts, &need);
   if (st != MIQ_OK) return st;
-  if (x_rows < 0 || x_rows > kMaxPositions) return bad("x_rows must lie in 0 .. 2^31 - 65");
   if (index == nullptr && x_rows < rows) return bad("without an index x has as many rows as y");
   if (!real_type(type)) return bad("type must be MIQ_F32 or MIQ_BF16");
   if (!stride_ok(ld_y, k)) return bad(kShortRows);
@@ -278,9 +294,11 @@ int miq_row8_experts(const int8_t* codes, const float* scales, const int8_t* w_c
     return null("codes or scales pointer is NULL");
   }
   if (y == nullptr) return null("output pointer is NULL");
+  if (need > 0 && workspace == nullptr) return null("workspace pointer is NULL");
+  if (workspace_bytes < need) return bad("workspace is smaller than miq_row8_workspace_size reports");
   if (!aligned(scales, 4) || !aligned(w_scales, 4) || !aligned(bias, 4) || !aligned(offsets, 4) || !aligned(index, 4) ||
-      !aligned(y, size_of(type))) {
-    return bad(kUnaligned);
+      !aligned(y, size_of(type)) || !aligned(workspace, 16)) {
+    return bad("a pointer is not aligned to its element, or the workspace to 16 bytes");
   }
   miq::Row8LinearArgs a{};
   a.x = codes;
@@ -291,6 +309,7 @@ int miq_row8_experts(const int8_t* codes, const float* scales, const int8_t* w_c
   a.offsets = offsets;
   a.index = index;
   a.y = y;
+  a.ws = workspace;
   a.ld_y = ld_y;
   a.x_rows = static_cast<int32_t>(x_rows);
   a.rows = static_cast<int32_t>(rows);

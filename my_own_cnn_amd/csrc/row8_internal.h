@@ -73,14 +73,20 @@ struct Row8LinearArgs {
   const int32_t* offsets;
   const int32_t* index;
   void* y;
+  void* ws;  // of row8_workspace_bytes
   int64_t ld_add, ld_y;
   int32_t x_rows, rows, c, k, experts;
   bool bf16;
 };
 hipError_t launch_row8_few(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream);
 hipError_t launch_row8_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream);
-// plan: whether the weights go straight to the matrix instructions (few rows), and a tile's rows and channels.
-void plan_row8_linear(int32_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]);
+// Two tensors' rows of c codes to rows of `width`, the rest zeros: x's, then w's.
+hipError_t launch_row8_pad(const int8_t* x, int64_t x_rows, const int8_t* w, int64_t w_rows, int32_t c, int32_t width,
+                           int8_t* to, hipStream_t stream);
+// plan: whether the weights go straight to the matrix instructions (few rows), a tile's rows and channels, whether
+// rows are first copied to the workspace.
+void plan_row8_linear(int32_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[4]);
+size_t row8_workspace_bytes(int32_t x_rows, int32_t rows, int32_t c, int32_t k, int32_t experts);
 hipError_t launch_row8_linear(const Row8LinearArgs& a, hipStream_t stream);
 
 struct ExpertsPlanArgs {

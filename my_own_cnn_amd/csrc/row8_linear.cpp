@@ -12,23 +12,25 @@ namespace miq {
 namespace {
 
 struct Shape {
-  bool few;
+  bool few, pad;
   int rows, channels;
 };
 
-// Tiles through LDS: us for a step of 64 codes of one workgroup that has its CU for itself, and of a CU that
+// Tiles through LDS: us for a step of 128 codes of one workgroup that has its CU for itself, and of a CU that
 // has many; us for a tile's output.
 struct Tile {
   int rows, channels;
   double alone, each, output;
 };
-constexpr Tile kTiles[] = {{64, 64, 0.18, 0.13, 0.4},
-                           {64, 128, 0.205, 0.21, 0.7},
-                           {128, 128, 0.24, 0.31, 1.3},
-                           {128, 256, 0.36, 0.57, 2.5},
-                           {256, 256, 0.55, 0.84, 7}};
-// Rows that do not start on 16 bytes go through registers.
-constexpr double kThroughRegisters = 1.5;
+constexpr Tile kTiles[] = {{64, 64, 0.17, 0.19, 0.4},
+                           {64, 128, 0.275, 0.31, 0.7},
+                           {128, 128, 0.44, 0.5, 1.3},
+                           {128, 256, 0.61, 0.94, 2.5},
+                           {256, 256, 1.1, 1.5, 7}};
+// Rows that do not start on 16 bytes go through registers, or are first copied to rows of whole lines in the
+// workspace, which takes a launch and moves them twice: 1003 x 2051 x 1537 19.7 us and 15, 8192 x 8193 x 8192
+// 809 and 500.
+constexpr double kThroughRegisters = 2.5, kCopy = 3, kCopyRate = 3.2e6;
 // Few rows: bound by what a CU takes in, 38 KB a us (21 where rows do not start on 4 bytes); us for a tile's
 // sums beyond the first two of a CU.
 struct Few {
@@ -38,7 +40,7 @@ struct Few {
 constexpr Few kFew[] = {{16, 16, 0.7}, {16, 32, 1.4}, {32, 16, 0.85}, {32, 32, 1.1}, {64, 32, 2.6}};
 constexpr double kIntake = 38e3, kOddIntake = 21e3, kLaunch = 3.5;
 
-Shape shape_of(int64_t rows, int64_t c, int64_t k, int64_t experts) {
+Shape shape_of(int64_t x_rows, int64_t rows, int64_t c, int64_t k, int64_t experts) {
   const auto over = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
   // experts: as if all that can have rows had as many
   const int64_t groups = std::min(rows, experts), part = over(rows, groups);
@@ -56,33 +58,59 @@ Shape shape_of(int64_t rows, int64_t c, int64_t k, int64_t experts) {
   for (const Few& t : kFew) {
     const int64_t tiles = groups * over(part, t.rows) * over(k, t.channels), rounds = over(tiles, 256);
     const double in = static_cast<double>(std::min<int64_t>(part, t.rows) + t.channels) * c;
-    take({true, t.rows, t.channels},
+    take({true, false, t.rows, t.channels},
          kLaunch + rounds * in / (c % 4 == 0 ? kIntake : kOddIntake) + std::max<int64_t>(rounds - 2, 0) * t.sums);
   }
-  const double steps = static_cast<double>(over(c, 64)) * (c % 16 == 0 ? 1.0 : kThroughRegisters);
+  if (c < 16) return best;
+  const double steps = static_cast<double>(over(c, 128));
+  const double copied = 2.0 * (x_rows + static_cast<double>(experts) * k) * c;
   for (const Tile& t : kTiles) {
-    if (c < 16 || (t.rows == 256 && c % 16 != 0)) continue;
     // of experts the last row tile is half full
     const double high = groups == 1 ? over(part, t.rows) : std::max(1.0, static_cast<double>(part) / t.rows + 0.5);
-    const int64_t tiles = static_cast<int64_t>(groups * high) * over(k, t.channels), rounds = over(tiles, 256);
-    take({false, t.rows, t.channels}, kLaunch + steps * std::max(t.alone, t.each * rounds) + t.output * rounds);
+    const int64_t rounds = over(static_cast<int64_t>(groups * high) * over(k, t.channels), 256);
+    const double each = steps * std::max(t.alone, t.each * rounds), rest = kLaunch + t.output * rounds;
+    if (c % 16 == 0) {
+      take({false, false, t.rows, t.channels}, each + rest);
+    } else {
+      if (t.rows != 256) take({false, false, t.rows, t.channels}, kThroughRegisters * each + rest);
+      take({false, true, t.rows, t.channels}, each + rest + kCopy + copied / kCopyRate);
+    }
   }
   return best;
 }
 
+// Codes of a copied row.
+int64_t padded(int64_t c) { return (c + 127) / 128 * 128; }
+
 }  // namespace
 
-void plan_row8_linear(int32_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[3]) {
-  const Shape s = shape_of(rows, c, k, experts);
+void plan_row8_linear(int32_t rows, int32_t c, int32_t k, int32_t experts, int32_t plan[4]) {
+  const Shape s = shape_of(rows, rows, c, k, experts);
   plan[0] = s.few;
   plan[1] = s.rows;
   plan[2] = s.channels;
+  plan[3] = s.pad;
+}
+
+size_t row8_workspace_bytes(int32_t x_rows, int32_t rows, int32_t c, int32_t k, int32_t experts) {
+  if (x_rows == 0 || !shape_of(x_rows, rows, c, k, experts).pad) return 0;
+  return static_cast<size_t>((x_rows + static_cast<int64_t>(experts) * k) * padded(c));
 }
 
 hipError_t launch_row8_linear(const Row8LinearArgs& a, hipStream_t stream) {
   Row8LinearArgs b = a;
   if (b.x_rows == 0) b.c = 0;  // every row stands for zeros
-  const Shape s = shape_of(b.rows, b.c, b.k, b.experts);
+  const Shape s = shape_of(b.x_rows, b.rows, b.c, b.k, b.experts);
+  if (s.pad) {
+    const int64_t weights = static_cast<int64_t>(b.experts) * b.k;
+    int8_t* const to = static_cast<int8_t*>(a.ws);
+    const int32_t width = static_cast<int32_t>(padded(a.c));
+    const hipError_t e = launch_row8_pad(a.x, a.x_rows, a.w, weights, a.c, width, to, stream);
+    if (e != hipSuccess) return e;
+    b.x = to;
+    b.w = to + static_cast<int64_t>(a.x_rows) * width;
+    b.c = width;
+  }
   return s.few ? launch_row8_few(b, s.rows, s.channels, stream) : launch_row8_tile(b, s.rows, s.channels, stream);
 }
 

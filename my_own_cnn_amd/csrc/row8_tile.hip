@@ -1,10 +1,10 @@
 // Products of 8-bit rows with 8-bit weights in tiles held by LDS (row8_linear.cpp has the formula).
 //
-// A workgroup computes BM rows by BN channels of y, 64 codes of the reduction a step.  Both operands lie
-// in LDS as rows of 64 bytes, STAGES steps of them; a step's bytes travel straight from global memory to
-// LDS (DMA; through registers where rows do not start on 16 bytes), two or more steps ahead.  A wave
-// reads the fragments of the next step while its matrix instructions run on this one's, so one barrier a
-// step is all that a wave waits for.
+// A workgroup computes BM rows by BN channels of y, 128 codes of the reduction a step: whole lines of the
+// caches.  Both operands lie in LDS as rows of 128 bytes, STAGES steps of them; a step's bytes travel
+// straight from global memory to LDS (DMA), or, where rows do not start on 16 bytes, through registers.  A
+// wave reads the fragments of the next half step while its matrix instructions run on this half, and meets
+// the others once a step.
 #include <algorithm>
 
 #include "row8_product.h"
@@ -12,19 +12,16 @@
 namespace miq {
 namespace {
 
-constexpr int kStep = 64;  // codes, and bytes of a row of LDS
+constexpr int kStep = 128;  // codes, and bytes of a row of LDS
 
 struct Tiling {
   int from, high, wide;  // the launch's first row tile and their number (the most, of experts), channel tiles
 };
 
 // The 16-byte units of a row of LDS are permuted by its number: an LDS read serves in one cycle the lanes
-// 0-3, 12-15, 20-23, 24-27 of a half-wave or the other 16, that is rows 0-3 and 12-15 at one unit and 4-11
-// at the next one, or the other way round, and these lie in different banks.
-__device__ __forceinline__ int unit(int row, int at) {
-  const int g = (row >> 2) & 3;
-  return at ^ (((g ^ (g >> 1)) & 1) << 1 | g >> 1);
-}
+// 0-3, 12-15, 20-23, 24-27 of a half-wave or the other 16, that is of a fragment the rows 0-3 and 12-15 at one
+// unit and 4-11 at the next one, or the other way round, and these lie in different banks.
+__device__ __forceinline__ int unit(int row, int at) { return at ^ ((row >> 1) & 7); }
 
 // The channel in row p of LDS.  Matrix instruction f of a group of 64 rows of LDS leaves its rows 4q .. 4q + 3
 // in lane group q: for 16-byte stores whose four lanes lie side by side a lane's channels are 8q .. 8q + 7 of
@@ -60,12 +57,12 @@ __device__ __forceinline__ int row_tiles(const Row8LinearArgs& a, const Tiling& 
 }
 
 template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 : 2) void row8_tile_kernel(Row8LinearArgs a, Tiling tiling) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void row8_tile_kernel(Row8LinearArgs a, Tiling tiling) {
   constexpr int kWaves = WM * WN;
-  constexpr int NX = BM / 16 / kWaves, NW = BN / 16 / kWaves;  // runs of 16 rows that a wave stages
+  constexpr int NX = BM / 8 / kWaves, NW = BN / 8 / kWaves;  // runs of 8 rows that a wave stages
   constexpr int kStage = (BM + BN) * kStep;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;  // a wave's fragments
-  static_assert(NX >= 1 && NW >= 1 && FN % 2 == 0, "whole runs and groups of 32 channels");
+  static_assert(NX >= 1 && NW >= 1 && FN % 2 == 0 && (DMA || STAGES == 2), "whole runs and groups of 32 channels");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -73,9 +70,7 @@ __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 :
   if (static_cast<int>(blockIdx.x) >= high * tiling.wide) return;
   const Place place = place_of<BM, BN>(a, tiling, high, blockIdx.x);
   const RowTile r = place.r;
-  const int n0 = place.n0;
-  const int rows = r.end - r.row0, channels = min(BN, a.k - n0);
-  const int64_t w_at = (static_cast<int64_t>(r.expert) * a.k + n0) * a.c;
+  const int n0 = place.n0, rows = r.end - r.row0, channels = min(BN, a.k - n0);
 
   // The output stage takes U runs of a lane's channels of each row, W values each.  Its scales are loaded first,
   // where registers are left for them.
@@ -100,13 +95,12 @@ __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 :
   };
   if constexpr (kEarly) load_scales();
 
-  // A wave's runs: lane l stages unit l & 3 of row l >> 2 of each.  Rows and channels beyond the tile's read
-  // another's or zeros: they reach no sum that is stored.
-  const int s_row = lane >> 2;
+  // A wave's runs: lane l stages one unit of row l >> 3 of each.  Rows and channels beyond the tile's read
+  // another's: they reach no sum that is stored.
   int x_row[NX], w_row[NW];
 #pragma unroll
   for (int i = 0; i < NX; ++i) {
-    const int row = (wave * NX + i) * 16 + s_row;
+    const int row = (wave * NX + i) * 8 + (lane >> 3);
     x_row[i] = row < rows ? row : 0;
     if (a.index != nullptr) {
       const int from = a.index[r.row0 + x_row[i]];
@@ -114,24 +108,27 @@ __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 :
     }
   }
 #pragma unroll
-  for (int i = 0; i < NW; ++i) w_row[i] = min(channel_of<T>((wave * NW + i) * 16 + s_row), channels - 1);
+  for (int i = 0; i < NW; ++i) w_row[i] = min(channel_of<T>((wave * NW + i) * 8 + (lane >> 3)), channels - 1);
   const int8_t* const x_base = a.index != nullptr ? a.x : a.x + static_cast<int64_t>(r.row0) * a.c;
-  const int8_t* const w_base = a.w + w_at;
+  const int8_t* const w_base = a.w + (w_of0 + n0) * a.c;
   const int steps = (a.c + kStep - 1) / kStep;
+  // the lane's channel in run i: its rows are 8i .. 8i + 7
+  auto run_at = [&](int i) { return unit(i * 8 + (lane >> 3), lane & 7) * 16; };
 
   // DMA: offsets of a wave's runs; past the tensor's end they read zeros.
   unsigned x_of[NX], w_of[NW];
   __amdgpu_buffer_rsrc_t x_rsrc, w_rsrc;
-  // registers: where a wave's runs start, and two steps of them on their way
+  // registers: where a wave's runs start, and a step of them on its way
   const int8_t* x_from[NX];
   const int8_t* w_from[NW];
-  v4i x_set[2][NX], w_set[2][NW];
-  const int s_at = unit(s_row, lane & 3) * 16;
+  v4i x_set[NX], w_set[NW];
   if constexpr (DMA) {
 #pragma unroll
-    for (int i = 0; i < NX; ++i) x_of[i] = static_cast<unsigned>(x_row[i]) * static_cast<unsigned>(a.c) + s_at;
+    for (int i = 0; i < NX; ++i)
+      x_of[i] = static_cast<unsigned>(x_row[i]) * static_cast<unsigned>(a.c) + run_at(wave * NX + i);
 #pragma unroll
-    for (int i = 0; i < NW; ++i) w_of[i] = static_cast<unsigned>(w_row[i]) * static_cast<unsigned>(a.c) + s_at;
+    for (int i = 0; i < NW; ++i)
+      w_of[i] = static_cast<unsigned>(w_row[i]) * static_cast<unsigned>(a.c) + run_at(wave * NW + i);
     x_rsrc = make_rsrc(x_base, static_cast<int>(static_cast<unsigned>(a.index != nullptr ? a.x_rows : rows) *
                                                 static_cast<unsigned>(a.c)));
     w_rsrc = make_rsrc(w_base, channels * a.c);
@@ -151,114 +148,112 @@ __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 :
     for (int i = 0; i < NW; ++i)
       load_lds16(w_rsrc, reinterpret_cast<v4i*>(to + BM * kStep + (wave * NW + i) * 1024), w_of[i], k);
   };
-  auto load = [&](int step, int set) {
-    const int k = min(step, steps - 1) * kStep + s_at;
+  auto load = [&](int step) {
+    const int k = min(step, steps - 1) * kStep;
     if (step < steps - 1) {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) x_set[set][i] = load16<false>(x_from[i] + k);
+      for (int i = 0; i < NX; ++i) x_set[i] = load16<false>(x_from[i] + k + run_at(wave * NX + i));
 #pragma unroll
-      for (int i = 0; i < NW; ++i) w_set[set][i] = load16<false>(w_from[i] + k);
+      for (int i = 0; i < NW; ++i) w_set[i] = load16<false>(w_from[i] + k + run_at(wave * NW + i));
     } else {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) x_set[set][i] = load_codes16(x_from[i], k, a.c);
+      for (int i = 0; i < NX; ++i) x_set[i] = load_codes16(x_from[i], k + run_at(wave * NX + i), a.c);
 #pragma unroll
-      for (int i = 0; i < NW; ++i) w_set[set][i] = load_codes16(w_from[i], k, a.c);
+      for (int i = 0; i < NW; ++i) w_set[i] = load_codes16(w_from[i], k + run_at(wave * NW + i), a.c);
     }
   };
-  auto write = [&](int set, int buffer) {
+  auto write = [&](int buffer) {
     char* const to = lds + buffer * kStage + lane * 16;
 #pragma unroll
-    for (int i = 0; i < NX; ++i) *reinterpret_cast<v4i*>(to + (wave * NX + i) * 1024) = x_set[set][i];
+    for (int i = 0; i < NX; ++i) *reinterpret_cast<v4i*>(to + (wave * NX + i) * 1024) = x_set[i];
 #pragma unroll
-    for (int i = 0; i < NW; ++i) *reinterpret_cast<v4i*>(to + BM * kStep + (wave * NW + i) * 1024) = w_set[set][i];
+    for (int i = 0; i < NW; ++i) *reinterpret_cast<v4i*>(to + BM * kStep + (wave * NW + i) * 1024) = w_set[i];
   };
 
   typedef __attribute__((address_space(3))) const char lds_char;
   typedef __attribute__((address_space(3))) const v4i lds_v4i;
-  lds_char* const f_from = (lds_char*)lds + f_row * kStep + unit(f_row, f_at) * 16;  // an address-space cast
-  lds_char* const x_part = f_from + wm * FM * 1024;
-  lds_char* const w_part = f_from + BM * kStep + wn * FN * 1024;
+  lds_char* f_from[2];  // of a half step
+#pragma unroll
+  for (int h = 0; h < 2; ++h) f_from[h] = (lds_char*)lds + f_row * kStep + unit(f_row, 4 * h + f_at) * 16;  // an address-space cast
   v4i fx[2][FM], fw[2][FN];
-  auto read = [&](int buffer, int set) {
-    lds_char* const x = x_part + buffer * kStage;
-    lds_char* const w = w_part + buffer * kStage;
+  auto read = [&](int buffer, int half) {
+    lds_char* const x = f_from[half] + wm * FM * 16 * kStep + buffer * kStage;
+    lds_char* const w = f_from[half] + BM * kStep + wn * FN * 16 * kStep + buffer * kStage;
 #pragma unroll
-    for (int i = 0; i < FN; ++i) fw[set][i] = *reinterpret_cast<lds_v4i*>(w + i * 1024);
+    for (int i = 0; i < FN; ++i) fw[half][i] = *reinterpret_cast<lds_v4i*>(w + i * 16 * kStep);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fx[set][i] = *reinterpret_cast<lds_v4i*>(x + i * 1024);
+    for (int i = 0; i < FM; ++i) fx[half][i] = *reinterpret_cast<lds_v4i*>(x + i * 16 * kStep);
   };
   v4i acc[FN][FM] = {};
-  auto multiply = [&](int set) {
+  auto multiply = [&](int half) {
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
       for (int j = 0; j < FM; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[set][i], fx[set][j], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[half][i], fx[half][j], acc[i][j], 0, 0, 0);
   };
-
-  // Step t multiplies the fragments read in step t - 1 and reads those of t + 1.  Past the last step the
-  // loads and reads repeat it.
-  // DMA: it starts the loads of t + STAGES - 1 into the buffer of t - 1, which every wave has read before the
-  // step's barrier; before the barrier a wave waits for its own loads of t + 1, and the STAGES - 3 steps
-  // after that stay in flight.
-  // Registers: at its end it writes t + 2, in place of t - 2, and loads t + 4.
-  constexpr int kLoads = NX + NW;
-  static_assert(STAGES == 4 && (STAGES - 2) * kLoads <= 15, "the buffers' numbers, and the counter's bits in use");
-  int now = 0;  // buffer of step t
-  if constexpr (DMA) {
+  // a read or a load after each matrix instruction
+  auto mix = [&]() {
+    if constexpr (DMA) {
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) stage(i, i);
-    wait_vmcnt((STAGES - 2) * kLoads);
-    barrier_only();
-  } else {
-    load(0, 0);
-    load(1, 1);
-    write(0, 0);
-    write(1, 1);
-    load(2, 0);
-    load(3, 1);
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    barrier_only();
-  }
-  read(0, 0);
-  auto step = [&](int t, int set) {
-    if constexpr (DMA) wait_vmcnt((STAGES - 3) * kLoads);
-    else __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): its writes of t + 1
-    barrier_only();
-    if constexpr (DMA) stage(t + STAGES - 1, now == 0 ? STAGES - 1 : now - 1);
-    now = now + 1 == STAGES ? 0 : now + 1;
-    read(now, set ^ 1);
-    multiply(set);
-    // a read or a load after each matrix instruction
-#pragma unroll
-    for (int i = 0; i < FN * FM; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // matrix
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);            // LDS reads
-      if constexpr (DMA) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // loads
+      for (int i = 0; i < FN * FM; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS reads
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // loads
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (!DMA) {
-      write(set, now + 1 == STAGES ? 0 : now + 1);
-      load(t + 4, set);
-    }
   };
-  int t = 0;
-  for (; t + 2 < steps; t += 2) {
-    step(t, 0);
-    step(t + 1, 1);
+
+  // The middle of step t is where the waves meet: each has read all of its buffer, so the loads of step t +
+  // STAGES (registers: the values of t + 2, loaded a step ago) go into it, and each has its part of t + 1 in
+  // LDS, so the fragments of that can be read.  STAGES - 2 steps stay in flight.  Past the last step the
+  // loads repeat it.
+  constexpr int kLoads = NX + NW;
+  static_assert((STAGES - 1) * kLoads <= 63, "the counter has 6 bits");
+  if constexpr (DMA) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) stage(i, i);
+    wait_vmcnt63((STAGES - 1) * kLoads);
+  } else {
+    load(0);
+    write(0);
+    load(1);
+    write(1);
+    load(2);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
   }
-  if (t + 1 < steps) {
-    step(t, 0);
-#pragma unroll
-    for (int j = 0; j < FM; ++j) fx[0][j] = fx[1][j];
-#pragma unroll
-    for (int i = 0; i < FN; ++i) fw[0][i] = fw[1][i];
+  barrier_only();
+  read(0, 0);
+  int now = 0;  // buffer of step t
+  for (int t = 0; t + 1 < steps; ++t) {
+    const int next = now + 1 == STAGES ? 0 : now + 1;
+    read(now, 1);
+    multiply(0);
+    mix();
+    if constexpr (DMA) wait_vmcnt63((STAGES - 2) * kLoads);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    barrier_only();
+    if constexpr (DMA) {
+      stage(t + STAGES, now);
+    } else {
+      write(now);
+      load(t + 3);
+    }
+    read(next, 0);
+    multiply(1);
+    mix();
+    now = next;
   }
   // the last step: codes past the rows' end do not count
-  const bool there = (steps - 1) * kStep + f_at * 16 < a.c;
+  read(now, 1);
 #pragma unroll
-  for (int j = 0; j < FM; ++j) fx[0][j] = there ? fx[0][j] : v4i{};
-  multiply(0);
+  for (int h = 0; h < 2; ++h) {
+    const bool there = (steps - 1) * kStep + (4 * h + f_at) * 16 < a.c;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) fx[h][j] = there ? fx[h][j] : v4i{};
+    multiply(h);
+  }
   wait_vmcnt(0);  // no load into LDS outlives the workgroup
 
   if constexpr (!kEarly) load_scales();
@@ -283,13 +278,10 @@ __global__ __launch_bounds__(WM* WN * 64, BM / WM * (BN / WN) >= 128 * 128 ? 1 :
   }
 }
 
-template <typename T, bool DMA, int BM, int BN, int WM, int WN>
-hipError_t launch(const Row8LinearArgs& a, hipStream_t stream) {
-  constexpr int kStages = 4, kSize = kStages * (BM + BN) * kStep;
-  const int wide = (a.k + BN - 1) / BN;
-  const int64_t high = a.offsets != nullptr ? most_tiles(a.rows, a.experts, BM)
-                                            : (static_cast<int64_t>(a.rows) + BM - 1) / BM;
-  auto* const kernel = row8_tile_kernel<T, DMA, BM, BN, WM, WN, kStages>;
+template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES>
+hipError_t launch(const Row8LinearArgs& a, int wide, int64_t high, hipStream_t stream) {
+  constexpr int kSize = STAGES * (BM + BN) * kStep;
+  auto* const kernel = row8_tile_kernel<T, DMA, BM, BN, WM, WN, STAGES>;
   if (kSize > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kSize);
@@ -307,16 +299,29 @@ hipError_t launch(const Row8LinearArgs& a, hipStream_t stream) {
 
 template <typename T, bool DMA>
 hipError_t by_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream) {
+  const int wide = (a.k + channels - 1) / channels;
+  const int64_t high = a.offsets != nullptr ? most_tiles(a.rows, a.experts, rows)
+                                            : (static_cast<int64_t>(a.rows) + rows - 1) / rows;
   if constexpr (DMA) {
-    // two steps of it in registers spill: 128 x 256 where they would be
-    if (rows == 256) return launch<T, DMA, 256, 256, 2, 4>(a, stream);
+    // Few tiles: as many steps in flight as LDS holds for the one or two workgroups of a CU.
+    const bool few = high * wide <= 512, one = high * wide <= 256;
+    if (rows == 256) return launch<T, DMA, 256, 256, 2, 4, 2>(a, wide, high, stream);
+    if (rows == 128 && channels == 256) return launch<T, DMA, 128, 256, 2, 4, 3>(a, wide, high, stream);
+    if (rows == 128 && one) return launch<T, DMA, 128, 128, 2, 2, 4>(a, wide, high, stream);
+    if (rows == 128) return launch<T, DMA, 128, 128, 2, 2, 2>(a, wide, high, stream);
+    if (channels == 128 && few) return launch<T, DMA, 64, 128, 2, 2, 3>(a, wide, high, stream);
+    if (channels == 128) return launch<T, DMA, 64, 128, 2, 2, 2>(a, wide, high, stream);
+    if (few) return launch<T, DMA, 64, 64, 2, 2, 4>(a, wide, high, stream);
+    return launch<T, DMA, 64, 64, 2, 2, 2>(a, wide, high, stream);
+  } else {
+    if (rows == 64 && channels == 64) return launch<T, DMA, 64, 64, 2, 2, 2>(a, wide, high, stream);
+    if (rows == 64) return launch<T, DMA, 64, 128, 2, 2, 2>(a, wide, high, stream);
+    if (channels == 128) return launch<T, DMA, 128, 128, 2, 2, 2>(a, wide, high, stream);
+    // (256 rows would spill)
+    return launch<T, DMA, 128, 256, 2, 4, 2>(a, (a.k + 255) / 256,
+                                                a.offsets != nullptr ? most_tiles(a.rows, a.experts, 128)
+                                                                     : (static_cast<int64_t>(a.rows) + 127) / 128, stream);
   }
-  if (rows == 64) {
-    if (channels == 64) return launch<T, DMA, 64, 64, 2, 2>(a, stream);
-    return launch<T, DMA, 64, 128, 2, 2>(a, stream);
-  }
-  if (channels == 128) return launch<T, DMA, 128, 128, 2, 2>(a, stream);
-  return launch<T, DMA, 128, 256, 2, 4>(a, stream);
 }
 
 template <typename T>
@@ -326,7 +331,7 @@ hipError_t by_way(const Row8LinearArgs& a, int rows, int channels, hipStream_t s
     return by_tile<T, true>(a, rows, channels, stream);
   }
   // Through registers a load from an odd address costs less than the second load and the shifts that few rows
-  // take (1003 x 2051 x 1537: 20 us and 30).
+  // take.
   return by_tile<T, false>(a, rows, channels, stream);
 }
 

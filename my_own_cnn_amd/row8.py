@@ -243,17 +243,28 @@ def row8_expand(x: Row8, *, dtype=None, out=None, stream=None):
 # ---- products ---------------------------------------------------------------------------------------
 
 def plan_row8_linear(rows: int, c: int, k: int, experts: int = 1):
-    """(few, rows, channels) of row8_linear and, with `experts`, row8_experts: whether the weights go
-    straight to the matrix instructions, and a tile's rows and channels (no GPU access)."""
-    out = (C.c_int32 * 3)()
+    """(few, rows, channels, copied) of row8_linear and, with `experts`, row8_experts on as many rows:
+    whether the weights go straight to the matrix instructions, a tile's rows and channels, and
+    whether rows of codes are first copied to the workspace (no GPU access)."""
+    out = (C.c_int32 * 4)()
     check(lib().miq_plan_row8_linear(rows, c, k, experts, out), "plan_row8_linear")
-    return bool(out[0]), out[1], out[2]
+    return bool(out[0]), out[1], out[2], bool(out[3])
 
 
-def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, stream=None):
+def row8_workspace_size(x_rows: int, rows: int, c: int, k: int, experts: int = 1) -> int:
+    """Bytes of device workspace row8_linear(..., workspace=...) (x_rows == rows) and, with `experts`,
+    row8_experts need: 0 wherever c is a multiple of 16, and for few rows (no GPU access)."""
+    out = C.c_size_t()
+    check(lib().miq_row8_workspace_size(x_rows, rows, c, k, experts, C.byref(out)), "row8_workspace_size")
+    return out.value
+
+
+def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, workspace=None, stream=None):
     """A linear layer of 8-bit rows x (..., C) by 8-bit weights w (K, C): the exact int8 product times the
     row's and the channel's scale, plus `bias` (K,), float32, plus `add` (..., K), of the result's
-    type; (..., K), float32 or bfloat16 (`dtype`, default bfloat16).  `out` may be `add`."""
+    type; (..., K), float32 or bfloat16 (`dtype`, default bfloat16).  `out` may be `add`.
+    `workspace`: a device buffer of at least row8_workspace_size() bytes, not used by another call in
+    flight; None allocates one from PyTorch for this call where it needs one."""
     shape = _row8(x, "x")
     w_shape = _row8(w, "w")
     c = shape[-1]
@@ -276,9 +287,13 @@ def row8_linear(x: Row8, w: Row8, *, bias=None, add=None, dtype=None, out=None, 
         y, ld_y, handle = codes.new_empty(y_shape, dtype=dtype), k, _raw_stream(codes.get_device())
     else:
         (y, ld_y), handle = _output(out, y_shape, dtype, codes, stream), _handle(codes, stream)
+    rows = scales.numel()
+    at, size, held = None, 0, None
+    if c % 16:
+        at, size, held = _workspace(workspace, "miq_row8_workspace_size", (rows, rows, c, k, 1), codes.device, stream)
     status = lib().miq_row8_linear(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(),
-                                   None if bias is None else _f32_of(bias, (k,), "bias"), add_at, y.data_ptr(),
-                                   scales.numel(), c, k, ld_add, ld_y, kind, handle)
+                                   None if bias is None else _f32_of(bias, (k,), "bias"), add_at, y.data_ptr(), rows, c,
+                                   k, ld_add, ld_y, kind, at, size, handle)
     if status:
         check(status, "row8_linear")
     return y
@@ -311,12 +326,14 @@ def experts_plan(ids, experts: int, *, stream=None) -> ExpertsPlan:
     return _MAKE(ExpertsPlan, (offsets, rows, places))
 
 
-def row8_experts(x: Row8, w: Row8, offsets, *, rows=None, bias=None, dtype=None, out=None, stream=None):
+def row8_experts(x: Row8, w: Row8, offsets, *, rows=None, bias=None, dtype=None, out=None, workspace=None,
+                 stream=None):
     """row8_linear by experts: rows offsets[e] .. offsets[e + 1] - 1 of the result by the weights w[e] of
     w (experts, K, C) and bias (experts, K).  Row i takes row rows[i] of x (N, C), or row i without
     `rows`; an entry of `rows` outside x stands for a row of zeros.  offsets (experts + 1,) and
     `rows` are int32 tensors on the device, as experts_plan gives them; offsets rise and end within
-    the rows.  Rows of the result behind the last expert's are not written."""
+    the rows.  Rows of the result behind the last expert's are not written.  `workspace`: as of
+    row8_linear."""
     shape = _row8(x, "x")
     w_shape = _row8(w, "w")
     if len(shape) != 2:
@@ -343,9 +360,12 @@ def row8_experts(x: Row8, w: Row8, offsets, *, rows=None, bias=None, dtype=None,
         y, ld_y, handle = codes.new_empty((n, k), dtype=dtype), k, _raw_stream(codes.get_device())
     else:
         (y, ld_y), handle = _output(out, (n, k), dtype, codes, stream), _handle(codes, stream)
+    at, size, held = None, 0, None
+    if c % 16:
+        at, size, held = _workspace(workspace, "miq_row8_workspace_size", (x_rows, n, c, k, experts), codes.device, stream)
     status = lib().miq_row8_experts(codes.data_ptr(), scales.data_ptr(), w[0].data_ptr(), w[1].data_ptr(),
                                     None if bias is None else _f32_of(bias, (experts, k), "bias"), offsets_at, rows_at,
-                                    y.data_ptr(), x_rows, n, c, k, experts, ld_y, kind, handle)
+                                    y.data_ptr(), x_rows, n, c, k, experts, ld_y, kind, at, size, handle)
     if status:
         check(status, "row8_experts")
     return y
@@ -380,4 +400,5 @@ def experts_join(y, places, share=None, *, add=None, out=None, stream=None):
 
 
 __all__ = ["ExpertsPlan", "Row8", "act_row8", "experts_join", "experts_plan", "plan_row8_linear", "rms_bprop",
-           "rms_bprop_workspace_size", "rms_fprop", "rms_row8", "row8_expand", "row8_experts", "row8_linear"]
+           "rms_bprop_workspace_size", "rms_fprop", "rms_row8", "row8_expand", "row8_experts", "row8_linear",
+           "row8_workspace_size"]

@@ -8,22 +8,57 @@ import my_own_cnn_amd as M
 
 F32, BF16 = torch.float32, torch.bfloat16
 
-# rows, c, k, experts and the (few rows?, tile) that the plan gives them
+# rows, c, k, experts and what the plan gives them: few rows?, a tile, rows copied first?  Few tiles and many.
 CASES = [
-    (3, 80, 50, 1, (True, 16, 16)), (3, 84, 50, 1, (True, 16, 16)), (3, 83, 50, 1, (True, 16, 16)),
-    (3, 9, 50, 1, (True, 16, 16)), (5, 4112, 33, 4, (True, 16, 16)),
-    (5, 64, 1033, 4, (True, 16, 32)), (1, 68, 4100, 1, (True, 16, 32)), (1, 67, 4101, 1, (True, 16, 32)),
-    (100, 64, 520, 4, (True, 32, 16)), (20, 68, 2050, 1, (True, 32, 16)), (20, 67, 2051, 1, (True, 32, 16)),
-    (200, 64, 520, 4, (True, 32, 32)), (20, 68, 4097, 1, (True, 32, 32)), (20, 67, 4100, 1, (True, 32, 32)),
-    (130, 64, 1030, 4, (True, 64, 32)), (33, 68, 4100, 1, (True, 64, 32)), (33, 67, 4099, 1, (True, 64, 32)),
-    (8200, 64, 130, 1, (False, 64, 64)), (5, 80, 8200, 4, (False, 64, 64)), (5, 68, 8201, 4, (False, 64, 64)),
-    (8200, 67, 130, 1, (False, 64, 64)),
-    (1, 64, 16400, 1, (False, 64, 128)), (5, 112, 4100, 4, (False, 64, 128)), (50, 68, 4099, 4, (False, 64, 128)),
-    (5, 67, 4100, 4, (False, 64, 128)),
-    (400, 80, 6150, 4, (False, 128, 128)), (200, 68, 8201, 1, (False, 128, 128)), (257, 67, 6150, 4, (False, 128, 128)),
-    (200, 656, 16397, 1, (False, 128, 256)), (700, 80, 8199, 4, (False, 128, 256)), (700, 68, 8200, 4, (False, 128, 256)),
-    (700, 67, 8200, 4, (False, 128, 256)),
-    (700, 656, 16397, 1, (False, 256, 256)), (1500, 592, 8200, 2, (False, 256, 256)),
+    (3, 80, 50, 1, (True, 16, 16, False)),
+    (3, 84, 50, 1, (True, 16, 16, False)),
+    (3, 83, 50, 1, (True, 16, 16, False)),
+    (3, 9, 50, 1, (True, 16, 16, False)),
+    (5, 4112, 33, 4, (True, 16, 16, False)),
+    (5, 64, 1033, 4, (True, 16, 32, False)),
+    (1, 68, 4100, 1, (True, 16, 32, False)),
+    (1, 67, 4101, 1, (True, 16, 32, False)),
+    (100, 64, 520, 4, (True, 32, 16, False)),
+    (20, 68, 2050, 1, (True, 32, 16, False)),
+    (20, 67, 2051, 1, (True, 32, 16, False)),
+    (200, 64, 520, 4, (True, 32, 32, False)),
+    (20, 68, 4097, 1, (True, 32, 32, False)),
+    (20, 67, 4100, 1, (True, 32, 32, False)),
+    (130, 64, 1030, 4, (True, 64, 32, False)),
+    (33, 68, 4100, 1, (True, 64, 32, False)),
+    (33, 67, 4099, 1, (True, 64, 32, False)),
+    (70, 336, 4100, 1, (False, 64, 64, False)),
+    (400, 80, 2049, 3, (False, 64, 64, False)),
+    (16400, 80, 70, 1, (False, 64, 64, False)),
+    (64, 4112, 4099, 1, (False, 64, 64, False)),
+    (8200, 80, 130, 1, (False, 64, 64, False)),
+    (70, 339, 4100, 1, (False, 64, 64, False)),
+    (64, 643, 4100, 3, (False, 64, 64, False)),
+    (260, 2051, 1030, 1, (False, 64, 64, True)),
+    (1030, 339, 4100, 1, (False, 64, 64, True)),
+    (70, 80, 8200, 1, (False, 64, 128, False)),
+    (1030, 1040, 2050, 1, (False, 128, 128, False)),
+    (400, 80, 8199, 3, (False, 64, 128, False)),
+    (70, 339, 8200, 1, (False, 64, 128, False)),
+    (64, 339, 8200, 3, (False, 64, 128, False)),
+    (1030, 2051, 1030, 1, (False, 64, 128, True)),
+    (1003, 2051, 1537, 1, (False, 64, 128, True)),
+    (4100, 643, 2050, 4, (False, 64, 128, True)),
+    (16400, 336, 70, 1, (False, 128, 128, False)),
+    (700, 80, 4100, 3, (False, 128, 128, False)),
+    (700, 656, 2050, 1, (False, 64, 128, False)),
+    (16400, 339, 70, 1, (False, 128, 128, False)),
+    (200, 339, 8200, 3, (False, 128, 128, False)),
+    (1030, 643, 2050, 1, (False, 128, 128, True)),
+    (8200, 67, 6150, 4, (False, 128, 128, True)),
+    (700, 80, 8200, 3, (False, 128, 256, False)),
+    (1030, 80, 6151, 1, (False, 128, 256, False)),
+    (700, 339, 8200, 3, (False, 128, 256, False)),
+    (1030, 2051, 6150, 1, (False, 128, 256, True)),
+    (4100, 67, 16400, 4, (False, 128, 256, True)),
+    (700, 1040, 16397, 1, (False, 256, 256, False)),
+    (2050, 1040, 6150, 4, (False, 256, 256, False)),
+    (2050, 643, 6150, 1, (False, 256, 256, True)),
 ]
 
 
@@ -32,8 +67,15 @@ def test_the_plan(rows, c, k, experts, plan):
     assert M.plan_row8_linear(rows, c, k, experts) == plan
 
 
+def test_every_tile_is_among_them():
+    plans = {c[4] for c in CASES}
+    few = {(True, r, k, False) for r, k in ((16, 16), (16, 32), (32, 16), (32, 32), (64, 32))}
+    tiles = {(False, r, k, p) for r, k in ((64, 64), (64, 128), (128, 128), (128, 256)) for p in (False, True)}
+    assert plans == few | tiles | {(False, 256, 256, False), (False, 256, 256, True)}
+
+
 def test_plans_of_nothing_and_refused():
-    assert M.plan_row8_linear(0, 64, 64) == (False, 0, 0) == M.plan_row8_linear(64, 64, 0)
+    assert M.plan_row8_linear(0, 64, 64) == (False, 0, 0, False) == M.plan_row8_linear(64, 64, 0)
     assert M.plan_row8_linear(64, 0, 64)[0]
     with pytest.raises(M.MiqError, match="131071"):
         M.plan_row8_linear(1, 131072, 1)

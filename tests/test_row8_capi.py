@@ -20,9 +20,9 @@ BACK = dict(dy=P, x=P, gain=P, dsum=P, dx=P, dgain=P, rows=4, c=8, ld_dy=8, ld_x
 ACT = dict(x=P, codes=P, scales=P, rows=4, c=8, ld_x=8, act=2, gated=0, type=0, stream=None)
 EXPAND = dict(codes=P, scales=P, y=P, rows=4, c=8, ld_y=8, type=0, stream=None)
 LINEAR = dict(codes=P, scales=P, w_codes=P, w_scales=P, bias=P, add=P, y=P, rows=4, c=8, k=8, ld_add=8, ld_y=8, type=0,
-              stream=None)
+              ws=P, ws_bytes=BIG, stream=None)
 EXPERTS = dict(codes=P, scales=P, w_codes=P, w_scales=P, bias=P, offsets=P, index=P, y=P, x_rows=4, rows=4, c=8, k=8,
-               experts=2, ld_y=8, type=0, stream=None)
+               experts=2, ld_y=8, type=0, ws=P, ws_bytes=BIG, stream=None)
 PLAN = dict(ids=P, offsets=P, rows=P, places=P, tokens=4, slots=2, experts=3, id_type=2, stream=None)
 JOIN = dict(y=P, places=P, share=P, add=P, out=P, rows=4, tokens=4, slots=2, c=8, ld_y=8, ld_add=8, ld_out=8, type=0,
             stream=None)
@@ -87,6 +87,12 @@ REFUSED = [
     ("miq_row8_linear", LINEAR, dict(y=None), NULL, "output"),
     ("miq_row8_linear", LINEAR, dict(bias=P + 2), BAD, "aligned"),
     ("miq_row8_linear", LINEAR, dict(add=P + 1, type=1), BAD, "aligned"),
+    ("miq_row8_linear", LINEAR, dict(ws=P + 8), BAD, "16 bytes"),
+    ("miq_row8_linear", LINEAR, dict(rows=8192, c=2001, k=4096, ld_add=4096, ld_y=4096, ws=None), NULL, "workspace"),
+    ("miq_row8_linear", LINEAR, dict(rows=8192, c=2001, k=4096, ld_add=4096, ld_y=4096, ws_bytes=8), BAD, "smaller"),
+    ("miq_row8_experts", EXPERTS, dict(rows=8192, x_rows=8192, c=2001, k=4096, ld_y=4096, ws=None), NULL, "workspace"),
+    ("miq_row8_experts", EXPERTS, dict(rows=8192, x_rows=8192, c=2001, k=4096, ld_y=4096, ws_bytes=8), BAD, "smaller"),
+    ("miq_row8_experts", EXPERTS, dict(ws=P + 4), BAD, "16 bytes"),
     ("miq_row8_experts", EXPERTS, dict(experts=0), BAD, "4096"),
     ("miq_row8_experts", EXPERTS, dict(experts=4097), BAD, "4096"),
     ("miq_row8_experts", EXPERTS, dict(x_rows=-1), BAD, "x_rows"),
@@ -146,6 +152,13 @@ def test_workspace_sizes():
     assert M.rms_bprop_workspace_size(1, 5) == 20
     assert M.rms_bprop_workspace_size(1 << 30, 4096) == 512 * 4096 * 4
     assert M.rms_bprop_workspace_size(1 << 17, 1 << 29) == 1 << 31
+    assert M.row8_workspace_size(8192, 8192, 2000, 4096) == 0 == M.row8_workspace_size(4, 4, 2001, 4096)
+    assert M.row8_workspace_size(8192, 8192, 2001, 4096) == (8192 + 4096) * 2048
+    assert M.row8_workspace_size(100, 8192, 2001, 4096, 3) == (100 + 3 * 4096) * 2048
+    assert M.row8_workspace_size(0, 8192, 2001, 4096) == 0 == M.row8_workspace_size(10, 0, 2001, 4096)
+    with pytest.raises(M.MiqError, match="x_rows"):
+        M.row8_workspace_size(-1, 1, 1, 1)
+    assert M.lib().miq_row8_workspace_size(1, 1, 1, 1, 1, None) == NULL
     with pytest.raises(M.MiqError, match="2\\^46"):
         M.rms_bprop_workspace_size(1 << 40, 1 << 10)
     assert M.lib().miq_rms_bprop_workspace_size(1, 1, None) == NULL
