@@ -14,8 +14,7 @@
 namespace miq {
 namespace {
 
-constexpr int kParts = 512;                // workgroups, and rows of the workspace, at most
-constexpr int64_t kWorkspace = 1 << 25;  // values of it, while that leaves a workgroup
+constexpr int64_t kWorkspace = 1 << 25;  // values of the workspace, while that leaves a workgroup
 
 // 16 bytes of a row as they lie in memory, zeros past its end.
 template <typename T>
@@ -234,14 +233,25 @@ __global__ __launch_bounds__(1024) void rms_grad_join_kernel(const float* __rest
   }
 }
 
-// Workgroups, each with a row of the workspace: two a CU while there are rows for them.
-int64_t parts_of(int64_t rows, int64_t c) {
-  return std::min({rows, static_cast<int64_t>(kParts), std::max<int64_t>(kWorkspace / c, 1)});
+// Four waves on rows of up to 2048 bf16 or 1024 fp32: their registers leave room for the next row's values
+// of five workgroups a CU (a wave a row leaves room for two: 67 us for the 54 of 16384 x 2048).
+RowShape shape_of(int64_t c, int wide, int64_t rows) {
+  const RowShape s = row_shape(c, wide, rows);
+  return s.threads == 64 && s.runs == 4 ? RowShape{256, 1} : s;
+}
+
+// Workgroups, each with a row of the workspace: as many as the CUs hold at once (a fifth more of them would
+// take a third longer), while there are rows for them.
+int64_t parts_of(int64_t rows, int64_t c, int wide) {
+  const RowShape s = shape_of(c, wide, rows);
+  const int64_t per_cu = s.threads == 1024 ? 1 : (s.runs == 1 ? 5 : (s.runs == 2 ? 3 : 2));
+  const int64_t at_once = s.threads == 64 ? 4 : 1;  // rows of a workgroup
+  return std::min({(rows + at_once - 1) / at_once, 256 * per_cu, std::max<int64_t>(kWorkspace / c, 1)});
 }
 
 template <typename T, typename G>
 void launch(const RmsGradArgs& a, int64_t parts, hipStream_t stream) {
-  by_shape(row_shape(a.c, kWide<T>, a.rows), [&](auto threads, auto runs) {
+  by_shape(shape_of(a.c, kWide<T>, a.rows), [&](auto threads, auto runs) {
     constexpr int THREADS = threads.value, V = runs.value;
     if constexpr (V == 0) {
       rms_grad_long_kernel<T, G><<<static_cast<unsigned>(parts), 1024, 0, stream>>>(a);
@@ -253,10 +263,10 @@ void launch(const RmsGradArgs& a, int64_t parts, hipStream_t stream) {
 
 }  // namespace
 
-size_t rms_grad_workspace_bytes(int64_t rows, int32_t c) { return static_cast<size_t>(parts_of(rows, c)) * c * sizeof(float); }
+size_t rms_grad_workspace_bytes(int64_t rows, int32_t c) { return static_cast<size_t>(std::max(parts_of(rows, c, 8), parts_of(rows, c, 4))) * c * sizeof(float); }
 
 hipError_t launch_rms_grad(const RmsGradArgs& a, hipStream_t stream) {
-  const int64_t parts = parts_of(a.rows, a.c);
+  const int64_t parts = parts_of(a.rows, a.c, a.bf16 ? 8 : 4);
   if (parts > 0) {
     if (a.bf16) a.gain_bf16 ? launch<__bf16, __bf16>(a, parts, stream) : launch<__bf16, float>(a, parts, stream);
     else a.gain_bf16 ? launch<float, __bf16>(a, parts, stream) : launch<float, float>(a, parts, stream);
