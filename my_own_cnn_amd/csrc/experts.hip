@@ -19,20 +19,21 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(ExpertsPlanA
   const int64_t each = (runs + kPlanWaves - 1) / kPlanWaves;
   const int64_t from = min(wave * each, runs) * 64;
   const int64_t to = min((wave + 1) * each, runs) * 64;
-  // four runs of 64 at a time, loaded together
-  auto load = [&](int64_t base, ID (&id)[4]) {
+  // eight runs of 64 at a time, loaded together
+  constexpr int kRuns = 8;
+  auto load = [&](int64_t base, ID (&id)[kRuns]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRuns; ++u) {
       const int64_t i = base + u * 64 + lane;
       id[u] = i < to && i < a.n ? ids[i] : -1;
     }
   };
   int less = 0, same = 0;
-  for (int64_t base = from; base < to; base += 256) {
-    ID id[4];
+  for (int64_t base = from; base < to; base += 64 * kRuns) {
+    ID id[kRuns];
     load(base, id);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRuns; ++u) {
       less += id[u] >= 0 && id[u] < expert;
       same += id[u] == expert;
     }
@@ -53,11 +54,11 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(ExpertsPlanA
     count += own[w];
   }
   at += start;
-  for (int64_t base = from; base < to; base += 256) {
-    ID id[4];
+  for (int64_t base = from; base < to; base += 64 * kRuns) {
+    ID id[kRuns];
     load(base, id);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRuns; ++u) {
       const int64_t i = base + u * 64 + lane;
       const uint64_t mine = __ballot(id[u] == expert);
       if (mine >> lane & 1) {

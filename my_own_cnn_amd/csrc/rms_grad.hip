@@ -245,7 +245,7 @@ RowShape shape_of(int64_t c, int wide, int64_t rows) {
 int64_t parts_of(int64_t rows, int64_t c, int wide) {
   const RowShape s = shape_of(c, wide, rows);
   const int64_t per_cu = s.threads == 1024 ? 1 : (s.runs == 1 ? 5 : (s.runs == 2 ? 3 : 2));
-  const int64_t at_once = s.threads == 64 ? 4 : 1;  // rows of a workgroup
+  const int64_t at_once = s.threads < 256 ? 256 / s.threads : 1;  // rows of a workgroup
   return std::min({(rows + at_once - 1) / at_once, 256 * per_cu, std::max<int64_t>(kWorkspace / c, 1)});
 }
 

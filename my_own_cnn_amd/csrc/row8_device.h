@@ -20,18 +20,18 @@ __device__ __forceinline__ void zero(V (&v)[N]) {
   for (int i = 0; i < N; ++i) v[i] = V{};
 }
 
-// The sums of `a` and `b` and the largest `top` over the THREADS that hold a row: a wave, or a whole
-// workgroup, which meets once.  `turn` alternates between rows, so that a wave that is a row ahead
+// The sums of `a` and `b` and the largest `top` over the THREADS that hold a row: a quarter, a half or all of a
+// wave, or a whole workgroup, which meets once.  `turn` alternates between rows, so that a wave that is a row ahead
 // writes where nobody reads any more.
 template <int THREADS>
 struct RowSums {
-  static constexpr int kWaves = THREADS / 64;
+  static constexpr int kWaves = THREADS > 64 ? THREADS / 64 : 1;
   float a[2][kWaves], b[2][kWaves];
   unsigned top[2][kWaves];
 };
 template <int THREADS>
 __device__ __forceinline__ void reduce_row(RowSums<THREADS>& lds, int turn, float* a, float* b, unsigned* top) {
-  for (int step = 1; step < 64; step *= 2) {
+  for (int step = 1; step < (THREADS < 64 ? THREADS : 64); step *= 2) {
     if (a != nullptr) *a += __shfl_xor(*a, step);
     if (b != nullptr) *b += __shfl_xor(*b, step);
     if (top != nullptr) *top = max(*top, static_cast<unsigned>(__shfl_xor(static_cast<int>(*top), step)));
@@ -74,6 +74,8 @@ struct RowShape {
 // The fewest threads that leave a thread few runs; runs == 0: more than registers hold.
 inline RowShape row_shape(int64_t c, int wide, int64_t rows) {
   const int64_t n = (c + wide - 1) / wide;
+  if (n <= 16) return {16, 1};
+  if (n <= 32) return {32, 1};
   if (n <= 64) return {64, 1};
   if (n <= 128) return {64, 2};
   if (n <= 256) return rows >= 1024 ? RowShape{64, 4} : RowShape{256, 1};
@@ -86,7 +88,11 @@ inline RowShape row_shape(int64_t c, int wide, int64_t rows) {
 template <typename F>
 void by_shape(const RowShape& s, F&& go) {
   using std::integral_constant;
-  if (s.threads == 64) {
+  if (s.threads == 16) {
+    go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  } else if (s.threads == 32) {
+    go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  } else if (s.threads == 64) {
     if (s.runs == 1) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (s.runs == 2) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
     else go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
@@ -101,9 +107,9 @@ void by_shape(const RowShape& s, F&& go) {
   }
 }
 
-// Workgroups (of at least 256 threads, a wave a row where THREADS is 64) of a kernel that loops over rows.
+// Workgroups (of at least 256 threads) of a kernel that loops over rows.
 inline unsigned row_blocks(const RowShape& s, int64_t rows, int64_t most) {
-  const int64_t per = s.threads == 64 ? 4 : 1;
+  const int64_t per = s.threads < 256 ? 256 / s.threads : 1;
   const int64_t blocks = (rows + per - 1) / per;
   return static_cast<unsigned>(blocks < most ? blocks : most);
 }
