@@ -257,23 +257,28 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void row8_tile_kernel(Row8LinearArg
   wait_vmcnt(0);  // no load into LDS outlives the workgroup
 
   if constexpr (!kEarly) load_scales();
+  typename Vec<W>::type bias[U] = {};
+  if (a.bias != nullptr) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int k = k0 + u * 4 * W, left = a.k - k;
-    if (left <= 0) continue;
-    typename Vec<W>::type bias = {};
-    if (a.bias != nullptr) bias = load_floats<W>(a.bias + w_of0 + k, left);
+    for (int u = 0; u < U; ++u) bias[u] = load_floats<W>(a.bias + w_of0 + k0 + u * 4 * W, a.k - (k0 + u * 4 * W));
+  }
+  // row by row, so that the halves of a line are written one after the other
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int row = (wm * FM + j) * 16 + f_row;
-      if (row >= rows) continue;
+  for (int j = 0; j < FM; ++j) {
+    const int row = (wm * FM + j) * 16 + f_row;
+    if (row >= rows) continue;
+    T* const y = static_cast<T*>(a.y) + (r.row0 + row) * a.ld_y + k0;
+    const T* const add = static_cast<const T*>(a.add) + (r.row0 + row) * a.ld_add + k0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int left = a.k - (k0 + u * 4 * W);
+      if (left <= 0) continue;
       typename Vec<W>::type v;
 #pragma unroll
       for (int i = 0; i < W; ++i) v[i] = scaled(acc[(u * W + i) / 4][j][i % 4], x_scale[j], w_scale[u][i]);
-      if (a.bias != nullptr) v += bias;
-      const int64_t y_row = r.row0 + row;
-      if (a.add != nullptr) v += load_some<false>(static_cast<const T*>(a.add) + y_row * a.ld_add + k, left);
-      store_some<false>(static_cast<T*>(a.y) + y_row * a.ld_y + k, v, left);
+      if (a.bias != nullptr) v += bias[u];
+      if (a.add != nullptr) v += load_some<false>(add + u * 4 * W, left);
+      store_some<false>(y + u * 4 * W, v, left);
     }
   }
 }
