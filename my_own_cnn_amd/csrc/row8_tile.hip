@@ -56,7 +56,7 @@ __device__ __forceinline__ int row_tiles(const Row8LinearArgs& a, const Tiling& 
   return min(tiling.high, count_tiles(a.offsets, a.experts, a.rows, BM) - tiling.from);
 }
 
-template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES>
+template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES, bool STREAM>
 __global__ __launch_bounds__(WM* WN * 64, 2) void row8_tile_kernel(Row8LinearArgs a, Tiling tiling) {
   constexpr int kWaves = WM * WN;
   constexpr int NX = BM / 8 / kWaves, NW = BN / 8 / kWaves;  // runs of 8 rows that a wave stages
@@ -278,15 +278,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void row8_tile_kernel(Row8LinearArg
       for (int i = 0; i < W; ++i) v[i] = scaled(acc[(u * W + i) / 4][j][i % 4], x_scale[j], w_scale[u][i]);
       if (a.bias != nullptr) v += bias[u];
       if (a.add != nullptr) v += load_some<false>(add + u * 4 * W, left);
-      store_some<false>(y + u * 4 * W, v, left);
+      store_some<STREAM>(y + u * 4 * W, v, left);
     }
   }
 }
 
-template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES>
+template <typename T, bool DMA, int BM, int BN, int WM, int WN, int STAGES, bool STREAM = false>
 hipError_t launch(const Row8LinearArgs& a, int wide, int64_t high, hipStream_t stream) {
   constexpr int kSize = STAGES * (BM + BN) * kStep;
-  auto* const kernel = row8_tile_kernel<T, DMA, BM, BN, WM, WN, STAGES>;
+  auto* const kernel = row8_tile_kernel<T, DMA, BM, BN, WM, WN, STAGES, STREAM>;
   if (kSize > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, kSize);
@@ -310,8 +310,12 @@ hipError_t by_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t 
   if constexpr (DMA) {
     // Few tiles: as many steps in flight as LDS holds for the one or two workgroups of a CU.
     const bool few = high * wide <= 512, one = high * wide <= 256;
+    // a large y past the caches: 16384 x 2048 x 8192 281 -> 255 us, 16384 x 4096 x 8192 the same
+    const bool past = channels == 256 && stream_stores(a.y, a.rows, a.k, a.ld_y, sizeof(T));
+    if (rows == 256 && past) return launch<T, DMA, 256, 256, 2, 4, 2, true>(a, wide, high, stream);
     if (rows == 256) return launch<T, DMA, 256, 256, 2, 4, 2>(a, wide, high, stream);
-    if (rows == 128 && channels == 256) return launch<T, DMA, 128, 256, 2, 4, 3>(a, wide, high, stream);
+    if (channels == 256 && past) return launch<T, DMA, 128, 256, 2, 4, 3, true>(a, wide, high, stream);
+    if (channels == 256) return launch<T, DMA, 128, 256, 2, 4, 3>(a, wide, high, stream);
     if (rows == 128 && one) return launch<T, DMA, 128, 128, 2, 2, 4>(a, wide, high, stream);
     if (rows == 128) return launch<T, DMA, 128, 128, 2, 2, 2>(a, wide, high, stream);
     if (channels == 128 && few) return launch<T, DMA, 64, 128, 2, 2, 3>(a, wide, high, stream);

@@ -121,3 +121,17 @@ def test_products(device, rows, c, k, experts, plan, kind):
             src = at if of is None else of[at].long()
             want = _want(x[src], w[e], xs[src], ws[e], bias[e] if with_bias else None, None, kind)
             assert torch.equal(got[cuts[e]: cuts[e + 1]], want), (e, of is None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c,tile", [(144, 128), (656, 256)])
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_a_large_output(device, c, tile, kind):
+    """One that is written past the caches; the last rows and channels of ragged tiles."""
+    g = torch.Generator(device=device).manual_seed(5)
+    rows, k = 16100, 8192
+    assert M.plan_row8_linear(rows, c, k)[:3] == (False, tile, 256)
+    x, w = _codes(g, rows, c), _codes(g, k, c)
+    xs, ws = torch.rand(rows, generator=g, device=device), torch.rand(k, generator=g, device=device)
+    got = M.row8_linear(M.Row8(x, xs), M.Row8(w, ws), dtype=kind)
+    assert torch.equal(got, _want(x, w, xs, ws, None, None, kind))
