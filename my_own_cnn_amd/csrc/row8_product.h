@@ -46,8 +46,10 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int experts
     const uint64_t past = __ballot(upto > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      const int row0 = __shfl(e.lo, at) + (tile - (__shfl(upto, at) - __shfl(e.tiles, at))) * high;
-      const int last = __shfl(e.hi, at), end = last - row0 < high ? last : row0 + high;
+      const int first = __shfl(e.lo, at), last = __shfl(e.hi, at);
+      const int row0 = first + (tile - (__shfl(upto, at) - __shfl(e.tiles, at))) * high;
+      if (row0 < first || row0 >= last) return {-1, 0, 0};  // only where offsets fall
+      const int end = last - row0 < high ? last : row0 + high;
       return {__builtin_amdgcn_readfirstlane(base + at), __builtin_amdgcn_readfirstlane(row0),
               __builtin_amdgcn_readfirstlane(end)};
     }

@@ -79,6 +79,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void row8_tile_kernel(Row8LinearArg
   if (static_cast<int>(blockIdx.x) >= high * tiling.wide) return;
   const Place place = place_of<BM, BN>(a, tiling, high, blockIdx.x);
   const RowTile r = place.r;
+  if (r.expert < 0) return;
   const int n0 = place.n0, rows = r.end - r.row0, channels = min(BN, a.k - n0);
 
   // The output stage takes U runs of a lane's channels of each row, W values each.  Its scales are loaded first,
