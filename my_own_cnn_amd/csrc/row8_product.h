@@ -46,12 +46,13 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* offsets, int experts
     const uint64_t past = __ballot(upto > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      const int first = __shfl(e.lo, at), last = __shfl(e.hi, at);
-      const int row0 = first + (tile - (__shfl(upto, at) - __shfl(e.tiles, at))) * high;
+      // Uniform before the branch: a tile whose rows might differ by lane puts every load of the product in a loop.
+      const int first = __builtin_amdgcn_readfirstlane(__shfl(e.lo, at));
+      const int last = __builtin_amdgcn_readfirstlane(__shfl(e.hi, at));
+      const int before = __builtin_amdgcn_readfirstlane(__shfl(upto, at) - __shfl(e.tiles, at));
+      const int row0 = first + (__builtin_amdgcn_readfirstlane(tile) - before) * high;
       if (row0 < first || row0 >= last) return {-1, 0, 0};  // only where offsets fall
-      const int end = last - row0 < high ? last : row0 + high;
-      return {__builtin_amdgcn_readfirstlane(base + at), __builtin_amdgcn_readfirstlane(row0),
-              __builtin_amdgcn_readfirstlane(end)};
+      return {base + at, row0, last - row0 < high ? last : row0 + high};
     }
     tile -= __shfl(upto, 63);
   }
