@@ -3,10 +3,12 @@
 //
 // A workgroup computes 16 * MT rows by 16 * NT channels.  Its eight waves share the reduction: wave w takes
 // steps w, w + 8, ... of 64 codes, straight from global memory into the operands of its matrix
-// instructions, U steps in flight; their sums meet in LDS at the end.
+// instructions, U steps in flight; their sums meet in LDS at the end.  U leaves registers for two workgroups a
+// CU (four steps of 16 x 32, 108 registers), so one's search for its rows and its sums hide behind the other's
+// loads: with eight (156) the 16 rows below took 22 us.
 //
 // Bound by the weights: one row by 4096 x 4096 (16.8 MB) 6.2 us, 2 of them the launch; 14 of 64 experts' 2048 x
-// 2048 for 16 rows (59 MB) 18.5 us.  With more rows by what a CU takes in, 38 KB a us in segments of 64 bytes:
+// 2048 for 16 rows (59 MB) 17 us.  With more rows by what a CU takes in, 38 KB a us in segments of 64 bytes:
 // 64 rows by 8192 x 4096 15 us, where tiles take 9.
 #include "row8_product.h"
 
@@ -126,7 +128,7 @@ hipError_t launch(const Row8LinearArgs& a, hipStream_t stream) {
 
 template <typename T, bool ODD>
 hipError_t by_tile(const Row8LinearArgs& a, int rows, int channels, hipStream_t stream) {
-  if (rows == 16) return channels == 16 ? launch<T, ODD, 1, 1, 8>(a, stream) : launch<T, ODD, 2, 1, 8>(a, stream);
+  if (rows == 16) return channels == 16 ? launch<T, ODD, 1, 1, 8>(a, stream) : launch<T, ODD, 2, 1, 4>(a, stream);
   if (rows == 32) return channels == 16 ? launch<T, ODD, 1, 2, 4>(a, stream) : launch<T, ODD, 2, 2, 4>(a, stream);
   return launch<T, ODD, 2, 4, 4>(a, stream);
 }
