@@ -8,8 +8,9 @@
 // the rows that a workgroup takes.  The workgroups' sums go to the workspace and are added by a second
 // launch, both in an order fixed by the sizes.
 //
-// Bound by memory: 16384 x 2048 bf16 with dsum (268 MB) 54 us, 5.0 TB/s, and 4.8 us for the sum of 1280 rows of
-// the workspace.  One row after another without loads ahead 90 us; a wave a row with them 67.
+// Bound by memory: 16384 x 2048 bf16 with dsum (268 MB) and the sum of 768 rows of the workspace 53 us a call,
+// without dsum 49.  With x and dy loaded when their row comes and not a row ahead 58 and 52, 8192 x 4096 65 (56
+// ahead), 16384 x 1000 38 (31).
 #include <algorithm>
 
 #include "row8_device.h"
@@ -67,7 +68,9 @@ __global__ __launch_bounds__(kRowBlock<THREADS>, THREADS == 1024 ? 4 : 2) void r
     g[j] = load_gain<W>(static_cast<const G*>(a.gain) + col, a.c - col);
     total[j] = Run{};
   }
-  // the next row's values travel while this one is summed
+  // The next row's values travel while this one is summed, where registers hold both: more than 16 values a thread (8
+  // of 1024 threads, which have 128 VGPRs each) would spill and are loaded when their row comes.
+  constexpr bool kAhead = V * W * (THREADS == 1024 ? 2 : 1) <= 16;
   typename RawOf<T>::type next_s[V], next_d[V], next_e[V];
   auto load = [&](int64_t row) {
 #pragma unroll
@@ -80,25 +83,20 @@ __global__ __launch_bounds__(kRowBlock<THREADS>, THREADS == 1024 ? 4 : 2) void r
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own;
-  if (row < a.rows) load(row);
+  if (kAhead && row < a.rows) load(row);
   int turn = 0;
   for (; row < a.rows; row += step) {
     Run s[V], d[V];
     typename RawOf<T>::type e[V];
+    if (!kAhead) load(row);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       s[j] = __builtin_convertvector(next_s[j], Run);
       d[j] = __builtin_convertvector(next_d[j], Run);
       e[j] = next_e[j];
     }
-    if (row + step < a.rows) load(row + step);
+    if (kAhead && row + step < a.rows) load(row + step);
     float squares = 0.0f, dot = 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int col = (j * THREADS + t) * W;
-      s[j] = load_some<false>(static_cast<const T*>(a.x) + row * a.ld_x + col, a.c - col);
-      d[j] = load_some<false>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.c - col);
-    }
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -236,19 +234,21 @@ __global__ __launch_bounds__(1024) void rms_grad_join_kernel(const float* __rest
   }
 }
 
-// Four waves on rows of 1025 to 2048 bf16: their registers leave room for the next row's values of five workgroups
-// a CU (a wave a row leaves room for two: 67 us for the 54 of 16384 x 2048).  fp32 rows of as many bytes
-// take half the registers and stay with a wave (5003 x 1001: 18 us with the sum of the workspace, 20 with four).
+// Four waves on rows of 1025 to 2048 bf16: a thread's 8 values leave room for the next row's, a wave's 32 a thread
+// do not.  16384 x 2048 with dsum 53 us, a wave a row 57; without dsum 49 and 44.  fp32 rows of as many bytes have 16
+// values a thread and stay with a wave (5003 x 1001 17 us, 18 with four).
 RowShape shape_of(int64_t c, int wide, int64_t rows) {
   const RowShape s = row_shape(c, wide, rows);
   return wide == 8 && s.threads == 64 && s.runs == 4 ? RowShape{256, 1} : s;
 }
 
-// Workgroups, each with a row of the workspace: as many as the CUs hold at once (a fifth more of them would
-// take a third longer), while there are rows for them.
+// Workgroups, each with a row of the workspace, while there are rows for them.  With the loads ahead few a CU keep
+// the memory busy, and more of them only add to the sum of the workspace: over 64 to 4096 channels of both types
+// with dsum 3 a CU took 1 to 11% less than 5 where a thread has one run, and 2 a CU 3 to 8% less than 3 where it
+// has more.
 int64_t parts_of(int64_t rows, int64_t c, int wide) {
   const RowShape s = shape_of(c, wide, rows);
-  const int64_t per_cu = s.threads == 1024 ? 1 : (s.runs == 1 ? 5 : (s.runs == 2 ? 3 : 2));
+  const int64_t per_cu = s.threads == 1024 ? 1 : (s.runs == 1 ? 3 : 2);
   const int64_t at_once = s.threads < 256 ? 256 / s.threads : 1;  // rows of a workgroup
   return std::min({(rows + at_once - 1) / at_once, 256 * per_cu, std::max<int64_t>(kWorkspace / c, 1)});
 }
