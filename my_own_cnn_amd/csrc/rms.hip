@@ -5,7 +5,8 @@
 //
 // A row stays in the registers of a wave or a workgroup between its one read and its one write.  For
 // 8-bit rows the codes need no r: the largest |s * gain| is found in the same pass as the sum of
-// squares, and a code is s * gain times 127 over it; only the row's scale is multiplied by r.
+// squares, and a code is s * gain times 127 over it; only the row's scale is multiplied by r.  Where
+// s * gain or the norm leaves 2^-110 .. infinity, the codes are those of s * r * gain, looked at once more.
 //
 // Bound by memory: 16384 x 4096 bf16 with an addend as 8-bit rows (470 MB) 95 us, 4.9 TB/s; 16384 x 2048 bf16
 // with an addend as real rows (268 MB) 53 us, 5.0 TB/s: a large copy's rate.  Rows of 64 channels share a
@@ -27,6 +28,13 @@ __device__ __forceinline__ typename Vec<W>::type load_gain(const G* p, int left)
       if (i < left) v[i] = static_cast<float>(p[i]);
     return v;
   }
+}
+
+// Whether codes of a row can be taken from s * gain, whose largest magnitude has the bits `top`: it and the norm's own
+// lie above the least one of a row and are finite.  False for rows with an infinity (r is 0) or a NaN.
+__device__ __forceinline__ bool in_range(unsigned top, float r) {
+  const float m = __uint_as_float(top), of_norm = m * r;
+  return m >= kLeastTop && top < 0x7f800000u && of_norm >= kLeastTop && __float_as_uint(of_norm) < 0x7f800000u;
 }
 
 // Values as the type holds them.
@@ -91,11 +99,22 @@ __global__ __launch_bounds__(kRowBlock<THREADS>) void rms_kernel(RmsArgs a) {
       turn ^= 1;
       eps = eps * kDown * kDown;
     }
-    const float r = inverse_rms(squares, a.c, eps);
+    float r = inverse_rms(squares, a.c, eps);
     if constexpr (CODES) {
+      if (!in_range(top, r)) {  // the same for all of the row's threads
+        top = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s[j] *= r;
+#pragma unroll
+          for (int i = 0; i < W; ++i) top = max(top, magnitude(s[j][i] * g[j][i]));
+        }
+        reduce_row<THREADS>(lds, turn, nullptr, nullptr, &top);
+        turn ^= 1;
+        r = 1.0f;
+      }
       const float m = fmaxf(__uint_as_float(top), kLeastTop);
-      // an infinity in s leaves r == 0, a NaN leaves NaN: neither row has codes
-      const bool bad = top >= 0x7f800000u || !(r > 0.0f);
+      const bool bad = top >= 0x7f800000u;
       const float inverse = 127.0f / m;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -126,7 +145,7 @@ __global__ __launch_bounds__(1024) void rms_long_kernel(RmsArgs a) {
     T* const sum = static_cast<T*>(a.sum) + row * a.ld_sum;
     const T* const from = ADD ? sum : x;
     const G* const gain = static_cast<const G*>(a.gain);
-    float squares = 0.0f, down = 1.0f, eps = a.eps;
+    float squares = 0.0f, down = 1.0f, by = 1.0f, eps = a.eps;  // codes are of s * down * by * gain
     unsigned top = 0;
     for (int again = 0; again < 2; ++again) {
       squares = 0.0f;
@@ -157,14 +176,28 @@ __global__ __launch_bounds__(1024) void rms_long_kernel(RmsArgs a) {
       down = kDown;
       eps = a.eps * kDown * kDown;
     }
-    const float r = inverse_rms(squares, a.c, eps);
+    float r = inverse_rms(squares, a.c, eps);
+    if (CODES && !in_range(top, r)) {  // the same for all of the row's threads
+      top = 0;
+      for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.c; at += kThreads * W) {
+        const int left = static_cast<int>(a.c - at);
+        const Run s = load_some<false>(from + at, left) * down * r;
+        const Run g = load_gain<W>(gain + at, left);
+#pragma unroll
+        for (int i = 0; i < W; ++i) top = max(top, magnitude(s[i] * g[i]));
+      }
+      reduce_row<kThreads>(lds, turn, nullptr, nullptr, &top);
+      turn ^= 1;
+      by = r;
+      r = 1.0f;
+    }
     const float m = fmaxf(__uint_as_float(top), kLeastTop), inverse = 127.0f / m;
-    const bool bad = top >= 0x7f800000u || !(r > 0.0f);
+    const bool bad = top >= 0x7f800000u;
     for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.c; at += kThreads * W) {
       const int left = static_cast<int>(a.c - at);
       const Run s = load_some<false>(from + at, left) * down;
       const Run g = load_gain<W>(gain + at, left);
-      if constexpr (CODES) store_codes<W>(a.codes + row * a.c + at, s * g, inverse, bad, left);
+      if constexpr (CODES) store_codes<W>(a.codes + row * a.c + at, s * by * g, inverse, bad, left);
       else store_some<false>(static_cast<T*>(a.y) + row * a.ld_y + at, s * r * g, left);
     }
     if (CODES && threadIdx.x == 0) a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : m * r / 127.0f;
