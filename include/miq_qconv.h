@@ -557,8 +557,9 @@ int miq_rms_bprop_workspace_size(int64_t rows, int32_t c, size_t* bytes);
 /* The backward pass of miq_rms_fprop at x (the sum, where it had an addend): with n = x / sqrt(mean(x^2) +
  * eps) and dn = dy * gain, dx = (dn - n * mean(dn * n)) / sqrt(mean(x^2) + eps), plus dsum (or NULL), the
  * gradient that reaches the sum by another way; and dgain = the sum over the rows of dy * n, added to
- * dgain where accumulate != 0.  The gradient of x and of add are both dx.  dy, x, dsum, dx: rows x c
- * of `type`; dgain: c of dgain_type.  rows == 0 gives a dgain of zeros. */
+ * dgain where accumulate != 0.  The gradient of x and of add are both dx.  Sums are fp32, and taken again over
+ * scaled values where they leave its range.  dy, x, dsum, dx: rows x c of `type`; dgain: c of dgain_type.
+ * rows == 0 gives a dgain of zeros. */
 int miq_rms_bprop(const void* dy, const void* x, const void* gain, const void* dsum, void* dx, void* dgain, int64_t rows,
                   int32_t c, int64_t ld_dy, int64_t ld_x, int64_t ld_dsum, int64_t ld_dx, float eps, int32_t accumulate,
                   int32_t type, int32_t gain_type, int32_t dgain_type, void* workspace, size_t workspace_bytes,

@@ -20,6 +20,10 @@ namespace {
 
 constexpr int64_t kWorkspace = 1 << 25;  // values of the workspace, while that leaves a workgroup
 
+// Whether the sum of dn * s over a row lost nothing that matters: it did not overflow, and what its terms lost below
+// the normal numbers is far below it.  Otherwise (zeros of dy among them) mean(dn * n) is summed over n / c.
+__device__ __forceinline__ bool in_range(float dot) { return fabsf(dot) > 1e-27f && fabsf(dot) < 1e38f; }
+
 // 16 bytes of a row as they lie in memory, zeros past its end.
 template <typename T>
 struct RawOf;
@@ -124,7 +128,17 @@ __global__ __launch_bounds__(kRowBlock<THREADS>, THREADS == 1024 ? 4 : 2) void r
       turn ^= 1;
     }
     const float r = inverse_rms(squares, a.c, eps);
-    const float along = dot * r / static_cast<float>(a.c);
+    float along = dot * r / static_cast<float>(a.c);
+    if (!in_range(dot)) {  // the same for all of the row's threads
+      const float each = r / static_cast<float>(a.c);
+      along = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < W; ++i) along += d[j][i] * g[j][i] * (s[j][i] * each);
+      reduce_row<THREADS>(lds, turn, &along, nullptr, nullptr);
+      turn ^= 1;
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int col = (j * THREADS + t) * W;
@@ -194,7 +208,20 @@ __global__ __launch_bounds__(1024) void rms_grad_long_kernel(RmsGradArgs a) {
       eps = a.eps * kDown * kDown;
     }
     const float r = inverse_rms(squares, a.c, eps);
-    const float along = dot * r / static_cast<float>(a.c);
+    float along = dot * r / static_cast<float>(a.c);
+    if (!in_range(dot)) {  // the same for all of the row's threads
+      const float each = r / static_cast<float>(a.c);
+      along = 0.0f;
+      for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.c; at += kThreads * W) {
+        const int left = static_cast<int>(a.c - at);
+        const Run s = load_some<false>(x + at, left) * down, d = load_some<false>(dy + at, left);
+        const Run g = load_gain<W>(gain + at, left);
+#pragma unroll
+        for (int i = 0; i < W; ++i) along += d[i] * g[i] * (s[i] * each);
+      }
+      reduce_row<kThreads>(lds, turn, &along, nullptr, nullptr);
+      turn ^= 1;
+    }
     for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.c; at += kThreads * W) {
       const int left = static_cast<int>(a.c - at);
       const Run n = load_some<false>(x + at, left) * down * r, d = load_some<false>(dy + at, left);
