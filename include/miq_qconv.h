@@ -546,7 +546,8 @@ int miq_rms_fprop(const void* x, const void* add, const void* gain, void* sum, v
                   int64_t ld_x, int64_t ld_add, int64_t ld_sum, int64_t ld_y, float eps, int32_t type,
                   int32_t gain_type, void* stream);
 
-/* miq_rms_fprop with y as 8-bit rows: of the norm in fp32, not rounded to `type`. */
+/* miq_rms_fprop with y as 8-bit rows: of the norm in fp32, not rounded to `type`.  c == 0 enqueues nothing
+ * (miq_act_row8 writes such rows' scales). */
 int miq_rms_row8(const void* x, const void* add, const void* gain, void* sum, int8_t* codes, float* scales, int64_t rows,
                  int32_t c, int64_t ld_x, int64_t ld_add, int64_t ld_sum, float eps, int32_t type, int32_t gain_type,
                  void* stream);

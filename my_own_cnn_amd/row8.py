@@ -144,6 +144,9 @@ def rms_row8(x, gain, *, add=None, eps: float = 1e-6, kept: Optional[Row8] = Non
     held = _new_row8(shape[:-1], c, x, kept, stream)
     status = lib().miq_rms_row8(x.data_ptr(), add_at, gain_at, total_at, held[0].data_ptr(), held[1].data_ptr(), rows, c,
                                 ld, ld_add, ld_total, eps, kind, gain_kind, _handle(x, stream))
+    if c == 0 and not status:  # rows of nothing: the entry point leaves their scales, this one writes the least
+        status = lib().miq_act_row8(None, None, held[1].data_ptr(), held[1].numel(), 0, 0, _act("none"), 0, kind,
+                                    _handle(x, stream))
     if status:
         check(status, "rms_row8")
     return held if add is None else (held, total)
