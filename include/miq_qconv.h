@@ -567,7 +567,8 @@ int miq_rms_bprop(const void* dy, const void* x, const void* gain, const void* d
                   void* stream);
 
 /* act(x) by rows of c, or act(gate) * up for gated rows [gate, up] of 2c, as 8-bit rows.  MIQ_ACT_NONE
- * makes 8-bit rows of x itself: of a layer's weights, k rows of c. */
+ * makes 8-bit rows of x itself: of a layer's weights, k rows of c.  A silu or gelu within 2^-126 (1 + |v|) of zero
+ * (v below -87 and -13) may read zero, whatever `up` is. */
 int miq_act_row8(const void* x, int8_t* codes, float* scales, int64_t rows, int32_t c, int64_t ld_x, int32_t act,
                  int32_t gated, int32_t type, void* stream);
 
