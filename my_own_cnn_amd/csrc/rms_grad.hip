@@ -8,9 +8,9 @@
 // the rows that a workgroup takes.  The workgroups' sums go to the workspace and are added by a second
 // launch, both in an order fixed by the sizes.
 //
-// Bound by memory: 16384 x 2048 bf16 with dsum (268 MB) and the sum of 768 rows of the workspace 53 us a call,
-// without dsum 49.  With x and dy loaded when their row comes and not a row ahead 58 and 52, 8192 x 4096 65 (56
-// ahead), 16384 x 1000 38 (31).
+// Bound by memory: 16384 x 2048 bf16 with dsum (268 MB) 49 us, 5.5 TB/s, and 4.7 us for the sum of 768 rows of the
+// workspace: 53 us a call, without dsum 49.  With x and dy loaded when their row comes and not a row ahead 58 and 52,
+// 8192 x 4096 65 (56 ahead), 16384 x 1000 38 (31).
 #include <algorithm>
 
 #include "row8_device.h"
